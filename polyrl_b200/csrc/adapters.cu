@@ -1,0 +1,322 @@
+// polyrl_b200 — what the adapters of a batch's rows add to a shared projection:
+//
+//   out[i, n] = s_l * sum_r B_l[n, r] * t_i[p(n) * rank + r]  (+ bias[n]) (+ res[i, n]),     t_i = A_l x_i,   l = ids[i]
+//
+// p(n) is the part of the fused projection that column n belongs to (query / key / value, or gate / up in blocks of 128).  A row without
+// an adapter gets bias and residual alone.  The shared product adds `out` to its fp32 sums before it rounds, so a result is rounded once
+// more than without adapters only in the small term: t and out are bf16 (relative 2^-9 each of what the adapter adds).
+//
+// plan   one block sorts the rows by adapter (stable, by counting) and cuts every adapter's rows into tiles.  One plan serves all
+//        projections of a step.
+// delta  a cluster of CTAs takes a tile.  Few rows: the adapter's weights are all there is to read, so each CTA takes a share of K in the
+//        first product and a share of N in the second and reads every weight once, 16 (8) bytes a lane, straight into the fragments of
+//        mma.m16n8k16; nothing goes through shared memory but t, which the CTAs sum in a fixed order over distributed shared memory.
+//        The lanes' k-indices (and the columns of the second product) are permuted so that a lane's fragments are contiguous in memory:
+//        both operands of a product use the same permutation, and sums do not mind.
+//        Ranks are a few dozen, so the products are bound by their operands' bytes and mma.sync keeps up; tcgen05 would want 128 rows of
+//        one adapter and a round trip through tensor memory, longer than the whole kernel at decode.
+#include "adapters.hpp"
+#include "common.cuh"
+
+namespace prl {
+
+// ------------------------------------------------------------------------------------------------------------ plan
+// Rows in passes of 1024: a warp ranks its rows among those of the same adapter by match, a scan over the 32 warps' counts does the rest.
+constexpr int kPlanThreads = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int tile_rows, int max_tiles,
+                                                            int32_t* __restrict__ order, AdapterTile* __restrict__ tiles, int32_t* __restrict__ num_tiles) {
+  extern __shared__ int32_t sm[];
+  const int G = L + 1;                               // the last group: no adapter
+  int32_t* at = sm;                                  // [G] where the group's next row goes
+  int32_t* tile_at = sm + G;                         // [G] its first tile
+  int32_t* per_warp = sm + 2 * G;                    // [32][G]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_behind();
+  for (int g = tid; g < G; g += kPlanThreads) at[g] = 0;
+  for (int i = tid; i < 32 * G; i += kPlanThreads) per_warp[i] = 0;
+  __syncthreads();
+  auto group_of = [&](int row) {
+    const int id = ids[row];
+    return id >= 0 && id < L ? id : L;
+  };
+  for (int i = tid; i < T; i += kPlanThreads) atomicAdd(&at[group_of(i)], 1);
+  __syncthreads();
+  if (warp == 0) {                                   // exclusive sums of rows and of tiles over the groups
+    int rows0 = 0, tiles0 = 0;
+    for (int g0 = 0; g0 < G; g0 += 32) {
+      const int g = g0 + lane, n = g < G ? at[g] : 0, nt = (n + tile_rows - 1) / tile_rows;
+      int rs = n, ts = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int r = __shfl_up_sync(0xffffffffu, rs, o), t = __shfl_up_sync(0xffffffffu, ts, o);
+        if (lane >= o) { rs += r; ts += t; }
+      }
+      if (g < G) {
+        const int first = rows0 + rs - n, t0 = tiles0 + ts - nt;
+        at[g] = first;
+        tile_at[g] = t0;
+        for (int k = 0; k < nt && t0 + k < max_tiles; ++k)
+          tiles[t0 + k] = AdapterTile{g < L ? g : -1, first + k * tile_rows, min(tile_rows, n - k * tile_rows), 0};
+      }
+      rows0 += __shfl_sync(0xffffffffu, rs, 31);
+      tiles0 += __shfl_sync(0xffffffffu, ts, 31);
+    }
+    if (lane == 0) *num_tiles = min(tiles0, max_tiles);
+  }
+  __syncthreads();
+  for (int i0 = 0; i0 < T; i0 += kPlanThreads) {
+    const int row = i0 + tid;
+    const int g = row < T ? group_of(row) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    if (g >= 0 && rank == 0) per_warp[warp * G + g] = __popc(same);
+    __syncthreads();
+    for (int k = tid; k < G; k += kPlanThreads) {    // counts -> places, and the group moves on
+      int p = at[k];
+      for (int w = 0; w < 32; ++w) {
+        const int c = per_warp[w * G + k];
+        per_warp[w * G + k] = p;
+        p += c;
+      }
+      at[k] = p;
+    }
+    __syncthreads();
+    if (g >= 0) order[per_warp[warp * G + g] + rank] = row;
+    __syncthreads();
+    for (int k = tid; k < 32 * G; k += kPlanThreads) per_warp[k] = 0;
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ delta
+constexpr int kDeltaThreads = 256, kDeltaWarps = 8;
+constexpr int kLowChunk = 64;                        // low-rank columns whose sums a warp holds at a time
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t map_shared(const void* p, uint32_t cta) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
+  return a;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
+// shared memory: partial sums [TM][R] fp32, those of the warps that split K [KW][TM][kLowChunk], t [TM][R + 8] bf16
+template <int TM>
+struct DeltaSmem {
+  static constexpr int KW = kDeltaWarps / (TM / 16);
+  static int bytes(int R) { return TM * R * 4 + KW * TM * kLowChunk * 4 + TM * (R + 8) * 2; }
+};
+
+template <int TM>
+__global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams p) {
+  constexpr int MT = TM / 16, KW = DeltaSmem<TM>::KW;
+  extern __shared__ __align__(16) uint8_t raw[];
+  const int R = p.parts * p.rank, ldt = R + 8;
+  float* part = reinterpret_cast<float*>(raw);
+  float* red = part + TM * R;
+  __nv_bfloat16* low = reinterpret_cast<__nv_bfloat16*>(red + KW * TM * kLowChunk);
+  __shared__ int32_t rows_sm[TM];
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, grp = lane >> 2;
+  const uint32_t cs = cluster_size(), rank = cluster_ctarank();
+  const int t = blockIdx.x / cs;
+  grid_behind();
+  if (t >= *p.num_tiles) return;
+  const AdapterTile tile = p.tiles[t];
+  if (tid < TM) rows_sm[tid] = tid < tile.rows ? p.order[tile.first + tid] : -1;
+  __syncthreads();
+
+  if (tile.adapter >= 0) {
+    // ---- t = A x over this CTA's share of K
+    const int mt = warp % MT, kw = warp / MT;
+    const int steps = p.K / 32, s0 = steps * rank / cs, s1 = steps * (rank + 1) / cs;
+    const int r0 = rows_sm[mt * 16 + grp], r1 = rows_sm[mt * 16 + grp + 8];
+    const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + static_cast<int64_t>(max(r0, 0)) * p.ldx + quad * 8;
+    const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + static_cast<int64_t>(max(r1, 0)) * p.ldx + quad * 8;
+    const int4 zero = make_int4(0, 0, 0, 0);
+    for (int c0 = 0; c0 < R; c0 += kLowChunk) {
+      const int nt = min(kLowChunk, R - c0) / 8;
+      const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<int64_t>(tile.adapter) * R + c0 + grp) * p.K + quad * 8;
+      float acc[8][4] = {};
+      const bool busy = mt * 16 < tile.rows;
+      if (busy) {
+#pragma unroll 2
+        for (int s = s0 + kw; s < s1; s += KW) {
+          const int4 u = r0 >= 0 ? __ldg(reinterpret_cast<const int4*>(x0 + s * 32)) : zero;
+          const int4 v = r1 >= 0 ? __ldg(reinterpret_cast<const int4*>(x1 + s * 32)) : zero;
+          int4 w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < nt) w[j] = __ldg(reinterpret_cast<const int4*>(a + static_cast<int64_t>(j) * 8 * p.K + s * 32));
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < nt) {
+              mma_bf16(acc[j], u.x, v.x, u.y, v.y, w[j].x, w[j].y);
+              mma_bf16(acc[j], u.z, v.z, u.w, v.w, w[j].z, w[j].w);
+            }
+        }
+      }
+      float* dst = red + (kw * TM + mt * 16 + grp) * kLowChunk + quad * 2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < nt) {
+          *reinterpret_cast<float2*>(dst + j * 8) = make_float2(acc[j][0], acc[j][1]);
+          *reinterpret_cast<float2*>(dst + 8 * kLowChunk + j * 8) = make_float2(acc[j][2], acc[j][3]);
+        }
+      __syncthreads();
+      for (int e = tid; e < TM * nt * 8; e += kDeltaThreads) {
+        const int m = e / (nt * 8), c = e % (nt * 8);
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) v += red[(k * TM + m) * kLowChunk + c];
+        part[m * R + c0 + c] = v;
+      }
+      __syncthreads();
+    }
+    // ---- the CTAs' sums, each for its share of the values, in the order of the ranks; scaled, rounded and given to all
+    const float scale = p.scales[tile.adapter];
+    if (cs > 1) cluster_sync_all();
+    const int pairs = tile.rows * (R / 2), e1 = pairs * (rank + 1) / cs;
+    for (int e = pairs * rank / cs + tid; e < e1; e += kDeltaThreads) {
+      const int m = e / (R / 2), c = e % (R / 2) * 2;
+      float2 v = make_float2(0.f, 0.f);
+      if (cs == 1) {
+        v = *reinterpret_cast<float2*>(part + m * R + c);
+      } else {
+        for (uint32_t k = 0; k < cs; ++k) {
+          const float2 q = ld_cluster_f2(map_shared(part + m * R + c, k));
+          v.x += q.x; v.y += q.y;
+        }
+      }
+      const uint32_t packed = pack_bf16(scale * v.x, scale * v.y);
+      if (cs == 1) {
+        *reinterpret_cast<uint32_t*>(low + m * ldt + c) = packed;
+      } else {
+        for (uint32_t k = 0; k < cs; ++k) st_cluster_u32(map_shared(low + m * ldt + c, k), packed);
+      }
+    }
+    if (cs > 1) cluster_sync_all();                  // after this nobody touches another CTA's shared memory
+    else __syncthreads();
+  }
+
+  // ---- out = t B^T (+ bias) (+ res) over this CTA's share of the columns, 32 at a time: a lane ends up with 8 consecutive ones
+  const int groups = p.N / 32, g1 = groups * (rank + 1) / cs;
+  const int ksteps = p.rank / 16;
+  for (int g = groups * rank / cs + warp; g < g1; g += kDeltaWarps) {
+    const int col = g * 32;
+    const int pt = p.interleaved ? (col >> 7) & 1 : (p.parts > 1 && col >= p.ends[0]) + (p.parts > 2 && col >= p.ends[1]);
+    int4 extra = make_int4(0, 0, 0, 0);
+    if (p.bias) extra = __ldg(reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.bias) + col + quad * 8));
+    int4 res[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = rows_sm[m * 16 + grp + 8 * h];
+        res[m][h] = p.res && row >= 0 ? ld_nc_v4(static_cast<const __nv_bfloat16*>(p.res) + static_cast<int64_t>(row) * p.ldr + col + quad * 8) : make_int4(0, 0, 0, 0);
+      }
+    float acc[MT][4][4] = {};
+    if (tile.adapter >= 0) {
+      const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<int64_t>(tile.adapter) * p.N + col + 8 * (grp >> 1) + (grp & 1)) * p.rank + quad * 4;
+      const __nv_bfloat16* tl = low + pt * p.rank + quad * 4;
+#pragma unroll 2
+      for (int k = 0; k < ksteps; ++k) {
+        uint2 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint2*>(b + 2 * j * p.rank + k * 16));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (MT > 1 && m * 16 >= tile.rows) break;
+          const uint2 u = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp) * ldt + k * 16);
+          const uint2 v = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp + 8) * ldt + k * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_bf16(acc[m][j], u.x, v.x, u.y, v.y, w[j].x, w[j].y);
+        }
+      }
+    }
+    const uint32_t ex[4] = {static_cast<uint32_t>(extra.x), static_cast<uint32_t>(extra.y), static_cast<uint32_t>(extra.z), static_cast<uint32_t>(extra.w)};
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = rows_sm[m * 16 + grp + 8 * h];
+        if (row < 0) continue;
+        const uint32_t rv[4] = {static_cast<uint32_t>(res[m][h].x), static_cast<uint32_t>(res[m][h].y), static_cast<uint32_t>(res[m][h].z),
+                                static_cast<uint32_t>(res[m][h].w)};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 e = unpack_bf16(ex[j]), r = unpack_bf16(rv[j]);
+          o[j] = pack_bf16(acc[m][j][2 * h] + e.x + r.x, acc[m][j][2 * h + 1] + e.y + r.y);
+        }
+        st_v4(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8,
+              make_int4(static_cast<int>(o[0]), static_cast<int>(o[1]), static_cast<int>(o[2]), static_cast<int>(o[3])));
+      }
+  }
+}
+
+template <int TM>
+static int run_delta(const DeltaParams& p, int ctas, cudaStream_t stream) {
+  const int smem = DeltaSmem<TM>::bytes(p.parts * p.rank);
+  auto kern = delta_kernel<TM>;
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles) * ctas);
+  cfg.blockDim = dim3(kDeltaThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  PRL_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+  PRL_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace prl
+
+extern "C" int prl_adapter_plan(const int32_t* ids, int T, int L, int tile_rows, int max_tiles, int32_t* order, void* tiles, int32_t* num_tiles, cudaStream_t stream) {
+  if (T <= 0 || L < 1 || L > prl::kPlanMaxAdapters || tile_rows < 1) return -1;
+  const int smem = 34 * (L + 1) * 4;
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(prl::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 34 * (prl::kPlanMaxAdapters + 1) * 4));
+  PRL_CUDA_CHECK(launch_behind(prl::plan_kernel, 1, prl::kPlanThreads, smem, stream, ids, T, L, tile_rows, max_tiles, order,
+                               static_cast<prl::AdapterTile*>(tiles), num_tiles));
+  PRL_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}
+
+// tile_rows 16 or 64, as the plan was made; ctas: of a tile's cluster, 0 = as many (8 at most) as leave about four for every SM
+extern "C" int prl_adapter_delta(const prl::DeltaParams* q, int tile_rows, int ctas, cudaStream_t stream) {
+  const prl::DeltaParams& p = *q;
+  if (p.max_tiles <= 0) return 0;
+  if (p.K <= 0 || p.K % 32 || p.N <= 0 || p.N % 32 || p.rank < 16 || p.rank % 16 || p.parts < 1 || p.parts > 3 || p.parts * p.rank > prl::kDeltaMaxLow) return -1;
+  if (ctas <= 0) {
+    ctas = 8;
+    while (ctas > 1 && static_cast<int64_t>(p.max_tiles) * ctas > 4 * 148) ctas >>= 1;
+  }
+  if (ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) return -2;
+  if (static_cast<int64_t>(p.max_tiles) * ctas > 0x7fffffff) return -3;
+  if (tile_rows == 16) return prl::run_delta<16>(p, ctas, stream);
+  if (tile_rows == 64) return prl::run_delta<64>(p, ctas, stream);
+  return -4;
+}

@@ -486,14 +486,19 @@ at::Tensor stream_gemm(const at::Tensor& x, const at::Tensor& w, const c10::opti
   const int B = x.size(0), K = x.size(1), N = w.size(0);
   TORCH_CHECK(w.size(1) == K && B <= 256 && K % 16 == 0);
   c10::cuda::CUDAGuard g(x.device());
-  const int n_out = mode == 1 ? N / 2 : N;
+  const int n_out = mode >= 1 ? N / 2 : N;          // 1: SwiGLU; 2: SwiGLU, `residual` [B, N] added before the activation
   at::Tensor out = out_opt.has_value() ? *out_opt : at::empty({B, n_out}, x.options().dtype(at::kBFloat16));
   CHECK_BF16(out);
   TORCH_CHECK(out.dim() == 2 && out.size(0) == B && out.size(1) == n_out && out.stride(1) == 1);
   const void* r = nullptr;
   if (residual.has_value()) {
     CHECK_BF16(*residual);
-    TORCH_CHECK(residual->dim() == 2 && residual->stride(1) == 1 && residual->stride(0) == out.stride(0) && residual->numel() == out.numel());
+    if (mode == 2) {
+      TORCH_CHECK(residual->dim() == 2 && residual->is_contiguous() && residual->size(0) == B && residual->size(1) == N &&
+                  (reinterpret_cast<uintptr_t>(residual->data_ptr()) & 15) == 0, "stream_gemm: [B, N] to add before the activation");
+    } else {
+      TORCH_CHECK(residual->dim() == 2 && residual->stride(1) == 1 && residual->stride(0) == out.stride(0) && residual->numel() == out.numel());
+    }
     r = residual->data_ptr();
   }
   const void* bs = nullptr;

@@ -2,6 +2,7 @@
 // attention, sampling and the sequence-mixer kernels.  Everything a rollout engine of a mixer stack needs is in this one
 // module, so a serving host builds it without the training and multi-GPU kernels of ``_C``.
 #include "bindings_common.hpp"
+#include "bindings_requests.hpp"
 #include "kv_manager.hpp"
 #include "scheduler.hpp"
 
@@ -15,6 +16,7 @@ int prl_paged_decode_workspace_floats(int, int, int, int);
 int prl_paged_decode(const void*, int64_t, const void*, const void*, const int32_t*, int64_t, const int32_t*, int, int, int, int, float, int, int, int, float*, void*, int64_t, cudaStream_t);
 int prl_gemm_clamped_glu_bf16(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, float, cudaStream_t);
 int prl_gemm_swiglu_bf16(const void*, const void*, void*, void*, int, int, int, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
+int prl_gemm_swiglu_add_bf16(const void*, const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
 int prl_gemm_experts_bf16(const void*, const void*, void*, const int32_t*, int, int, int, int, int, float, float, cudaStream_t);
 int prl_sink_decode(const void*, const void*, const void*, const int32_t*, int64_t, const int32_t*, int, int, int, int, int, float, int, const float*, float*, void*, cudaStream_t);
 int prl_map_attn_fwd(const void*, const void*, const void*, void*, const int32_t*, const int32_t*, int, int, int, int, int, int, int, int, int, float, int, const float*, float, float, int, cudaStream_t);
@@ -551,6 +553,21 @@ std::vector<at::Tensor> gemm_swiglu(const at::Tensor& a, const at::Tensor& wgu, 
   return {h};
 }
 
+// the same with `add` [M, N2] (layout of the weight's rows) on the projection before the activation
+at::Tensor gemm_swiglu_add(const at::Tensor& a, const at::Tensor& wgu, const at::Tensor& add) {
+  CHECK_BF16(a); CHECK_BF16(wgu); CHECK_BF16(add); CHECK_LASTDIM(a); CHECK_LASTDIM(wgu); CHECK_LASTDIM(add);
+  const int M = a.size(0), K = a.size(1), N2 = wgu.size(0);
+  TORCH_CHECK(wgu.size(1) == K && N2 % 256 == 0 && K % 8 == 0 && add.dim() == 2 && add.size(0) == M && add.size(1) == N2 && a.device() == wgu.device() &&
+              a.device() == add.device(), "gemm_swiglu_add: x [M, K], w [N, K], add [M, N]");
+  c10::cuda::CUDAGuard g(a.device());
+  at::Tensor h = at::empty({M, N2 / 2}, a.options());
+  if (M == 0) return h;
+  const at::Tensor ws = split_scratch(M > 128 ? prl_gemm2_ws_floats(M, N2, K) : 0, a);
+  check(prl_gemm_swiglu_add_bf16(a.data_ptr(), wgu.data_ptr(), add.data_ptr(), h.data_ptr(), M, N2, K, a.stride(0), wgu.stride(0), add.stride(0), h.stride(0),
+                                 split_ptr(ws), cur_stream()), "gemm_swiglu_add");
+  return h;
+}
+
 at::Tensor mix_silu_glu(const at::Tensor& gu, int64_t blk) {
   const int dt = dt_of(gu, "mix_silu_glu");
   TORCH_CHECK(gu.dim() == 2 && gu.is_contiguous() && blk > 0 && gu.size(1) % (2 * blk) == 0);
@@ -1036,6 +1053,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample", &sample, py::arg("logits"), py::arg("scales"), py::arg("seeds"), py::arg("greedy"), py::arg("inverse") = true);
   m.def("sample_topk_topp", &sample_topk_topp, py::arg("logits"), py::arg("scales"), py::arg("seeds"), py::arg("greedy"), py::arg("top_k"), py::arg("top_p"),
         py::arg("inverse") = true);
+  m.def("adjust_logits", &adjust_logits);
+  m.def("gemm_swiglu_add", &gemm_swiglu_add);
+  m.def("adapter_plan", &adapter_plan);
+  m.def("adapter_delta", &adapter_delta, py::arg("x"), py::arg("a"), py::arg("b"), py::arg("scales"), py::arg("plan"), py::arg("tile_rows"), py::arg("max_tiles"),
+        py::arg("widths"), py::arg("interleaved"), py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("ctas") = 0);
   m.def("mix_embed", &mix_embed);
   m.def("mix_norm_add_", &mix_norm_add_);
   m.def("mix_rms", &mix_rms);

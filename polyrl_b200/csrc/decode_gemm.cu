@@ -35,6 +35,7 @@ constexpr int kSgSmemBudget = 196 * 1024;
 struct StreamParams {
   __nv_bfloat16* out;          // [B, ldo]
   const __nv_bfloat16* res;    // optional residual [B, ldo]
+  const __nv_bfloat16* pre;    // SwiGLU: optional [B, N], in the order of the weight's rows, added before the activation
   const __nv_bfloat16* bias;   // optional [N]
   const float* x_scale;        // optional fp8: per batch row
   const float* w_scale;        // optional fp8: per weight row
@@ -275,10 +276,23 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
           }
         }
         const float xs = p.x_scale ? p.x_scale[b] : 1.f;
+        float pg[8], pu[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { pg[q] = 0.f; pu[q] = 0.f; }
+        if (p.pre) {
+          const __nv_bfloat16* pr = p.pre + static_cast<int64_t>(b) * p.N + (n0 >> 7) * 256 + (n0 & 127);
+          const int4 a4 = ld_nc_v4(pr), b4 = ld_nc_v4(pr + 128);
+          const int ga[4] = {a4.x, a4.y, a4.z, a4.w}, ua[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 gv = unpack_bf16(ga[q]), uv = unpack_bf16(ua[q]);
+            pg[2 * q] = gv.x; pg[2 * q + 1] = gv.y; pu[2 * q] = uv.x; pu[2 * q + 1] = uv.y;
+          }
+        }
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           if (p.swiglu) {
-            const float g = y[q] * xs, uu = u[q] * xs;
+            const float g = y[q] * xs + pg[q], uu = u[q] * xs + pu[q];
             y[q] = g / (1.f + __expf(-g)) * uu;
           } else {
             y[q] = y[q] * xs + bv[q];
@@ -367,7 +381,8 @@ static int launch_stream(const void* X, const void* W, StreamParams p, int64_t l
 
 using namespace prl;
 
-// mode: 0 = store (+bias, +residual), 1 = SwiGLU (W block-interleaved [128 gate | 128 up] per 256 rows, out is [B, N/2]).
+// mode: 0 = store (+bias, +residual), 1 = SwiGLU (W block-interleaved [128 gate | 128 up] per 256 rows, out is [B, N/2]), 2 = SwiGLU of the product
+// plus `res` [B, N] (layout of the weight's rows, contiguous).
 // dtype: 0 = bf16, 1 = fp8 e4m3 (x_scale per batch row, w_scale per weight row required).
 // splits: k-splits S per cluster (0 = auto).  pair: 1 = CTA pairs (cta_group::2, 256 weight rows per MMA, bf16 only),
 // 0 = single CTAs, -1 = auto (pairs whenever the shape allows).
@@ -377,14 +392,15 @@ extern "C" int prl_stream_gemm(const void* X, const void* W, void* out, const vo
   if (B <= 0 || B > 256) return -60;
   StreamParams p;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.res = static_cast<const __nv_bfloat16*>(res);
+  p.res = mode == 2 ? nullptr : static_cast<const __nv_bfloat16*>(res);
+  p.pre = mode == 2 ? static_cast<const __nv_bfloat16*>(res) : nullptr;
   p.bias = static_cast<const __nv_bfloat16*>(bias);
   p.x_scale = x_scale; p.w_scale = w_scale;
   p.ldo = ldo; p.B = B; p.N = N; p.K = K;
   p.BP = ((B + 15) / 16) * 16;
-  p.swiglu = mode == 1;
-  if (mode == 1 && N % 256 != 0) return -63;
-  const int n_out = mode == 1 ? N / 2 : N;
+  p.swiglu = mode >= 1;
+  if (p.swiglu && N % 256 != 0) return -63;
+  const int n_out = p.swiglu ? N / 2 : N;
   if (n_out % 8 != 0 || ldo % 8 != 0) return -65;
   const int block_k = dtype == 1 ? 128 : 64;
   const int num_kb = (K + block_k - 1) / block_k;

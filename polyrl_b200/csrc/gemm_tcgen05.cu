@@ -81,14 +81,37 @@ struct SwigluParams {
   __nv_bfloat16* H;      // [M, ldh]   N/2 columns
   __nv_bfloat16* GU;     // optional [M, ldgu]  N columns (same interleaved layout as the weight rows)
   int64_t ldh, ldgu;
+  const __nv_bfloat16* R = nullptr;      // ADD: [M, ldr] added to gate and up before the activation (N columns, as GU)
+  int64_t ldr = 0;
 };
-struct EpiSwiglu {
+template <bool ADD>
+struct EpiSwigluOf {
   using Params = SwigluParams;
+  // v += 32 consecutive bf16 values
+  __device__ __forceinline__ static void add32(float (&v)[32], const __nv_bfloat16* r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int4 q = ld_nc_v4(r + 8 * i);
+      const float2 a = unpack_bf16(q.x), b = unpack_bf16(q.y), c = unpack_bf16(q.z), d = unpack_bf16(q.w);
+      v[8 * i + 0] += a.x; v[8 * i + 1] += a.y; v[8 * i + 2] += b.x; v[8 * i + 3] += b.y;
+      v[8 * i + 4] += c.x; v[8 * i + 5] += c.y; v[8 * i + 6] += d.x; v[8 * i + 7] += d.y;
+    }
+  }
+  __device__ __forceinline__ static void add4(float4& v, const __nv_bfloat16* r) {
+    const uint2 q = *reinterpret_cast<const uint2*>(r);
+    const float2 a = unpack_bf16(q.x), b = unpack_bf16(q.y);
+    v.x += a.x; v.y += a.y; v.z += b.x; v.w += b.y;
+  }
   static constexpr bool kFinish = true;
   template <class Sum>
   __device__ __forceinline__ static void finish(const Params& p, const Sum& sum, int row, int n0, int c, int N) {
     if (c >= 128 || n0 + 128 + c >= N) return;
-    const float4 g = sum(c), u = sum(128 + c);
+    float4 g = sum(c), u = sum(128 + c);
+    if constexpr (ADD) {
+      const __nv_bfloat16* r = p.R + static_cast<int64_t>(row) * p.ldr + n0 + c;
+      add4(g, r);
+      add4(u, r + 128);
+    }
     if (p.GU) {
       __nv_bfloat16* o = p.GU + static_cast<int64_t>(row) * p.ldgu + n0 + c;
       *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(g.x, g.y), pack_bf16(g.z, g.w));
@@ -111,6 +134,11 @@ struct EpiSwiglu {
       acc.load(c, g);
       acc.load(128 + c, u);
       if (!row_ok || n0 + 128 + c >= N) continue;
+      if constexpr (ADD) {
+        const __nv_bfloat16* r = p.R + static_cast<int64_t>(row) * p.ldr + n0 + c;
+        add32(g, r);
+        add32(u, r + 128);
+      }
       if (p.GU) {
         store_row_chunk(p.GU + static_cast<int64_t>(row) * p.ldgu + n0 + c, g, 32);
         store_row_chunk(p.GU + static_cast<int64_t>(row) * p.ldgu + n0 + 128 + c, u, 32);
@@ -124,6 +152,8 @@ struct EpiSwiglu {
     }
   }
 };
+
+using EpiSwiglu = EpiSwigluOf<false>;
 
 // the same weight layout with a clamped gate: H = g sigmoid(alpha g) (u + 1), g = min(gate, limit), u = clamp(up, -limit, limit)
 struct ClampedGluParams {
@@ -276,6 +306,19 @@ extern "C" int prl_gemm_swiglu_bf16(const void* A, const void* Wgu, void* H, voi
   using Cfg = GemmCfg<256, 2>;
   return launch_gemm<Cfg, EpiSwiglu, Behind, false>(A, Wgu, M, N2, K, lda * 2, ldw * 2, sp, Behind::Params{}, 0, 0,
                                                     stream);
+}
+
+// H = silu(A·Wg^T + Rg) * (A·Wu^T + Ru), R [M, N2] in the layout of the weight's rows (16-byte aligned rows): what adapters add, before the activation
+extern "C" int prl_gemm_swiglu_add_bf16(const void* A, const void* Wgu, const void* R, void* H, int M, int N2, int K, int64_t lda, int64_t ldw, int64_t ldr,
+                                        int64_t ldh, float* ws, cudaStream_t stream) {
+  if (N2 % 256 != 0) return -11;
+  if (ldr % 8 != 0 || (reinterpret_cast<uintptr_t>(R) & 15) != 0) return -12;
+  SwigluParams sp{static_cast<__nv_bfloat16*>(H), nullptr, ldh, 0, static_cast<const __nv_bfloat16*>(R), ldr};
+  if (M > kBlockM) {
+    using Cfg2 = Gemm2Cfg<256, false, false, false>;
+    return launch_gemm2<Cfg2, EpiSwigluOf<true>>(A, Wgu, nullptr, M, N2, K, lda * 2, ldw * 2, 0, sp, 0, stream, Sched{0, 1, 0}, ws);
+  }
+  return launch_gemm<GemmCfg<256, 2>, EpiSwigluOf<true>, Behind, false>(A, Wgu, M, N2, K, lda * 2, ldw * 2, sp, Behind::Params{}, 0, 0, stream);
 }
 
 extern "C" int prl_gemm_clamped_glu_bf16(const void* A, const void* Wgu, void* H, int M, int N2, int K, int64_t lda, int64_t ldw, int64_t ldh, float limit,

@@ -100,6 +100,13 @@ from .functional import (  # noqa: E402
     paged_decode_attention,
     sample_tokens,
 )
+from .adapters import (  # noqa: E402
+    AdapterPlan,
+    adapter_linear,
+    adapter_linear_swiglu,
+    adapter_plan,
+)
+from .logits import LogitRules, adjust_logits, token_mask  # noqa: E402
 
 __all__ = [
     "ext",
@@ -117,4 +124,11 @@ __all__ = [
     "linear_cross_entropy_tp",
     "paged_decode_attention",
     "sample_tokens",
+    "AdapterPlan",
+    "adapter_linear",
+    "adapter_linear_swiglu",
+    "adapter_plan",
+    "LogitRules",
+    "adjust_logits",
+    "token_mask",
 ]

@@ -1,0 +1,144 @@
+"""Low-rank adapters beside a shared projection.
+
+``adapter_plan`` / ``adapter_linear`` / ``adapter_linear_swiglu``: inference over rows that belong to requests with different adapters, or none
+(csrc/adapters.cu; plain PyTorch on CPU tensors).  Reference capability: the adapters that the SGLang server of a rollout worker serves by
+name; the reference's trainer merges its one adapter before rollout (3rdparty/verl/verl/utils/fsdp_utils.py:569-694)."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import functional as fn
+from . import reference as ref
+
+
+def _C():
+    from . import ext
+
+    return ext()
+
+
+# --------------------------------------------------------------------------------------------
+# many adapters at once (inference)
+# --------------------------------------------------------------------------------------------
+@dataclass
+class AdapterPlan:
+    """Rows sorted by adapter and cut into tiles: made once a step by ``adapter_plan``, used by every projection of the step."""
+
+    ids: torch.Tensor            # [T] int32; outside [0, num_adapters): the row has none
+    num_adapters: int
+    tile_rows: int = 0
+    max_tiles: int = 0
+    buf: torch.Tensor | None = None
+
+
+def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
+    """Plan of a batch whose row i belongs to adapter ``ids[i]`` (int32; a negative id, or one that is not below ``num_adapters``, means no
+    adapter).  One kernel, no host synchronisation: a captured step makes its plan anew at every replay."""
+    if ids.dim() != 1 or ids.dtype != torch.int32:
+        raise ValueError(f"adapter_plan: one int32 id a row, not {ids.dtype} {tuple(ids.shape)}")
+    if not 1 <= num_adapters <= 1024:
+        raise ValueError("adapter_plan: 1 to 1024 adapters")
+    t = ids.shape[0]
+    if not ids.is_cuda:
+        return AdapterPlan(ids, num_adapters)
+    tile = 16 if t <= 256 else 64
+    groups = min(num_adapters + 1, t)
+    most = (t - groups) // tile + groups           # tiles: the groups' rows, each rounded up
+    return AdapterPlan(ids, num_adapters, tile, most, _C().adapter_plan(ids, num_adapters, tile, most))
+
+
+def _check_adapters(name: str, x, w, a, b, scales, plan: AdapterPlan, widths, bias=None, residual=None) -> None:
+    n, k = w.shape
+    if x.dim() != 2 or x.shape[1] != k or not x.is_floating_point():
+        raise ValueError(f"{name}: rows [T, {k}] expected, not {tuple(x.shape)}")
+    if plan.ids.shape[0] != x.shape[0] or plan.ids.device != x.device:
+        raise ValueError(f"{name}: the plan is of {plan.ids.shape[0]} rows on {plan.ids.device}, x has {x.shape[0]} on {x.device}")
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[0] != plan.num_adapters:
+        raise ValueError(f"{name}: a [{plan.num_adapters}, parts * rank, K] and b [{plan.num_adapters}, N, rank] expected, not {tuple(a.shape)} and {tuple(b.shape)}")
+    if a.shape[2] != k or b.shape[1] != n or a.shape[1] != len(widths) * b.shape[2] or sum(widths) != n:
+        raise ValueError(f"{name}: stacked adapters {tuple(a.shape)}, {tuple(b.shape)} do not fit a projection {tuple(w.shape)} in parts {tuple(widths)}")
+    if not 1 <= len(widths) <= 3 or any(m <= 0 or m % 32 for m in widths) or k % 32 or b.shape[2] % 16 or not 16 <= b.shape[2] or len(widths) * b.shape[2] > 384:
+        raise ValueError(f"{name}: one to three parts of a multiple of 32 columns, K a multiple of 32, a rank that is a multiple of 16, parts * rank at most 384")
+    if scales.shape != (plan.num_adapters,) or scales.dtype != torch.float32:
+        raise ValueError(f"{name}: one fp32 scale an adapter")
+    if any(t.dtype != x.dtype or t.device != x.device for t in (a, b) + tuple(t for t in (bias, residual) if t is not None)):
+        raise ValueError(f"{name}: adapters, bias and residual of the rows' type and device")
+    if bias is not None and bias.shape != (n,) or residual is not None and residual.shape != (x.shape[0], n):
+        raise ValueError(f"{name}: bias [N], residual [T, N]")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows as the kernels read them: unit inner stride, pitch and base on 16 bytes."""
+    return t if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else fn._aligned(t)
+
+
+def _delta(x, a, b, scales, plan, widths, interleaved, bias, residual):
+    return _C().adapter_delta(_rows(x), a, b, scales, plan.buf, plan.tile_rows, plan.max_tiles, list(widths), interleaved,
+                              None if bias is None else fn._aligned(bias), None if residual is None else _rows(residual))
+
+
+def _delta_reference(x, a, b, scales, ids, widths, interleaved):
+    out = torch.zeros(x.shape[0], b.shape[1], dtype=torch.float32, device=x.device)
+    n, r = b.shape[1], b.shape[2]
+    part = (torch.arange(n) // 128) % 2 if interleaved else torch.repeat_interleave(torch.arange(len(widths)), torch.tensor(widths))
+    for l in range(a.shape[0]):
+        rows = torch.nonzero(ids == l).flatten()
+        if rows.numel():
+            low = (x[rows].float() @ a[l].float().t()).view(rows.numel(), len(widths), r) * scales[l]
+            for i in range(len(widths)):
+                cols = torch.nonzero(part == i).flatten()
+                out[rows[:, None], cols] = low[:, i] @ b[l, cols].float().t()
+    return out
+
+
+@torch.no_grad()
+def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan, widths=None,
+                   bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of ``x`` [T, K] through the shared projection ``w`` [N, K] (or an ``Fp8Weight``) and each through its own adapter l:
+
+        y_i = w x_i + scales[l] * b[l] (a[l] x_i)  (+ bias) (+ residual_i)
+
+    ``widths``: the columns of a fused projection's parts (query, key, value), each with ``rank`` rows of ``a`` [adapters, parts * rank, K] and its
+    rows of ``b`` [adapters, N, rank]; an adapter that leaves a part alone has zeros there.  Ranks are multiples of 16 (smaller ones are padded with
+    zeros).  What the adapters add is rounded to the rows' type before the product's sums are added to it.  Inference only."""
+    widths = (w.shape[0],) if widths is None else tuple(int(m) for m in widths)
+    _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
+    if not fn._is_kernel_tensor(x):
+        y = fn.linear(x, w, bias, residual)
+        return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
+    d, x = _delta(x, a, b, scales, plan, widths, False, bias, residual), _rows(x)
+    if isinstance(w, fn.Fp8Weight):
+        return fn._linear_fp8(x, w, None, d)
+    if fn._cublas() or w.dtype != x.dtype:
+        return d.addmm_(x, w.to(x.dtype).t())
+    # The framework's own products, which add the adapters' part to their fp32 sums.  (The library's, which plain decode products go to, may
+    # cut the reduction and round the pieces' sums to bf16 first.)
+    if 0 < x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._streams(w):
+        return fn.skinny_linear(x, w, None, d)
+    return _C().gemm_bf16(x, fn._g2_operand(w), d)
+
+
+@torch.no_grad()
+def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
+    """``linear_swiglu`` with an adapter for every row: ``a`` [adapters, 2 * rank, K] (gate, up), ``b`` [adapters, 2 F, rank] with its rows in the
+    order of ``wgu``'s (blocks of 128 gate and 128 up rows); the adapters act before the activation.  Inference only."""
+    n = wgu.shape[0]
+    _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
+    if n % 256:
+        raise ValueError("adapter_linear_swiglu: gate and up in blocks of 128 rows each")
+    if not fn._is_kernel_tensor(x):
+        gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
+        return ref.swiglu(gu).to(x.dtype)
+    d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True, None, None), _rows(x)
+    if isinstance(wgu, fn.Fp8Weight):
+        xq, xs = fn.quantize_fp8_rowwise(x)
+        if 0 < x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._stream_impl():
+            return _C().stream_gemm(xq, wgu.q, d, None, xs, wgu.scale, 2, 0, None, 0)
+        return ref.swiglu(_C().gemm_fp8(xq, wgu.q, xs, wgu.scale, 0) + d)
+    if fn._cublas():
+        return ref.swiglu(d.addmm_(x, wgu.t()))
+    if fn._stream_swiglu(x, wgu):
+        return _C().stream_gemm(x, wgu, d, None, None, None, 2, 0, None, -1)
+    return _C().gemm_swiglu_add(x, wgu, d)

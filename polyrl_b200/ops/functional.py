@@ -290,20 +290,24 @@ class _LinearSwigluFn(torch.autograd.Function):
         return dx, dw
 
 
+def _stream_swiglu(x: torch.Tensor, wgu: torch.Tensor) -> bool:
+    """Rows [B, K] of a decode step whose gate / up product the stream kernel takes instead of the tile kernel."""
+    # The tile kernel has one CTA per 256 weight rows: with fewer than half the SMs it cannot draw the weights fast enough.  The stream
+    # kernel splits the reduction over clusters, while two of its CTAs fit the SMs for every 256 weight rows.  In a graph, tile and stream,
+    # 16 and 128 rows: [5632, 1024] 15.7 -> 7.2, 16.1 -> 12.0 us; [12288, 2048] 23.1 -> 15.6, 23.5 -> 23.1; [16384, 2560] 29.3 -> 19.1,
+    # 28.7 -> 26.2; [18944, 3584], the last one, 39.6 -> 25.9, 37.4 -> 34.3; [9728, 896] 15.7 -> 9.3, but 16.0 -> 17.0 at 128 rows.  Beyond
+    # the line it loses, [22016, 4096] 43.0 -> 54.1 and 43.9 -> 67.8; so it does at 256 rows.
+    return (_decode_policy() == "auto" and not _cublas() and _is_decode_shape(x, wgu) and 0 < x.shape[0] <= 128 and wgu.shape[0] <= 74 * 256
+            and wgu.shape[0] % 256 == 0 and x.shape[1] % 16 == 0 and x.data_ptr() % 16 == 0 and _streams(wgu) and _stream_impl())
+
+
 def linear_swiglu(x: torch.Tensor, wgu: torch.Tensor) -> torch.Tensor:
     """silu(x @ Wg.T) * (x @ Wu.T) with W_gu stored block-interleaved ([128 gate | 128 up] rows)."""
     if isinstance(wgu, Fp8Weight):
         return _linear_fp8(x, wgu, swiglu=True)
     if _is_kernel_tensor(x) and wgu.dtype == torch.bfloat16 and x.dim() == 2 and _use_skinny(x, wgu):
         return skinny_linear(x, wgu, None, None, 1)
-    if _is_kernel_tensor(x) and wgu.dtype == torch.bfloat16 and x.dim() == 2 and _decode_policy() == "auto" and not _cublas() \
-            and _is_decode_shape(x, wgu) and 0 < x.shape[0] <= 128 and wgu.shape[0] <= 74 * 256 and wgu.shape[0] % 256 == 0 \
-            and x.shape[1] % 16 == 0 and x.data_ptr() % 16 == 0 and _streams(wgu) and _stream_impl():
-        # The tile kernel has one CTA per 256 weight rows: with fewer than half the SMs it cannot draw the weights fast enough.  The stream
-        # kernel splits the reduction over clusters, while two of its CTAs fit the SMs for every 256 weight rows.  In a graph, tile and stream,
-        # 16 and 128 rows: [5632, 1024] 15.7 -> 7.2, 16.1 -> 12.0 us; [12288, 2048] 23.1 -> 15.6, 23.5 -> 23.1; [16384, 2560] 29.3 -> 19.1,
-        # 28.7 -> 26.2; [18944, 3584], the last one, 39.6 -> 25.9, 37.4 -> 34.3; [9728, 896] 15.7 -> 9.3, but 16.0 -> 17.0 at 128 rows.  Beyond
-        # the line it loses, [22016, 4096] 43.0 -> 54.1 and 43.9 -> 67.8; so it does at 256 rows.
+    if _is_kernel_tensor(x) and wgu.dtype == torch.bfloat16 and x.dim() == 2 and _stream_swiglu(x, wgu):
         return skinny_linear(x, wgu, None, None, 1)
     if _is_kernel_tensor(x) and wgu.dtype == torch.bfloat16 and not _cublas():
         return _LinearSwigluFn.apply(x, wgu)

@@ -274,7 +274,7 @@ template <int TM>
 static int run_delta(const DeltaParams& p, int ctas, cudaStream_t stream) {
   const int smem = DeltaSmem<TM>::bytes(p.parts * p.rank);
   auto kern = delta_kernel<TM>;
-  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaSmem<TM>::bytes(kDeltaMaxLow)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles) * ctas);
   cfg.blockDim = dim3(kDeltaThreads);

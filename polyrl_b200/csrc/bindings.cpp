@@ -2,6 +2,7 @@
 // Kernel translation units are torch-free (raw pointers + cudaStream_t) so they compile in seconds;
 // only the bindings*.cpp files see torch headers (bindings_serve.cpp: what serving needs).
 #include "bindings_common.hpp"
+#include "lora.hpp"
 
 #include <cstdint>
 #include <string>
@@ -10,6 +11,11 @@
 extern "C" {
 int prl_gemm2_bf16(const void*, const void*, void*, const void*, int, int, int, int64_t, int64_t, int64_t, int, int, int, float*, cudaStream_t);
 int64_t prl_gemm2_ws_floats(int, int, int);
+int64_t prl_gemm2_tail_ws_floats(int, int, int, int);
+int prl_gemm2_tail_bf16(const void*, const void*, const void*, const void*, void*, const void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int, float*, cudaStream_t);
+int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
+int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, cudaStream_t);
+int prl_lora_pack(const prl::LoraPackParams*, cudaStream_t);
 int prl_gemm2_grads_joint(int, int, int);
 int prl_gemm2_grads(const void*, const void*, const void*, void*, float*, float, void*, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, cudaStream_t);
 int prl_gemm2_bf16_accum_f32(const void*, const void*, float*, float, int, int, int, int64_t, int64_t, int64_t, int, int, float*, cudaStream_t);
@@ -511,6 +517,105 @@ at::Tensor stream_gemm(const at::Tensor& x, const at::Tensor& w, const c10::opti
   return out;
 }
 
+// ---------------------------------------------------------------------------------------------- adapters that are trained (lora.cu)
+using OptT = c10::optional<at::Tensor>;
+const void* lora_operand(const at::Tensor& t, const at::Tensor& like, const char* what) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1 && t.stride(0) % 8 == 0 &&
+              t.stride(0) >= t.size(1) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+              what, ": bf16 matrix on the rows' device, unit inner stride, pitch a multiple of 8, 16-byte aligned");
+  return t.data_ptr();
+}
+
+// parts of a fused projection's adapters -> A one below the other [R, K], B block-diagonal [N, R (+ 8 with a bias)]; ranks padded to 8
+std::vector<at::Tensor> lora_pack(const std::vector<OptT>& a, const std::vector<OptT>& b, const std::vector<int64_t>& widths, bool interleaved, const OptT& bias) {
+  prl::LoraPackParams p{};
+  p.parts = widths.size();
+  TORCH_CHECK(p.parts >= 1 && p.parts <= 3 && a.size() == widths.size() && b.size() == widths.size(), "lora_pack: one to three parts");
+  at::Tensor like;
+  int64_t R = 0, N = 0, K = 0;
+  for (int i = 0; i < p.parts; ++i) {
+    N += widths[i];
+    p.ends[i] = N;
+    p.off[i] = R;
+    TORCH_CHECK(a[i].has_value() == b[i].has_value(), "lora_pack: both matrices of a part or none");
+    if (!a[i].has_value()) continue;
+    const at::Tensor &u = *a[i], &v = *b[i];
+    if (!like.defined()) { like = u; K = u.size(1); }
+    TORCH_CHECK(u.is_cuda() && u.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && u.device() == like.device() && v.device() == like.device() &&
+                u.dim() == 2 && v.dim() == 2 && u.is_contiguous() && v.is_contiguous() && u.size(1) == K && v.size(0) == widths[i] && v.size(1) == u.size(0) && u.size(0) > 0 &&
+                (reinterpret_cast<uintptr_t>(u.data_ptr()) & 15) == 0, "lora_pack: contiguous bf16 A [rank, K] and B [columns, rank]");
+    p.a[i] = u.data_ptr(); p.b[i] = v.data_ptr(); p.rank[i] = u.size(0);
+    R += (u.size(0) + 7) / 8 * 8;
+  }
+  TORCH_CHECK(like.defined() && K % 8 == 0 && N > 0 && N <= 0x7fffffff && K <= 0x7fffffff, "lora_pack: no adapter, or sizes");
+  TORCH_CHECK(!interleaved || (p.parts == 2 && widths[0] == widths[1] && N % 256 == 0), "lora_pack: gate and up in blocks of 128");
+  const int64_t ldb = R + (bias.has_value() ? 8 : 0);
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == like.device() && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() && bias->numel() == N, "lora_pack: bf16 bias [N]");
+    p.bias = bias->data_ptr();
+  }
+  c10::cuda::CUDAGuard g(like.device());
+  at::Tensor ao = at::empty({R, K}, like.options()), bo = at::empty({N, ldb}, like.options());
+  p.a_out = ao.data_ptr(); p.b_out = bo.data_ptr(); p.interleaved = interleaved; p.R = R; p.K = K; p.N = N; p.ldb = ldb;
+  check(prl_lora_pack(&p, cur_stream()), "lora_pack");
+  return {ao, bo};
+}
+
+// layout 0: scale a [M, K] b [R, K]^T; 1: scale a [M, K] b [K, R]; 2: scale a [K, M]^T b [K, R]; 3: the transpose of that, [R, M].  `rank` columns of
+// b take part (0: all); pad: further columns, ones in the first
+at::Tensor lora_thin(const at::Tensor& a, const at::Tensor& b, int64_t layout, double scale, int64_t rank, int64_t pad, int64_t split) {
+  TORCH_CHECK(a.is_cuda() && layout >= 0 && layout <= 3 && pad >= 0 && pad % 8 == 0 && (layout != 3 || pad == 0), "lora_thin: layout");
+  const void *pa = lora_operand(a, a, "lora_thin: a"), *pb = lora_operand(b, a, "lora_thin: b");
+  const int64_t M = layout >= 2 ? a.size(1) : a.size(0), K = layout >= 2 ? a.size(0) : a.size(1), Kb = layout == 0 ? b.size(1) : b.size(0),
+                width = layout == 0 ? b.size(0) : b.size(1), R = rank > 0 ? rank : width;
+  TORCH_CHECK(K == Kb && R <= width && R % 8 == 0 && M <= 0x7fffffff && K <= 0x7fffffff, "lora_thin: sizes");
+  c10::cuda::CUDAGuard g(a.device());
+  at::Tensor out = layout == 3 ? at::empty({R, M}, a.options()) : at::empty({M, R + pad}, a.options());
+  if (K == 0) return out.zero_();
+  check(prl_lora_thin(pa, pb, out.data_ptr(), M, R, K, a.stride(0), b.stride(0), out.stride(0), static_cast<float>(scale), static_cast<int>(layout),
+                      static_cast<int>(pad), static_cast<int>(split), cur_stream()), "lora_thin");
+  return out;
+}
+
+// x w^T + t b^T (b_mn: x w + t b, w [K, N], b [R, N]) (+ residual)
+at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const at::Tensor& b, bool b_mn, const OptT& residual) {
+  const void *px = lora_operand(x, x, "lora_gemm: x"), *pw = lora_operand(w, x, "lora_gemm: w"), *pt = lora_operand(t, x, "lora_gemm: t"),
+             *pb = lora_operand(b, x, "lora_gemm: b");
+  const int64_t M = x.size(0), K = x.size(1), N = b_mn ? w.size(1) : w.size(0), R = t.size(1);
+  TORCH_CHECK((b_mn ? w.size(0) : w.size(1)) == K && t.size(0) == M && (b_mn ? b.size(0) : b.size(1)) == R && (b_mn ? b.size(1) : b.size(0)) == N && N % 8 == 0 &&
+              K > 0 && R > 0 && M <= 0x7fffffff && K <= 0x7fffff00 && N <= 0x7fffffff, "lora_gemm: sizes");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor d = at::empty({M, N}, x.options());
+  if (M == 0) return d;
+  const void* r = nullptr;
+  if (residual.has_value()) {
+    r = lora_operand(*residual, x, "lora_gemm: residual");
+    TORCH_CHECK(residual->sizes() == d.sizes() && residual->stride(0) == N, "lora_gemm: residual like the result");
+  }
+  const at::Tensor ws = split_scratch(prl_gemm2_tail_ws_floats(M, N, K, R), x);
+  check(prl_gemm2_tail_bf16(px, pw, pt, pb, d.data_ptr(), r, M, N, K, R, x.stride(0), w.stride(0), t.stride(0), b.stride(0), N, b_mn, split_ptr(ws), cur_stream()),
+        "lora_gemm");
+  return d;
+}
+
+// {silu(gate) * up, the projection itself if save} of x w^T + t b^T
+std::vector<at::Tensor> lora_gemm_swiglu(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const at::Tensor& b, bool save) {
+  const void *px = lora_operand(x, x, "lora_gemm_swiglu: x"), *pw = lora_operand(w, x, "lora_gemm_swiglu: w"), *pt = lora_operand(t, x, "lora_gemm_swiglu: t"),
+             *pb = lora_operand(b, x, "lora_gemm_swiglu: b");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0), R = t.size(1);
+  TORCH_CHECK(w.size(1) == K && t.size(0) == M && b.size(1) == R && b.size(0) == N && N % 256 == 0 && K > 0 && R > 0 && M <= 0x7fffffff && K <= 0x7fffff00,
+              "lora_gemm_swiglu: sizes");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor h = at::empty({M, N / 2}, x.options()), gu = save ? at::empty({M, N}, x.options()) : at::Tensor();
+  if (M > 0) {
+    const at::Tensor ws = split_scratch(prl_gemm2_tail_ws_floats(M, N, K, R), x);
+    check(prl_gemm_swiglu_tail_bf16(px, pw, pt, pb, h.data_ptr(), save ? gu.data_ptr() : nullptr, M, N, K, R, x.stride(0), w.stride(0), t.stride(0), b.stride(0), N / 2,
+                                    N, split_ptr(ws), cur_stream()), "lora_gemm_swiglu");
+  }
+  if (save) return {h, gu};
+  return {h};
+}
+
 // Row-parallel TP linear with the all-reduce fused into the GEMM epilogue over NVLink peer memory.
 at::Tensor skinny_gemm_tp(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& residual,
                           at::Tensor workspace, at::Tensor counters, int64_t splits, const std::vector<int64_t>& inbox_ptrs,
@@ -699,6 +804,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("force_bn") = 0);
   m.def("skinny_gemm", &skinny_gemm);
   m.def("skinny_gemm_tp", &skinny_gemm_tp);
+  m.def("lora_pack", &lora_pack);
+  m.def("lora_thin", &lora_thin, py::arg("a"), py::arg("b"), py::arg("layout"), py::arg("scale") = 1.0, py::arg("rank") = 0, py::arg("pad") = 0,
+        py::arg("split") = 0);
+  m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("b"), py::arg("b_mn") = false, py::arg("residual") = py::none());
+  m.def("lora_gemm_swiglu", &lora_gemm_swiglu);
   m.def("stream_gemm", &stream_gemm, py::arg("x"), py::arg("w"), py::arg("residual") = py::none(), py::arg("bias") = py::none(),
         py::arg("x_scale") = py::none(), py::arg("w_scale") = py::none(), py::arg("mode") = 0, py::arg("splits") = 0,
         py::arg("out") = py::none(), py::arg("pair") = -1);

@@ -111,3 +111,22 @@ extern "C" int prl_gemm2_bf16_accum_f32(const void* A, const void* B, float* D, 
   if (a_mn && b_mn) return run2_accum<true, true>(A, B, D, beta, M, N, K, lda, ldb, ldd, ws, stream);
   return run2_accum<true, false>(A, B, D, beta, M, N, K, lda, ldb, ldd, ws, stream);
 }
+
+// D[M,N] = sum_k A(m,k) B(n,k) + sum_r A2(m,r) B2(n,r) (+R): A [M,K] and A2 [M,R2] row-major; B and B2 as b_mn says.  ws: prl_gemm2_tail_ws_floats floats
+// of scratch, or null.
+extern "C" int64_t prl_gemm2_tail_ws_floats(int M, int N, int K, int R2) { return prl_gemm2_ws_floats(M, N, tail_k(K, R2)); }
+extern "C" int prl_gemm2_tail_bf16(const void* A, const void* B, const void* A2, const void* B2, void* D, const void* R, int M, int N, int K, int R2, int64_t lda,
+                                   int64_t ldb, int64_t lda2, int64_t ldb2, int64_t ldd, int b_mn, float* ws, cudaStream_t stream) {
+  TmaStoreParams ep{static_cast<const __nv_bfloat16*>(R), ldd, static_cast<__nv_bfloat16*>(D)};
+  const TailOperands to{A2, B2, R2, lda2 * 2, ldb2 * 2};
+#define PRL_TAIL(BN_, BM_)                                                                                                             \
+  return launch_gemm2<Gemm2Cfg<BN_, false, BM_, true, 1, true>, EpiTmaStore>(A, B, D, M, N, K, lda * 2, ldb * 2, ldd * 2, ep, 0, stream, \
+                                                                             Sched{0, 1, 0}, ws, &to)
+  if (N > 128) {
+    if (b_mn) PRL_TAIL(256, true);
+    PRL_TAIL(256, false);
+  }
+  if (b_mn) PRL_TAIL(128, true);
+  PRL_TAIL(128, false);
+#undef PRL_TAIL
+}

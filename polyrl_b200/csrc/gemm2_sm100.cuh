@@ -28,6 +28,8 @@
 // store, optional fused residual add; each epilogue warp double-buffers its own 32 x 64
 // box so no cross-warp barrier is needed.
 #pragma once
+#include <type_traits>
+
 #include "gemm_sm100.cuh"
 
 namespace prl {
@@ -37,8 +39,19 @@ constexpr int kSmemMax = 232448;   // 227 KB opt-in limit per CTA
 // EPI_GROUPS: warpgroups that share a tile's columns in the epilogue.  One is enough where the epilogue converts and stores; an epilogue
 // that takes an exponential per element gets two, because a warp per scheduler cannot hide its latencies and short reductions
 // (K of about a thousand) leave it no time: the figures are beside its users.
-template <int BN, bool A_MN_, bool B_MN_, bool TMA_STORE_, int EPI_GROUPS_ = 1>
+// TAIL: the sum goes on over a second pair of operands, D = A B^T + A2 B2^T with A2 [M, R] K-major and B2 laid out as B: further k-blocks of the
+// same tiles, out of other tensor maps.  A low-rank adapter beside a weight costs ceil(R / 64) k-blocks this way and no pass over D.
+struct alignas(64) Gemm2Tail {
+  CUtensorMap A, B;
+  int main_kb;             // k-blocks of the first pair; K counts those of both, 64 each
+};
+struct NoTail {};
+
+template <int BN, bool A_MN_, bool B_MN_, bool TMA_STORE_, int EPI_GROUPS_ = 1, bool TAIL_ = false>
 struct Gemm2Cfg {
+  static constexpr bool TAIL = TAIL_;
+  using Tail = std::conditional_t<TAIL, Gemm2Tail, NoTail>;
+  static_assert(!(TAIL && A_MN_), "the second pair's A is K-major");
   static constexpr int EPI_GROUPS = EPI_GROUPS_, EPI_WARPS = 4 * EPI_GROUPS, THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int GROUP_N = BN / EPI_GROUPS;     // columns of a group
   static constexpr bool A_MN = A_MN_, B_MN = B_MN_, TMA_STORE = TMA_STORE_;
@@ -133,7 +146,8 @@ template <class Cfg, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg::THREADS, 1)
 gemm2_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmD, typename Epi::Params ep, int M, int N, int K,
-                   int num_m_blocks, int num_n_blocks, int n_splits, int nb_per_split, Sched sc, KSplit ks) {
+                   int num_m_blocks, int num_n_blocks, int n_splits, int nb_per_split, Sched sc, KSplit ks,
+                   const __grid_constant__ typename Cfg::Tail tail) {
   constexpr int BN = Cfg::BLOCK_N;
   constexpr int kStages = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -160,6 +174,10 @@ gemm2_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     if constexpr (Cfg::TMA_STORE) tma_prefetch_desc(&tmD);
+    if constexpr (Cfg::TAIL) {
+      tma_prefetch_desc(&tail.A);
+      tma_prefetch_desc(&tail.B);
+    }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full_bar[i], 1);
       mbar_init(&empty_bar[i], 1);
@@ -192,20 +210,28 @@ gemm2_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
           uint8_t* sa = smem_a + stage * Cfg::A_BYTES;
           uint8_t* sb = smem_b + stage * Cfg::B_BYTES;
-          const int k0 = kb * Cfg::BLOCK_K;
+          int k0 = kb * Cfg::BLOCK_K;
+          const CUtensorMap *ta = &tmA, *tb = &tmB;
+          if constexpr (Cfg::TAIL) {
+            if (kb >= tail.main_kb) {
+              k0 = (kb - tail.main_kb) * Cfg::BLOCK_K;
+              ta = &tail.A;
+              tb = &tail.B;
+            }
+          }
           if constexpr (!Cfg::A_MN) {
-            tma_load_2d_2sm(&tmA, &full_bar[stage], sa, k0, m0, kEvictNormal);
+            tma_load_2d_2sm(ta, &full_bar[stage], sa, k0, m0, kEvictNormal);
           } else {
 #pragma unroll
             for (int c = 0; c < Cfg::CTA_M / 64; ++c)
-              tma_load_2d_2sm(&tmA, &full_bar[stage], sa + c * 8192, m0 + c * 64, k0, kEvictNormal);
+              tma_load_2d_2sm(ta, &full_bar[stage], sa + c * 8192, m0 + c * 64, k0, kEvictNormal);
           }
           if constexpr (!Cfg::B_MN) {
-            tma_load_2d_2sm(&tmB, &full_bar[stage], sb, k0, n0, kEvictNormal);
+            tma_load_2d_2sm(tb, &full_bar[stage], sb, k0, n0, kEvictNormal);
           } else {
 #pragma unroll
             for (int c = 0; c < Cfg::CTA_N / 64; ++c)
-              tma_load_2d_2sm(&tmB, &full_bar[stage], sb + c * 8192, n0 + c * 64, k0, kEvictNormal);
+              tma_load_2d_2sm(tb, &full_bar[stage], sb + c * 8192, n0 + c * 64, k0, kEvictNormal);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -465,12 +491,23 @@ inline KSplit plan_k_split(int M, int N, int K) {
 // host launcher.  Pitches in BYTES.  For an MN-major operand the pointer addresses the
 // [reduction, M-or-N] row-major matrix (i.e. the tensor as it lies in memory).
 // ------------------------------------------------------------------------------------------
+// second pair of operands (Cfg::TAIL): A2 [M, R], B2 as B, pitches in bytes
+struct TailOperands {
+  const void *A, *B;
+  int R;
+  int64_t lda_bytes, ldb_bytes;
+};
+inline int tail_blocks(int R) { return (R + 63) / 64; }
+// reduction length of a product with a tail, in whole k-blocks: what plan_k_split and the workspace go by
+inline int tail_k(int K, int R) { return 64 * ((K + 63) / 64 + tail_blocks(R)); }
+
 template <class Cfg, class Epi>
 int launch_gemm2(const void* A, const void* B, void* D, int M, int N, int K, int64_t lda_bytes, int64_t ldb_bytes,
                  int64_t ldd_bytes, const typename Epi::Params& ep, int n_splits, cudaStream_t stream,
-                 Sched sc = Sched{0, 1, 0}, float* ws = nullptr) {
+                 Sched sc = Sched{0, 1, 0}, float* ws = nullptr, const TailOperands* to = nullptr) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   CUtensorMap tmA, tmB, tmD;
+  typename Cfg::Tail tail;
   if (Cfg::A_MN ? make_tmap_kmajor(&tmA, A, K, M, lda_bytes, 64, 2) : make_tmap_kmajor(&tmA, A, M, K, lda_bytes, Cfg::CTA_M, 2))
     return -2;
   if (Cfg::B_MN ? make_tmap_kmajor(&tmB, B, K, N, ldb_bytes, 64, 2) : make_tmap_kmajor(&tmB, B, N, K, ldb_bytes, Cfg::CTA_N, 2))
@@ -479,6 +516,13 @@ int launch_gemm2(const void* A, const void* B, void* D, int M, int N, int K, int
     if (make_tmap_kmajor(&tmD, D, M, N, ldd_bytes, 32, 2)) return -4;
   } else {
     tmD = tmA;
+  }
+  if constexpr (Cfg::TAIL) {
+    if (to == nullptr || to->R <= 0) return -5;
+    if (make_tmap_kmajor(&tail.A, to->A, M, to->R, to->lda_bytes, Cfg::CTA_M, 2)) return -6;
+    if (Cfg::B_MN ? make_tmap_kmajor(&tail.B, to->B, to->R, N, to->ldb_bytes, 64, 2) : make_tmap_kmajor(&tail.B, to->B, N, to->R, to->ldb_bytes, Cfg::CTA_N, 2)) return -7;
+    tail.main_kb = (K + 63) / 64;
+    K = tail_k(K, to->R);
   }
   const int num_m_blocks = (M + Cfg::BLOCK_M - 1) / Cfg::BLOCK_M;
   const int num_n_blocks = (N + Cfg::BLOCK_N - 1) / Cfg::BLOCK_N;
@@ -500,7 +544,7 @@ int launch_gemm2(const void* A, const void* B, void* D, int M, int N, int K, int
   }
   if (!ks.tiles && total < clusters) clusters = total;
   kern<<<2 * clusters, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(tmA, tmB, tmD, ep, M, N, K, num_m_blocks, num_n_blocks,
-                                                               n_splits, nb_per_split, sc, ks);
+                                                               n_splits, nb_per_split, sc, ks, tail);
   PRL_CUDA_CHECK(cudaGetLastError());
   if constexpr (Epi::kFinish) {
     if (ks.tiles) {

@@ -321,6 +321,15 @@ extern "C" int prl_gemm_swiglu_add_bf16(const void* A, const void* Wgu, const vo
   return launch_gemm<GemmCfg<256, 2>, EpiSwigluOf<true>, Behind, false>(A, Wgu, M, N2, K, lda * 2, ldw * 2, sp, Behind::Params{}, 0, 0, stream);
 }
 
+// H = silu of gate times up of A·Wgu^T + A2·B2^T, GU the projection itself; A2 [M, R2], B2 [N2, R2] in the order of Wgu's rows
+extern "C" int prl_gemm_swiglu_tail_bf16(const void* A, const void* Wgu, const void* A2, const void* B2, void* H, void* GU, int M, int N2, int K, int R2, int64_t lda,
+                                         int64_t ldw, int64_t lda2, int64_t ldb2, int64_t ldh, int64_t ldgu, float* ws, cudaStream_t stream) {
+  if (N2 % 256 != 0) return -11;
+  SwigluParams sp{static_cast<__nv_bfloat16*>(H), static_cast<__nv_bfloat16*>(GU), ldh, ldgu};
+  const TailOperands to{A2, B2, R2, lda2 * 2, ldb2 * 2};
+  return launch_gemm2<Gemm2Cfg<256, false, false, false, 1, true>, EpiSwiglu>(A, Wgu, nullptr, M, N2, K, lda * 2, ldw * 2, 0, sp, 0, stream, Sched{0, 1, 0}, ws, &to);
+}
+
 extern "C" int prl_gemm_clamped_glu_bf16(const void* A, const void* Wgu, void* H, int M, int N2, int K, int64_t lda, int64_t ldw, int64_t ldh, float limit,
                                          float alpha, cudaStream_t stream) {
   if (N2 % 256 != 0) return -11;

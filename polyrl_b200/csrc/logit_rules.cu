@@ -150,7 +150,7 @@ static int run_rules(const RuleParams& p, cudaStream_t stream) {
   auto kern = wide ? inplace ? rules_kernel<T, VEC, true> : rules_kernel<T, VEC, false> : inplace ? rules_kernel<T, 1, true> : rules_kernel<T, 1, false>;
   const size_t smem = p.chunk * 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleMaxChunk * 4);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   PRL_CUDA_CHECK(launch_behind(kern, static_cast<unsigned>(blocks), kRuleThreads, smem, stream, p, chunks));
@@ -169,6 +169,6 @@ extern "C" int prl_adjust_logits(const prl::RuleParams* q, int fp32, cudaStream_
     p.chunk = 16384;
     while (p.chunk > 2048 && static_cast<int64_t>(p.rows) * ((p.V + p.chunk - 1) / p.chunk) < 2 * 148) p.chunk >>= 1;
   }
-  if (p.chunk % 128 || p.chunk > 32768) return -2;
+  if (p.chunk % 128 || p.chunk > prl::kRuleMaxChunk) return -2;
   return fp32 ? prl::run_rules<float>(p, stream) : prl::run_rules<__nv_bfloat16>(p, stream);
 }

@@ -5,6 +5,7 @@
 namespace prl {
 
 constexpr int kRuleThreads = 256;
+constexpr int kRuleMaxChunk = 32768;
 constexpr int kRuleCountBits = 20;                  // a history is shorter than 2^20 tokens
 constexpr int kRuleMaxBias = 2046;                  // entries of a row's bias list
 

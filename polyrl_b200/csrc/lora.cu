@@ -1,0 +1,281 @@
+// polyrl_b200 — the thin products of a low-rank adapter that is trained beside a frozen projection y = x W^T:
+//
+//   t  = s x A^T     [T, R]      forward               dt = s dy B      [T, R]      backward, towards x and A
+//   dA = dt^T x      [R, K]                            dB = dy^T t      [N, R]
+//
+// R is a few dozen (all parts of a fused projection side by side, B block-diagonal), the other two sides are thousands, so each product reads
+// its one large operand (x or dy) once and is bound by that.  y += t B^T and dx += dt A are not here: t and dt are further k-blocks of the
+// large products (gemm2_sm100.cuh, Gemm2Tail), so what the adapter adds is summed in fp32 with the rest, rounds nothing of its own and moves
+// no [T, N] or [T, K] array.  t and dt are rounded to bf16 (2^-8 relative at most), as every operand of a product is.
+//
+// thin   D[m, r] = scale * sum_k A(m, k) B(r, k), 128 rows of D a tile: tcgen05.mma 128 x R x 16, both operands by TMA (K-major, or MN-major
+//        where the sum runs over tokens: dA is computed as x^T dt and stored transposed).  A cluster of S CTAs shares a tile's reduction,
+//        because R is narrow and 128-row tiles alone are too few to draw HBM bandwidth: 32 tiles for dA of a 4096-wide layer.  The CTAs
+//        leave their fp32 sums in shared memory and each adds up its share of the tile over distributed shared memory, in the order of the
+//        ranks: results do not depend on timing.
+// pack   A parts one below the other, B parts block-diagonal in the order of the projection's columns, ranks padded to 8 with zeros; a bias
+//        becomes one more column of B against a column of ones in t, which the forward product then adds for nothing.
+#include "gemm_sm100.cuh"
+#include "lora.hpp"
+
+namespace prl {
+
+constexpr int kThinThreads = 192;                    // warp 0 TMA, warp 1 MMA, warps 2..5 accumulators -> shared memory; all of them store
+constexpr int kThinStageA = kBlockM * 128;
+constexpr int kThinSmemMax = 201 * 1024;
+
+template <bool MN>
+__host__ __device__ constexpr int thin_b_bytes(int NR) { return MN ? (NR + 63) / 64 * 8192 : NR * 128; }
+
+struct ThinParams {
+  __nv_bfloat16* out;
+  int64_t ldo;
+  int M, R, K, NR, stages;
+  float scale;
+  int pad;                                           // columns after the last one: the first is 1, the rest 0 (row-major output)
+};
+
+// grid (tiles * S, blocks of NR columns); A_MN / B_MN: the reduction runs over the operand's rows in memory; TRANS: out is [R, M]
+template <bool A_MN, bool B_MN, bool TRANS>
+__global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const ThinParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[8], empty_bar[8], done_bar;
+  __shared__ uint32_t tmem_slot;
+  const int b_bytes = thin_b_bytes<B_MN>(p.NR), stage_bytes = kThinStageA + b_bytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t S;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
+  const uint32_t rank = cluster_ctarank();
+  const int m0 = blockIdx.x / S * kBlockM, r0 = blockIdx.y * p.NR;
+  const int num_kb = (p.K + 63) / 64, kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
+  const uint32_t tmem_cols = p.NR <= 32 ? 32 : p.NR <= 64 ? 64 : p.NR <= 128 ? 128 : 256;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], 1);
+    }
+    mbar_init(&done_bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        mbar_wait(&empty_bar[stage], phase ^ 1);
+        mbar_expect_tx(&full_bar[stage], stage_bytes);
+        uint8_t* sa = smem + stage * stage_bytes;
+        uint8_t* sb = sa + kThinStageA;
+        if constexpr (A_MN) {
+          tma_load_2d(&tmA, &full_bar[stage], sa, m0, kb * 64);
+          tma_load_2d(&tmA, &full_bar[stage], sa + 8192, m0 + 64, kb * 64);
+        } else {
+          tma_load_2d(&tmA, &full_bar[stage], sa, kb * 64, m0);
+        }
+        if constexpr (B_MN) {
+          for (int c = 0; c < p.NR; c += 64) tma_load_2d(&tmB, &full_bar[stage], sb + c / 64 * 8192, r0 + c, kb * 64);
+        } else {
+          tma_load_2d(&tmB, &full_bar[stage], sb, kb * 64, r0);
+        }
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_major(kBlockM, p.NR, 1, 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
+      constexpr uint32_t a_step = A_MN ? (16 * 128) >> 4 : 32 >> 4, b_step = B_MN ? (16 * 128) >> 4 : 32 >> 4;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        mbar_wait(&full_bar[stage], phase);
+        tc_fence_after();
+        const uint8_t* sa = smem + stage * stage_bytes;
+        const uint8_t* sb = sa + kThinStageA;
+        const uint64_t da = A_MN ? umma_desc_sw128_mnmajor(sa, 8192) : umma_desc_sw128_kmajor(sa);
+        const uint64_t db = B_MN ? umma_desc_sw128_mnmajor(sb, 8192) : umma_desc_sw128_kmajor(sb);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem, da + k * a_step, db + k * b_step, idesc, kb != kb0 || k != 0);
+        umma_commit(&empty_bar[stage]);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(&done_bar);
+    }
+  } else {
+    // every load has landed and every product has read its stage: the pipeline's memory takes the sums, rows of NR + 4 floats (an odd number
+    // of 16-byte units, so that 8 lanes' rows start in different banks)
+    mbar_wait(&done_bar, 0);
+    tc_fence_after();
+    const int quad = warp & 3, row = quad * 32 + lane;
+    float* dst = reinterpret_cast<float*>(smem) + row * (p.NR + 4);
+    for (int c = 0; c < p.NR; c += 16) {
+      uint32_t r[16];
+      __syncwarp();
+      tmem_ld_32x16(tmem + c + (static_cast<uint32_t>(quad * 32) << 16), r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + c + 4 * j) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+
+  const uint32_t base = smem_u32(smem);
+  auto peer = [&](uint32_t k) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base), "r"(k));
+    return a;
+  };
+  if constexpr (!TRANS) {                            // a share of the rows, four columns a thread
+    const int rows0 = kBlockM * rank / S, rows1 = kBlockM * (rank + 1) / S;
+    const int cols = min(p.NR, p.R - r0), last = blockIdx.y + 1 == gridDim.y ? p.pad : 0, quads = (cols + last) / 4;
+    for (int e = threadIdx.x; e < (rows1 - rows0) * quads; e += kThinThreads) {
+      const int row = rows0 + e / quads, c = e % quads * 4;
+      if (m0 + row >= p.M) break;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < cols) {
+        const uint32_t off = (row * (p.NR + 4) + c) * 4;
+        for (uint32_t k = 0; k < S; ++k) {
+          float4 q;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(peer(k) + off) : "memory");
+          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+        }
+        v.x *= p.scale; v.y *= p.scale; v.z *= p.scale; v.w *= p.scale;
+      } else if (c == cols) {
+        v.x = 1.f;
+      }
+      *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(m0 + row) * p.ldo + r0 + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    }
+  } else {                                           // a share of the columns, lanes along the tile's rows
+    const int cols = min(p.NR, p.R - r0), c0 = cols * rank / S, c1 = cols * (rank + 1) / S;
+    for (int e = threadIdx.x; e < (c1 - c0) * kBlockM; e += kThinThreads) {
+      const int c = c0 + e / kBlockM, row = e % kBlockM;
+      if (m0 + row >= p.M) continue;
+      const uint32_t off = (row * (p.NR + 4) + c) * 4;
+      float v = 0.f;
+      for (uint32_t k = 0; k < S; ++k) {
+        float q;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(peer(k) + off) : "memory");
+        v += q;
+      }
+      p.out[static_cast<int64_t>(r0 + c) * p.ldo + m0 + row] = __float2bfloat16(p.scale * v);
+    }
+  }
+  cluster_sync_all();                                // a peer may still read this CTA's sums
+}
+
+template <bool A_MN, bool B_MN, bool TRANS>
+static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int64_t ldb, int split, cudaStream_t stream) {
+  p.NR = p.R >= 256 ? 256 : (p.R + 15) / 16 * 16;
+  const int stage = kThinStageA + thin_b_bytes<B_MN>(p.NR), sums = kBlockM * (p.NR + 4) * 4;
+  const int budget = p.NR <= 128 ? 100 * 1024 : 200 * 1024;           // two CTAs an SM where two fit
+  p.stages = budget / stage > 8 ? 8 : budget / stage;
+  const int smem = (p.stages * stage > sums ? p.stages * stage : sums) + 1024;
+  CUtensorMap tmA, tmB;
+  if (A_MN ? make_tmap_kmajor(&tmA, A, p.K, p.M, lda * 2, 64, 2) : make_tmap_kmajor(&tmA, A, p.M, p.K, lda * 2, kBlockM, 2)) return -2;
+  if (B_MN ? make_tmap_kmajor(&tmB, B, p.K, p.R, ldb * 2, 64, 2) : make_tmap_kmajor(&tmB, B, p.R, p.K, ldb * 2, p.NR, 2)) return -3;
+  const int tiles = (p.M + kBlockM - 1) / kBlockM, blocks = (p.R + p.NR - 1) / p.NR, num_kb = (p.K + 63) / 64;
+  int S = split;
+  if (S <= 0) {
+    S = 1;
+    while (S < 8 && static_cast<int64_t>(tiles) * blocks * S < 200 && num_kb / (2 * S) >= 4) S *= 2;
+  }
+  if (S > 8 || S > num_kb || (S & (S - 1))) return -4;
+  auto kern = thin_kernel<A_MN, B_MN, TRANS>;
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kThinSmemMax));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles * S, blocks);
+  cfg.blockDim = dim3(kThinThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = S;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  PRL_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, static_cast<const ThinParams>(p)));
+  PRL_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}
+
+// ------------------------------------------------------------------------------------------------------------ pack
+__global__ void __launch_bounds__(256) lora_pack_kernel(const LoraPackParams p) {
+  const int64_t na = static_cast<int64_t>(p.R) * p.K, nb = static_cast<int64_t>(p.N) * p.ldb;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e * 8 < na + nb; e += static_cast<int64_t>(gridDim.x) * 256) {
+    union { int4 v; __nv_bfloat16 h[8]; } o;
+    if (e * 8 < na) {                                // a row of A, or a row of padding
+      const int r = static_cast<int>(e * 8 / p.K), k = static_cast<int>(e * 8 - static_cast<int64_t>(r) * p.K);
+      int i = 0;
+      while (i + 1 < p.parts && r >= p.off[i + 1]) ++i;
+      const int own = r - p.off[i];
+      o.v = own < p.rank[i] ? *reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.a[i]) + static_cast<int64_t>(own) * p.K + k) : make_int4(0, 0, 0, 0);
+      reinterpret_cast<int4*>(p.a_out)[e] = o.v;
+    } else {                                         // eight columns of a row of the block-diagonal B
+      const int64_t f = e * 8 - na;
+      const int n = static_cast<int>(f / p.ldb), c = static_cast<int>(f - static_cast<int64_t>(n) * p.ldb);
+      int i = 0, row = n;
+      if (p.interleaved) {
+        i = (n >> 7) & 1;
+        row = (n >> 8) * 128 + (n & 127);
+      } else {
+        while (i + 1 < p.parts && n >= p.ends[i]) ++i;
+        row = n - (i ? p.ends[i - 1] : 0);
+      }
+      const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b[i]) + static_cast<int64_t>(row) * p.rank[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int own = c + j - p.off[i];
+        o.h[j] = own >= 0 && own < p.rank[i] ? b[own] : __float2bfloat16(0.f);
+      }
+      if (p.bias && c == p.R) o.h[0] = static_cast<const __nv_bfloat16*>(p.bias)[n];
+      reinterpret_cast<int4*>(p.b_out)[f / 8] = o.v;
+    }
+  }
+}
+
+}  // namespace prl
+
+using namespace prl;
+
+// layout 0: A [M, K], B [R, K]; 1: A [M, K], B [K, R]; 2: A [K, M], B [K, R]; 3: as 2, out [R, M].  Pitches in elements, multiples of 8.
+// pad > 0 (layouts 0 to 2): so many more columns of out, ones in the first.
+extern "C" int prl_lora_thin(const void* A, const void* B, void* out, int M, int R, int K, int64_t lda, int64_t ldb, int64_t ldo, float scale, int layout, int pad,
+                             int split, cudaStream_t stream) {
+  if (M <= 0 || R <= 0 || K <= 0) return 0;
+  if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || (layout != 3 && ldo % 4)) return -1;
+  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad};
+  switch (layout) {
+    case 0: return run_thin<false, false, false>(A, B, p, lda, ldb, split, stream);
+    case 1: return run_thin<false, true, false>(A, B, p, lda, ldb, split, stream);
+    case 2: return run_thin<true, true, false>(A, B, p, lda, ldb, split, stream);
+    case 3: return run_thin<true, true, true>(A, B, p, lda, ldb, split, stream);
+  }
+  return -5;
+}
+
+extern "C" int prl_lora_pack(const prl::LoraPackParams* q, cudaStream_t stream) {
+  const int64_t units = (static_cast<int64_t>(q->R) * q->K + static_cast<int64_t>(q->N) * q->ldb) / 8;
+  if (q->K % 8 || q->ldb % 8 || q->R % 8) return -1;
+  const int64_t blocks = (units + 255) / 256;
+  lora_pack_kernel<<<static_cast<unsigned>(blocks < 8 * 148 ? blocks : 8 * 148), 256, 0, stream>>>(*q);
+  PRL_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}

@@ -105,6 +105,8 @@ from .adapters import (  # noqa: E402
     adapter_linear,
     adapter_linear_swiglu,
     adapter_plan,
+    lora_linear,
+    lora_linear_swiglu,
 )
 from .logits import LogitRules, adjust_logits, token_mask  # noqa: E402
 
@@ -128,6 +130,8 @@ __all__ = [
     "adapter_linear",
     "adapter_linear_swiglu",
     "adapter_plan",
+    "lora_linear",
+    "lora_linear_swiglu",
     "LogitRules",
     "adjust_logits",
     "token_mask",

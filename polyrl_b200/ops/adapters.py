@@ -1,5 +1,8 @@
 """Low-rank adapters beside a shared projection.
 
+``lora_linear`` / ``lora_linear_swiglu``: a (frozen) projection with one adapter, with gradients: the trainer's LoRA path (csrc/lora.cu,
+gemm2_sm100.cuh).  Reference capability: peft LoRA layers through FSDP (3rdparty/verl/verl/workers/fsdp_workers.py:269-577).
+
 ``adapter_plan`` / ``adapter_linear`` / ``adapter_linear_swiglu``: inference over rows that belong to requests with different adapters, or none
 (csrc/adapters.cu; plain PyTorch on CPU tensors).  Reference capability: the adapters that the SGLang server of a rollout worker serves by
 name; the reference's trainer merges its one adapter before rollout (3rdparty/verl/verl/utils/fsdp_utils.py:569-694)."""
@@ -142,3 +145,134 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
     if fn._stream_swiglu(x, wgu):
         return _C().stream_gemm(x, wgu, d, None, None, None, 2, 0, None, -1)
     return _C().gemm_swiglu_add(x, wgu, d)
+
+
+# --------------------------------------------------------------------------------------------
+# one adapter, trained
+# --------------------------------------------------------------------------------------------
+def _lora_reference(x, w, parts, widths, scale, bias, residual, interleaved):
+    """The plain form, which autograd differentiates: library products."""
+    deltas = [torch.nn.functional.linear(torch.nn.functional.linear(x, p[0].to(x.dtype)), p[1].to(x.dtype)) if p is not None
+              else x.new_zeros(*x.shape[:-1], m) for p, m in zip(parts, widths)]
+    if interleaved:
+        lead, f = x.shape[:-1], widths[0]
+        d = torch.stack([t.reshape(*lead, f // 128, 128) for t in deltas], dim=-2).reshape(*lead, 2 * f)
+    else:
+        d = torch.cat(deltas, dim=-1) if len(deltas) > 1 else deltas[0]
+    return fn.linear(x, w, bias, residual) + d * scale
+
+
+class _LoraFn(torch.autograd.Function):
+    """x [T, K] through w [N, K] and the adapters a0, b0, a1, b1, ... (None, None: a part without).  swiglu: gate and up interleaved."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, scale, widths, swiglu, *ab):
+        C = _C()
+        x = _rows(x)
+        w = fn._g2_operand(w)
+        a, b = ([None if t is None else t.contiguous() for t in ab[i::2]] for i in (0, 1))
+        ranks = [0 if t is None else t.shape[0] for t in a]
+        if len(a) == 1 and bias is None and ranks[0] % 8 == 0 and a[0].data_ptr() % 16 == 0 and b[0].data_ptr() % 16 == 0:
+            pa, pb = a[0], b[0]
+        else:
+            pa, pb = C.lora_pack([None if t is None else fn._aligned(t) for t in a], b, list(widths), swiglu, bias)
+        t = C.lora_thin(x, pa, 0, scale, 0, pb.shape[1] - pa.shape[0])
+        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or any(ctx.needs_input_grad[7:])
+        gu = None
+        if swiglu:
+            y, *rest = C.lora_gemm_swiglu(x, w, t, pb, need)
+            gu = rest[0] if rest else None
+        else:
+            r = residual
+            if r is not None and not (r.is_contiguous() and r.data_ptr() % 16 == 0):
+                r = fn._aligned(r)
+            y = C.lora_gemm(x, w, t, pb, False, r)
+        if need:
+            ctx.save_for_backward(x, w, pa, pb, t, *([gu] if swiglu else []))
+        ctx.meta = (scale, widths, swiglu, ranks)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        C = _C()
+        scale, widths, swiglu, ranks = ctx.meta
+        need = ctx.needs_input_grad
+        dres = dy if need[3] else None
+        dbias = dy.sum(0) if need[2] else None
+        if not (need[0] or need[1] or any(need[7:])):
+            return (None, None, dbias, dres, *[None] * (3 + 2 * len(ranks)))
+        x, w, pa, pb, t, *gu = ctx.saved_tensors
+        dy = C.swiglu_bwd(gu[0], fn._aligned(dy)) if swiglu else _rows(dy)
+        r = pa.shape[0]
+        dx = dw = da = db = None
+        if need[0] or any(need[7::2]):
+            dt = C.lora_thin(dy, pb, 1, scale, r)
+            if need[0]:
+                dx = C.lora_gemm(dy, w, dt, pa, True)
+            if any(need[7::2]):
+                da = C.lora_thin(x, dt, 3)
+        if any(need[8::2]):
+            db = C.lora_thin(dy, t, 2, 1.0, r)
+        if need[1]:
+            dw = fn.mm_tn(dy, x, out=fn._sink_for(w))
+        grads, col, row = [], 0, 0
+        for i, (rank, m) in enumerate(zip(ranks, widths)):
+            grads.append(da[col:col + rank] if rank and need[7 + 2 * i] else None)
+            if rank and need[8 + 2 * i]:
+                mine = db.view(-1, 2, 128, r)[:, i].reshape(m, r) if swiglu else db[row:row + m]
+                grads.append(mine[:, col:col + rank])
+            else:
+                grads.append(None)
+            col, row = col + -(-rank // 8) * 8, row + m
+        return (dx, dw, dbias, dres, None, None, None, *grads)
+
+
+def _check_lora(name, x, w, parts, bias=None, residual=None) -> tuple:
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"{name}: rows {tuple(x.shape)} do not fit a projection {tuple(w.shape)}")
+    widths = []
+    for p in parts:
+        if isinstance(p, int):
+            widths.append(p)
+            continue
+        a, b = p
+        if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[1] != w.shape[1] or a.shape[0] < 1:
+            raise ValueError(f"{name}: A [rank, {w.shape[1]}] and B [columns, rank] expected, not {tuple(a.shape)} and {tuple(b.shape)}")
+        if a.device != x.device or b.device != x.device:
+            raise ValueError(f"{name}: adapters on {a.device} and {b.device}, rows on {x.device}")
+        widths.append(b.shape[0])
+    if not 1 <= len(parts) <= 3 or any(m < 1 for m in widths) or sum(widths) != w.shape[0]:
+        raise ValueError(f"{name}: parts of {widths} columns do not make up the projection's {w.shape[0]}")
+    if bias is not None and bias.shape != w.shape[:1] or residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
+        raise ValueError(f"{name}: bias [N], residual [.., N]")
+    return tuple(widths)
+
+
+def _lora(x, w, parts, widths, scale, bias, residual, swiglu):
+    adapters = [None if isinstance(p, int) else p for p in parts]
+    kernel = fn._is_kernel_tensor(x) and not fn._cublas() and w.dtype == torch.bfloat16 and fn._g2_ok(*w.shape) and any(p is not None for p in adapters) \
+        and x.numel() > 0 and all(t is None or t.dtype == torch.bfloat16 for t in (bias, residual))
+    if not kernel:
+        y = _lora_reference(x, w, adapters, widths, scale, bias, residual, swiglu)
+        return ref.swiglu(y) if swiglu else y
+    ab = [t for p in adapters for t in ((None, None) if p is None else (p[0].to(x.dtype), p[1].to(x.dtype)))]
+    y = _LoraFn.apply(x.reshape(-1, x.shape[-1]), w, bias, None if residual is None else residual.reshape(-1, w.shape[0]), float(scale), widths, swiglu, *ab)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, parts, scale: float, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x @ w.T + scale * (x @ A.T) @ B.T (+ bias) (+ residual), with gradients of everything (``w`` is frozen as a rule).
+
+    ``parts``: the projection's slices of columns in order, each an adapter (A [rank, K], B [columns, rank]) or, without one, its number of
+    columns: ``[(qa, qb), 1024, (va, vb)]``.  Ranks may differ.  What the adapters add is part of the product's fp32 sums."""
+    parts = list(parts)
+    return _lora(x, w, parts, _check_lora("lora_linear", x, w, parts, bias, residual), scale, bias, residual, False)
+
+
+def lora_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, gate, up, scale: float) -> torch.Tensor:
+    """``linear_swiglu`` with adapters on gate and up (each (A [rank, K], B [F, rank]) or None), which act before the activation."""
+    f = wgu.shape[0] // 2
+    parts = [f if p is None else p for p in (gate, up)]
+    if wgu.shape[0] % 256 or _check_lora("lora_linear_swiglu", x, wgu, parts) != (f, f):
+        raise ValueError("lora_linear_swiglu: gate and up in blocks of 128 rows each")
+    return _lora(x, wgu, parts, (f, f), scale, None, None, True)

@@ -28,11 +28,11 @@ MODULES: dict[str, dict] = {
                "cu": ["gemm_tcgen05.cu", "gemm2.cu", "attn_fwd.cu", "decode_attn.cu", "sampling.cu", "mix_elem.cu", "mix_scan.cu", "mix_chunk.cu", "mix_chunk_tc.cu", "mix_delta.cu", "mix_latent.cu",
                       "mix_window.cu", "mix_maps.cu", "mix_block.cu", "mix_experts.cu", "mix_streams.cu", "mix_selective.cu", "mix_gla.cu", "logit_rules.cu", "adapters.cu"]},
     "_C": {"bindings": "bindings.cpp",
-           "cu": ["gemm_tcgen05.cu", "gemm2.cu", "gemm2_grads.cu", "skinny_gemm.cu", "decode_gemm.cu", "vmm.cu", "linear_ce.cu", "ag_gemm.cu", "elementwise.cu", "qk_rope.cu",
+           "cu": ["gemm_tcgen05.cu", "gemm2.cu", "gemm2_grads.cu", "skinny_gemm.cu", "decode_gemm.cu", "vmm.cu", "linear_ce.cu", "lora.cu", "ag_gemm.cu", "elementwise.cu", "qk_rope.cu",
                   "optim.cu", "attn_bwd.cu", "attn_fwd.cu", "p2p.cu", "nvls.cu"]},
 }
-HEADERS = ["common.cuh", "gemm_sm100.cuh", "gemm2_sm100.cuh", "mixers.cuh", "mix_tc.cuh", "mix_params.hpp", "logit_rules.hpp", "adapters.hpp"]
-HOST_HEADERS = ["kv_manager.hpp", "scheduler.hpp", "bindings_common.hpp", "bindings_requests.hpp", "mix_params.hpp", "logit_rules.hpp", "adapters.hpp"]          # included by the bindings only
+HEADERS = ["common.cuh", "gemm_sm100.cuh", "gemm2_sm100.cuh", "mixers.cuh", "mix_tc.cuh", "mix_params.hpp", "logit_rules.hpp", "adapters.hpp", "lora.hpp"]
+HOST_HEADERS = ["kv_manager.hpp", "scheduler.hpp", "bindings_common.hpp", "bindings_requests.hpp", "mix_params.hpp", "logit_rules.hpp", "adapters.hpp", "lora.hpp"]          # included by the bindings only
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

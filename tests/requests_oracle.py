@@ -122,3 +122,83 @@ def swiglu64(z, err):
     eg, eu = e[..., 0, :].flatten(-2), e[..., 1, :].flatten(-2)
     s = g / (1 + torch.exp(-g))
     return s * up, 1.1 * eg * (up.abs() + eu) + (s.abs() + 1.1 * eg) * eu + 2.0 ** -18 * (s * up).abs()
+
+
+def merged64(w, parts, widths, scale, interleaved=False):
+    """The projection's weight with its adapters in it."""
+    part = part_of(w.shape[0], widths, interleaved).to(w.device)
+    m = w.double().clone()
+    for i, p in enumerate(parts):
+        if p is not None:
+            cols = torch.nonzero(part == i).flatten()
+            m[cols] += scale * (p[1].double() @ p[0].double())
+    return m
+
+
+def lora_value64(x, w, parts, widths, scale, dy, bias=None, residual=None, swiglu=False):
+    """sum(dy * y) in 64 bits."""
+    z = x.double() @ merged64(w, parts, widths, scale, swiglu).t()
+    for extra in (bias, residual):
+        if extra is not None:
+            z = z + extra.double()
+    if swiglu:
+        v = z.unflatten(-1, (-1, 2, 128))
+        g, up = v[..., 0, :].flatten(-2), v[..., 1, :].flatten(-2)
+        z = g / (1 + torch.exp(-g)) * up
+    return (dy.double() * z).sum()
+
+
+def lora64(x, w, parts, widths, scale, dy, bias=None, residual=None, swiglu=False):
+    """{name: (value, bound before the last rounding)} of y, dx and of every part's da, db: low-rank values, their gradients and, with swiglu, the
+    projection and its gradient are rounded to bf16; sums in fp32."""
+    u = 2.0 ** -8
+    x, w, dy = x.double(), w.double(), dy.double()
+    (t_rows, k), n, dev = x.shape, w.shape[0], x.device
+    part = part_of(n, widths, swiglu).to(dev)
+    ab = [None if p is None else (p[0].double(), p[1].double()) for p in parts]
+    cols = [torch.nonzero(part == i).flatten() for i in range(len(widths))]
+    z, mag, err = x @ w.t(), x.abs() @ w.abs().t(), torch.zeros(t_rows, n, dtype=torch.float64, device=dev)
+    low = []
+    for c, p in zip(cols, ab):
+        if p is None:
+            low.append(None)
+            continue
+        a, b = p
+        t = scale * (x @ a.t())
+        et = u * t.abs() + (k + 3) * U32 * abs(scale) * (x.abs() @ a.abs().t())
+        z[:, c] += t @ b.t()
+        mag[:, c] += t.abs() @ b.abs().t()
+        err[:, c] += et @ b.abs().t()
+        low.append((t, et))
+    for extra in (bias, residual):
+        if extra is not None:
+            z, mag = z + extra.double(), mag + extra.double().abs()
+    err = err + (k + 400) * U32 * mag
+    out, ed = {}, torch.zeros_like(err)
+    if swiglu:
+        out["y"] = swiglu64(z, err)
+        v, e = z.unflatten(-1, (-1, 2, 128)), (err + u * (z.abs() + err)).unflatten(-1, (-1, 2, 128))
+        g, up, eg, eu = v[..., 0, :].flatten(-2), v[..., 1, :].flatten(-2), e[..., 0, :].flatten(-2), e[..., 1, :].flatten(-2)
+        s = 1 / (1 + torch.exp(-g))
+        d1 = s * (1 + g * (1 - s))                                         # silu', |silu'| <= 1.1, |silu''| <= 1/2
+        dg, du = dy * up * d1, dy * g * s
+        edg = dy.abs() * (eu * d1.abs() + 0.5 * eg * (up.abs() + eu)) + 2.0 ** -18 * dy.abs() * up.abs() * (1 + g.abs())
+        edu = dy.abs() * 1.1 * eg + 2.0 ** -18 * (dy * g).abs()
+        edg, edu = edg + u * (dg.abs() + edg), edu + u * (du.abs() + edu)
+        join = lambda p, q: torch.stack([p.unflatten(-1, (-1, 128)), q.unflatten(-1, (-1, 128))], -2).flatten(-3)  # noqa: E731
+        dy, ed = join(dg, du), join(edg, edu)
+    else:
+        out["y"] = (z, err)
+    dx, edx, mdx = dy @ w, ed @ w.abs(), dy.abs() @ w.abs()
+    for i, (c, p, l) in enumerate(zip(cols, ab, low)):
+        if p is None:
+            continue
+        (a, b), (t, et), d, e = p, l, dy[:, c], ed[:, c]
+        dt = scale * (d @ b)
+        edt = abs(scale) * (e @ b.abs())
+        edt = edt + u * (dt.abs() + edt) + (n + 3) * U32 * abs(scale) * ((d.abs() + e) @ b.abs())
+        dx, edx, mdx = dx + dt @ a, edx + edt @ a.abs(), mdx + dt.abs() @ a.abs()
+        out[f"da{i}"] = (dt.t() @ x, edt.t() @ x.abs() + (t_rows + 8) * U32 * (dt.abs().t() @ x.abs()))
+        out[f"db{i}"] = (d.t() @ t, e.t() @ (t.abs() + et) + d.abs().t() @ et + (t_rows + 8) * U32 * (d.abs().t() @ t.abs()))
+    out["dx"] = (dx, edx + (n + 400) * U32 * (mdx + edx))
+    return out

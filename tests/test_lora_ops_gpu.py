@@ -1,0 +1,131 @@
+"""Trained adapters beside a projection: the sm_100a kernels against the 64-bit oracle and against differences of it."""
+import pytest
+import torch
+
+from polyrl_b200 import ops
+
+from .requests_oracle import check_near, half_step, lora64, lora_value64
+from .test_lora_ops_cpu import check_lora, lora_case, run_lora
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("m,r,k,split", [(1, 8, 64, 0), (128, 16, 64, 1), (130, 24, 200, 2), (300, 48, 4096, 8), (77, 256, 512, 4), (257, 264, 1000, 0), (64, 520, 136, 1)])
+@pytest.mark.parametrize("layout", [0, 1, 2, 3])
+def test_thin_products(layout, m, r, k, split):
+    g = torch.Generator().manual_seed(m + r)
+    m8 = (m + 7) // 8 * 8 if layout >= 2 else m
+    a, b = torch.randn(m8, k, generator=g).to(BF).cuda(), torch.randn(r, k, generator=g).to(BF).cuda()
+    ref, mag = 0.5 * (a.double() @ b.double().t()), 0.5 * (a.double().abs() @ b.double().abs().t())
+    pad = 8 if layout < 3 else 0
+    got = ops.ext().lora_thin(a.t().contiguous() if layout >= 2 else a, b if layout == 0 else b.t().contiguous(), layout, 0.5, 0, pad, split)
+    if layout == 3:
+        got = got.t()
+    else:
+        assert (got[:, r] == 1).all() and (got[:, r + 1:] == 0).all()
+        got = got[:, :r]
+    check_near(got, ref, (k + 2) * 2.0 ** -24 * mag)
+
+
+@pytest.mark.parametrize("t,k,widths,ranks", [
+    (1, 8, (8,), (1,)), (1, 64, (64,), (8,)), (3, 72, (40,), (5,)), (127, 896, (896, 128, 128), (8, 8, 8)), (129, 256, (128,), (16,)), (256, 200, (136,), (64,)),
+    (300, 896, (896, 128, 128), (3, 0, 20)), (515, 512, (512, 64, 64), (0, 16, 16)), (640, 2048, (896,), (128,)), (1000, 264, (264, 264, 264), (96, 88, 100)),
+    (2100, 1000, (520,), (64,))])
+@pytest.mark.parametrize("extra", [False, True])
+def test_lora_linear(t, k, widths, ranks, extra):
+    check_lora(lora_case(t, k, widths, ranks, t + k, BF, "cuda", bias=extra, residual=extra))
+
+
+@pytest.mark.parametrize("t,k,f,ranks", [(1, 64, 128, (8, 8)), (65, 896, 4864, (8, 8)), (300, 256, 512, (0, 5)), (301, 256, 512, (33, 0)), (777, 520, 1280, (64, 64))])
+def test_lora_linear_swiglu(t, k, f, ranks):
+    check_lora(lora_case(t, k, (f, f), ranks, t, BF, "cuda", swiglu=True))
+
+
+def test_adapters_part_is_not_lost_beside_a_frozen_bias():
+    """Every output that a subset of the leaves asks for, and the gradient of a trained weight."""
+    c = lora_case(200, 128, (128, 64), (8, 16), 0, BF, "cuda", bias=True, residual=True)
+    full = run_lora(c)
+    for need in (("x",), ("parts",), ()):
+        for name, t in run_lora(c, need).items():
+            assert torch.equal(t, full[name]), name
+    leaves = {n: c[n].detach().requires_grad_() for n in ("x", "w", "bias", "residual")}
+    y = ops.lora_linear(leaves["x"], leaves["w"], c["parts"], 2.0, leaves["bias"], leaves["residual"])
+    dx, dw, db, dr = torch.autograd.grad(y, list(leaves.values()), c["dy"])
+    assert torch.equal(dx, full["dx"]) and torch.equal(dr, c["dy"])
+    d, x = c["dy"].double(), c["x"].double()
+    check_near(dw, d.t() @ x, 202 * 2.0 ** -24 * (d.abs().t() @ x.abs()))
+    check_near(db, d.sum(0), 202 * 2.0 ** -24 * d.abs().sum(0))
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_gradients_against_differences(swiglu):
+    """Along a random direction, the kernels' gradients give the slope of the 64-bit value: to the sum of their bounds."""
+    c = lora_case(96, 128, (256, 256) if swiglu else (128, 64), (8, 4), 3, BF, "cuda", swiglu=swiglu)
+    ref, got = lora64(**c), run_lora(c)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for name, get, put in [("dx", lambda: c["x"], lambda v: dict(c, x=v))] + [
+            (f"d{n}{i}", lambda i=i, j=j: c["parts"][i][j], lambda v, i=i, j=j: dict(c, parts=[tuple(v if (a, b) == (i, j) else c["parts"][a][b] for b in (0, 1)) for a in (0, 1)]))
+            for i in (0, 1) for j, n in enumerate("ab")]:
+        at = get().double()
+        v = torch.randn(at.shape, generator=g, device="cuda", dtype=torch.float64)
+        h = 1e-4
+        slope = (lora_value64(**put(at + h * v)) - lora_value64(**put(at - h * v))) / (2 * h)
+        value, err = ref[name]
+        tol = ((err + half_step(BF) * (value.abs() + err)) * v.abs()).sum() + 1e-6 * (value.abs() * v.abs()).sum()
+        assert (slope - (got[name].double() * v).sum()).abs() <= tol
+        assert (slope - (value * v).sum()).abs() <= 1e-6 * (value.abs() * v.abs()).sum()
+
+
+def test_views_and_odd_starts():
+    c = lora_case(150, 64, (64, 32), (8, 8), 5, BF, "cuda", bias=True, residual=True)
+    full = run_lora(c)
+
+    def shifted(t, by):
+        buf = torch.empty(t.shape[0], t.shape[1] + 16, dtype=t.dtype, device="cuda")
+        v = buf[:, by:by + t.shape[1]]
+        v.copy_(t)
+        return v
+
+    for by in (8, 3):
+        o = dict(c, x=shifted(c["x"], by), w=shifted(c["w"], by), dy=shifted(c["dy"], by), residual=shifted(c["residual"], by),
+                 parts=[tuple(shifted(m, by) for m in p) for p in c["parts"]])
+        for name, t in run_lora(o).items():
+            assert torch.equal(t, full[name]), name
+
+
+def test_stream_and_graph():
+    c = lora_case(260, 128, (128, 64), (8, 8), 6, BF, "cuda", residual=True)
+    full = run_lora(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run_lora(c)
+        graph = torch.cuda.CUDAGraph()
+    side.synchronize()
+    assert all(torch.equal(got[n], full[n]) for n in full)
+    with torch.cuda.graph(graph):
+        got = run_lora(c)
+    c["x"].mul_(2.0)
+    graph.replay()
+    ref = lora64(**c)
+    for name, t in got.items():
+        check_near(t, *ref[name])
+
+
+def test_rows_that_are_not_finite_stay_alone():
+    c = lora_case(300, 128, (128,), (16,), 7, BF, "cuda")
+    full = run_lora(c)
+    x = c["x"].clone()
+    x[17], x[299] = float("nan"), float("inf")
+    got = run_lora(dict(c, x=x))
+    rest = torch.ones(300, dtype=torch.bool, device="cuda")
+    rest[[17, 299]] = False
+    for name in ("y", "dx"):
+        assert torch.equal(got[name][rest], full[name][rest])
+
+
+def test_no_rows():
+    c = lora_case(0, 64, (64,), (8,), 0, BF, "cuda")
+    got = run_lora(c)
+    assert got["y"].shape == (0, 64) and got["dx"].shape == (0, 64) and not got["da0"].any() and not got["db0"].any()

@@ -15,6 +15,7 @@ from dataclasses import dataclass
 
 import torch
 
+from .. import ops
 from ..ops import reference as ref
 from .config import ModelConfig
 
@@ -78,40 +79,36 @@ def lora_param_specs(cfg: ModelConfig, lcfg: LoraConfig) -> list[tuple[str, tupl
     return specs
 
 
-def _delta(x: torch.Tensor, w: dict, proj: str) -> torch.Tensor | None:
+def _part(w: dict, proj: str):
+    """The adapter of one projection, or None."""
     a = w.get(f"lora_{proj}_A")
-    if a is None:
-        return None
-    b = w[f"lora_{proj}_B"]
-    return torch.nn.functional.linear(torch.nn.functional.linear(x, a.to(x.dtype)), b.to(x.dtype))
+    return None if a is None else (a, w[f"lora_{proj}_B"])
 
 
 def has_lora(w: dict, *projs: str) -> bool:
     return any(f"lora_{p}_A" in w for p in projs)
 
 
-def qkv_delta(cfg: ModelConfig, w: dict, h: torch.Tensor) -> torch.Tensor:
-    """Low-rank update of the fused [q | k | v] projection output."""
+def qkv_linear(cfg: ModelConfig, w: dict, h: torch.Tensor) -> torch.Tensor:
+    """The fused [q | k | v] projection with the adapters of its parts."""
+    if not has_lora(w, "q_proj", "k_proj", "v_proj"):
+        return ops.linear(h, w["wqkv"], bias=w.get("bqkv"))
     dims = _proj_dims(cfg)
-    parts = []
-    for p in ("q_proj", "k_proj", "v_proj"):
-        d = _delta(h, w, p)
-        parts.append(d if d is not None else h.new_zeros(h.shape[0], dims[p][0]))
-    return torch.cat(parts, dim=-1) * w["_lora_scale"]
+    return ops.lora_linear(h, w["wqkv"], [_part(w, p) or dims[p][0] for p in ("q_proj", "k_proj", "v_proj")], w["_lora_scale"], bias=w.get("bqkv"))
 
 
-def single_delta(w: dict, x: torch.Tensor, proj: str) -> torch.Tensor:
-    return _delta(x, w, proj) * w["_lora_scale"]
+def single_linear(w: dict, x: torch.Tensor, name: str, proj: str, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Projection ``w[name]`` with the adapter of ``proj``, where it has one (+ residual)."""
+    if not has_lora(w, proj):
+        return ops.linear(x, w[name], residual=residual)
+    return ops.lora_linear(x, w[name], [_part(w, proj)], w["_lora_scale"], residual=residual)
 
 
-def gate_up_delta(cfg: ModelConfig, w: dict, h: torch.Tensor) -> torch.Tensor:
-    """Update of the block-interleaved [128 gate | 128 up] fused projection output."""
-    f = cfg.intermediate_size
-    t = h.shape[0]
-    dg, du = _delta(h, w, "gate_proj"), _delta(h, w, "up_proj")
-    dg = dg if dg is not None else h.new_zeros(t, f)
-    du = du if du is not None else h.new_zeros(t, f)
-    return torch.stack([dg.view(t, f // 128, 128), du.view(t, f // 128, 128)], dim=2).reshape(t, 2 * f) * w["_lora_scale"]
+def gate_up_swiglu(w: dict, h: torch.Tensor) -> torch.Tensor:
+    """silu(gate) * up of the block-interleaved [128 gate | 128 up] projection; adapters act before the activation."""
+    if not has_lora(w, "gate_proj", "up_proj"):
+        return ops.linear_swiglu(h, w["wgu"])
+    return ops.lora_linear_swiglu(h, w["wgu"], _part(w, "gate_proj"), _part(w, "up_proj"), w["_lora_scale"])
 
 
 @torch.no_grad()

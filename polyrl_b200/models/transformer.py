@@ -468,9 +468,7 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
                 raise NotImplementedError("LoRA adapters are not implemented for MLA attention")
             x = ops.linear(mla.attention_forward(cfg, w, h, inp, kv_sink), w["wo"], residual=x)
             return x if w.get("_skip_mlp") else _mlp_forward(cfg, w, x, aux_out)
-        qkv = ops.linear(h, w["wqkv"], bias=w.get("bqkv"))
-        if lora and L.has_lora(w, "q_proj", "k_proj", "v_proj"):
-            qkv = qkv + L.qkv_delta(cfg, w, h)
+        qkv = L.qkv_linear(cfg, w, h) if lora else ops.linear(h, w["wqkv"], bias=w.get("bqkv"))
         pos, cos, sin = inp.rope_inputs(cfg, x.device)
         a = None
         if kv_sink is not None:
@@ -498,14 +496,10 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
             a = attention_varlen(q, k, v, inp.cu_seqlens, inp.max_seqlen, causal=True)
         a = a.reshape(t, nq * d)
         if cfg.sandwich_norm:
-            o = ops.linear(a, w["wo"])
-            if lora and L.has_lora(w, "o_proj"):
-                o = o + L.single_delta(w, a, "o_proj")
+            o = L.single_linear(w, a, "wo", "o_proj") if lora else ops.linear(a, w["wo"])
             x = x + ops.rmsnorm(o, w["ln_attn"], cfg.rms_norm_eps)
         else:
-            x = ops.linear(a, w["wo"], residual=x)
-            if lora and L.has_lora(w, "o_proj"):
-                x = x + L.single_delta(w, a, "o_proj")
+            x = L.single_linear(w, a, "wo", "o_proj", residual=x) if lora else ops.linear(a, w["wo"], residual=x)
         if w.get("_skip_mlp"):              # callers that supply their own MLP (expert parallelism, parallel/expert.py)
             return x
         h, x = ops.rmsnorm_residual(x, w["ln2"], cfg.rms_norm_eps)
@@ -516,19 +510,11 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
             if lora:
                 raise NotImplementedError("LoRA adapters are not implemented for the xIELU MLP")
             return xielu_mlp(w, h, x)
-        if lora and L.has_lora(w, "gate_proj", "up_proj"):
-            a = ref.swiglu(ops.linear(h, w["wgu"]) + L.gate_up_delta(cfg, w, h))    # adapters act before the activation
-        else:
-            a = ops.linear_swiglu(h, w["wgu"])
+        a = L.gate_up_swiglu(w, h) if lora else ops.linear_swiglu(h, w["wgu"])
         if cfg.sandwich_norm:
-            y = ops.linear(a, w["wd"])
-            if lora and L.has_lora(w, "down_proj"):
-                y = y + L.single_delta(w, a, "down_proj")
+            y = L.single_linear(w, a, "wd", "down_proj") if lora else ops.linear(a, w["wd"])
             return x + ops.rmsnorm(y, w["ln_mlp"], cfg.rms_norm_eps)
-        y = ops.linear(a, w["wd"], residual=x)
-        if lora and L.has_lora(w, "down_proj"):
-            y = y + L.single_delta(w, a, "down_proj")
-        return y
+        return L.single_linear(w, a, "wd", "down_proj", residual=x) if lora else ops.linear(a, w["wd"], residual=x)
     # ---- gpt2 block (library ops; plumbing / CPU config)
     h = F.layer_norm(x, (cfg.hidden_size,), w["ln1_w"], w["ln1_b"], cfg.rms_norm_eps)
     qkv = F.linear(h, w["wqkv"], w["bqkv"])

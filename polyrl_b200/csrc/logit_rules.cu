@@ -8,167 +8,246 @@
 //
 // All in fp32, rounded once to the logits' type; what no rule touches is copied bit for bit (in place: not touched at all).
 //
-// Split: a block takes `chunk` consecutive tokens of the vocabulary of one row.  Its table in shared memory has a 32-bit word per token of
-// the chunk, addressed by the token itself, so nothing is hashed, sorted or kept between calls: the words are cleared, the row's biases and
-// stop tokens marked, its whole history read (coalesced, out of L2 for all but a row's first block) and counted with shared-memory atomics,
-// which are integers and therefore give the same words in any order.  Then the chunk is streamed once, 16 bytes a thread.
-#include <type_traits>
-
+// Split: a block takes a part of one row's vocabulary and has a word in shared memory for each of its tokens.  Half of its warps clear the words, read the
+// row's whole history (out of L2 for all but the row's first block) and count the tokens of the part with shared-memory atomics, while the other half
+// copy the part under the row's mask, 16 bytes a thread.  Then all of them look through the words for touched tokens, pack them 32 to a warp, compute
+// those logits from the input and write them over the copy.  In place only masked and touched tokens are written.  Nothing is hashed, sorted or kept
+// between calls; counters are integers, so results do not depend on the order of the threads.
+// Histories are sparse, so what bounds it is instructions before it is bytes.  A hashed table asked again for every token of the history ran its few hits
+// a warp one lane at a time (256 rows of 128256 bf16 logits with histories of up to 1100: 52 us); a list that the counting threads append to saves the
+// search but waits for every atomic's answer (24 rows with histories of 30011: 42 us).
 #include "common.cuh"
 #include "logit_rules.hpp"
 
 namespace prl {
 
-// word of the table: output count in the low 20 bits, "in the prompt", place in the bias list + 1
-constexpr uint32_t kCountMask = (1u << kRuleCountBits) - 1, kPrompt = 1u << kRuleCountBits;
-constexpr int kBiasShift = kRuleCountBits + 1;
-constexpr uint32_t kBanned = (1u << (32 - kBiasShift)) - 1;
-static_assert(kRuleMaxBias == kBanned - 1, "the last place means banned");
+// Word of a token: output count, then "in the prompt", "in the bias list", "may not come yet".  Adding to the count and setting bits commute.
+// 16 bits a token where the count fits 13, two tokens to a 32-bit word of memory: half the memory, so more blocks on an SM, and half the words
+// to clear and to look through.
+template <int BITS>
+struct RuleWord {
+  static constexpr int kCountBits = BITS == 16 ? kRuleShortBits : kRuleCountBits;
+  static constexpr uint32_t kCount = (1u << kCountBits) - 1, kPrompt = 1u << kCountBits, kBias = kPrompt << 1, kBanned = kPrompt << 2;
+  static_assert(kCountBits + 3 <= BITS);
+  static __device__ __forceinline__ void add(uint32_t* words, uint32_t at, uint32_t v) {
+    if (BITS == 16) atomicAdd(words + (at >> 1), v << (16 * (at & 1)));
+    else atomicAdd(words + at, v);
+  }
+  static __device__ __forceinline__ void mark(uint32_t* words, uint32_t at, uint32_t bit) {
+    if (BITS == 16) atomicOr(words + (at >> 1), bit << (16 * (at & 1)));
+    else atomicOr(words + at, bit);
+  }
+  // which of the words in 16 bytes are not clear, a bit each
+  static __device__ __forceinline__ uint32_t set(const uint4& q) {
+    if (BITS == 32) return (q.x != 0) | (q.y != 0) << 1 | (q.z != 0) << 2 | (q.w != 0) << 3;
+    const uint32_t a = __vsetne2(q.x, 0), b = __vsetne2(q.y, 0), c = __vsetne2(q.z, 0), d = __vsetne2(q.w, 0);
+    return ((a | a >> 15) & 3) | ((b | b >> 15) & 3) << 2 | ((c | c >> 15) & 3) << 4 | ((d | d >> 15) & 3) << 6;
+  }
+  static __device__ __forceinline__ uint32_t get(const uint32_t* words, int at) {
+    return BITS == 16 ? reinterpret_cast<const uint16_t*>(words)[at] : words[at];
+  }
+};
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16(v); }
 
-struct RowRules {
-  float rep, pres, freq;
-  const float* bias;
-  __device__ __forceinline__ float operator()(float z, uint32_t word) const {
-    if (word & (kCountMask | kPrompt)) z = z > 0.f ? z / rep : z * rep;
-    const uint32_t c = word & kCountMask, at = word >> kBiasShift;
-    if (c) z = z - freq * static_cast<float>(c) - pres;
-    if (at) z = at == kBanned ? -INFINITY : z + bias[at - 1];
-    return z;
-  }
-};
+__device__ __forceinline__ const uint32_t* mask_of(const RuleParams& p, int64_t row) {
+  if (!p.masks) return nullptr;
+  const int64_t m = p.mask_rows ? p.mask_rows[row] : row;
+  return m >= 0 && m < p.num_masks ? reinterpret_cast<const uint32_t*>(p.masks) + m * p.ld_masks : nullptr;
+}
 
-template <class T, int VEC, bool INPLACE>
-__global__ void __launch_bounds__(kRuleThreads) rules_kernel(RuleParams p, int chunks) {
-  extern __shared__ uint32_t table[];
-  const int row = blockIdx.x / chunks, base = (blockIdx.x % chunks) * p.chunk, size = min(p.chunk, p.V - base);
-  grid_behind();
-  const RowRules rr{p.rep ? p.rep[row] : 1.f, p.pres ? p.pres[row] : 0.f, p.freq ? p.freq[row] : 0.f,
-                    p.bias_ids ? p.bias_values + row * p.ld_bias : nullptr};
-  const int len = p.lens ? p.lens[row] : p.max_tokens;
-  const bool counts = p.tokens && (rr.rep != 1.f || rr.pres != 0.f || rr.freq != 0.f);
-  const bool early = p.stop_ids && len < p.min_lens[row];
-  const int mask_row = p.masks ? p.mask_rows ? p.mask_rows[row] : row : -1;
-  const uint32_t* mask = mask_row >= 0 && mask_row < p.num_masks ? reinterpret_cast<const uint32_t*>(p.masks) + mask_row * p.ld_masks + (base >> 5) : nullptr;
-  const bool words = counts || early || p.bias_ids != nullptr;
-  if (INPLACE && !words && !mask) return;
-
-  if (words) {
-    for (int i = threadIdx.x; i < p.chunk / 4; i += kRuleThreads) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    if (p.bias_ids)                                    // of entries with the same token the last one counts
-      for (int j = threadIdx.x; j < p.num_bias; j += kRuleThreads) {
-        const uint32_t at = static_cast<uint32_t>(p.bias_ids[row * p.ld_bias + j] - base);
-        if (at < static_cast<uint32_t>(size)) atomicMax(&table[at], static_cast<uint32_t>(j + 1) << kBiasShift);
-      }
-    if (early)
-      for (int j = threadIdx.x; j < p.num_stop; j += kRuleThreads) {
-        const uint32_t at = static_cast<uint32_t>(p.stop_ids[row * p.ld_stop + j] - base);
-        if (at < static_cast<uint32_t>(size)) atomicMax(&table[at], kBanned << kBiasShift);
-      }
-    __syncthreads();                                   // marks first: counts are added below them
-    if (counts) {
-      const int n = min(max(len, 0), p.max_tokens), prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
-      const int32_t* tok = p.tokens + row * p.ld_tokens;
-      int i = threadIdx.x;
-      for (; i + 3 * kRuleThreads < n; i += 4 * kRuleThreads) {
-        uint32_t at[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) at[u] = static_cast<uint32_t>(tok[i + u * kRuleThreads] - base);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (at[u] < static_cast<uint32_t>(size)) {
-            if (i + u * kRuleThreads < prompt) atomicOr(&table[at[u]], kPrompt);
-            else atomicAdd(&table[at[u]], 1u);
-          }
-      }
-      for (; i < n; i += kRuleThreads) {
-        const uint32_t at = static_cast<uint32_t>(tok[i] - base);
-        if (at >= static_cast<uint32_t>(size)) continue;
-        if (i < prompt) atomicOr(&table[at], kPrompt);
-        else atomicAdd(&table[at], 1u);
-      }
-    }
-    __syncthreads();
-  }
-
-  const T* z = static_cast<const T*>(p.z) + row * p.ldz + base;
-  T* out = static_cast<T*>(p.out) + row * p.ldo + base;
-  if constexpr (VEC > 1) {
-    using Raw = int4;
-    static_assert(sizeof(T) * VEC == sizeof(Raw));
-#pragma unroll 4
-    for (int i = threadIdx.x; i < size / VEC; i += kRuleThreads) {
-      const int v = i * VEC;
-      const uint32_t bits = mask ? mask[v >> 5] >> (v & 31) : ~0u;
-      uint32_t w[VEC], any = 0;
-#pragma unroll
-      for (int q = 0; q < VEC; q += 4) {
-        const uint4 t = words ? *reinterpret_cast<const uint4*>(table + v + q) : make_uint4(0, 0, 0, 0);
-        w[q] = t.x; w[q + 1] = t.y; w[q + 2] = t.z; w[q + 3] = t.w;
-        any |= t.x | t.y | t.z | t.w;
-      }
-      const bool all = (bits & ((1u << VEC) - 1)) == (1u << VEC) - 1;
-      if (INPLACE && all && !any) continue;
-      union { Raw raw; T e[VEC]; } x;
-      x.raw = INPLACE ? ld_v4(z + v) : ld_nc_v4(z + v);
-      if (any || !all) {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          if (w[q]) from_f32(rr(to_f32(x.e[q]), w[q]), x.e[q]);
-          if (!((bits >> q) & 1)) from_f32(-INFINITY, x.e[q]);
-        }
-      }
-      st_v4(out + v, x.raw);
-    }
-  }
-  // what is left of the row, or all of it where rows do not start on 16 bytes
-#pragma unroll 4
-  for (int v = (VEC > 1 ? size / VEC * VEC : 0) + threadIdx.x; v < size; v += kRuleThreads) {
-    const uint32_t word = words ? table[v] : 0;
-    const bool ok = !mask || ((mask[v >> 5] >> (v & 31)) & 1);
-    if (INPLACE && ok && !word) continue;
+// Tokens [0, size) of a part from z to out under its mask, 16 bytes at a time between the first and the last 16-byte boundary inside (rows start
+// anywhere; where z and out start differently, token by token).  In place nothing but masked tokens is touched.
+template <class T, bool INPLACE>
+__device__ __forceinline__ void copy_part(const T* z, T* out, int size, const uint32_t* mask, int tid, int threads) {
+  constexpr int VEC = 16 / sizeof(T), kVecs = 4;
+  constexpr uint32_t kAll = (1u << VEC) - 1;
+  if (INPLACE && !mask) return;
+  auto one = [&](int v) {
+    const bool ok = !mask || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1);
+    if (INPLACE && ok) return;
     T e = z[v];
-    if (word) from_f32(rr(to_f32(e), word), e);
     if (!ok) from_f32(-INFINITY, e);
     out[v] = e;
+  };
+  const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const int head = alike ? min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) % 16 / sizeof(T)), size) : size;
+  const int tail = head + (size - head) / VEC * VEC;
+#pragma unroll 8
+  for (int v = tid; v < head; v += threads) one(v);
+  for (int v = tail + tid; v < size; v += threads) one(v);
+  for (int v0 = head + tid * VEC; v0 < tail; v0 += kVecs * threads * VEC) {
+    int4 x[kVecs];
+    uint32_t bits[kVecs];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int v = v0 + j * threads * VEC;
+      if (v >= tail) continue;
+      if constexpr (!INPLACE) x[j] = ld_nc_v4(z + v);
+      bits[j] = mask ? __funnelshift_r(__ldg(mask + (v >> 5)), __ldg(mask + ((v + VEC - 1) >> 5)), v & 31) & kAll : kAll;
+    }
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int v = v0 + j * threads * VEC;
+      if (v >= tail || (INPLACE && bits[j] == kAll)) continue;
+      if constexpr (INPLACE) {
+        if (bits[j] != 0) x[j] = ld_v4(z + v);
+      }
+      if (bits[j] != kAll) {
+        int* w = reinterpret_cast<int*>(&x[j]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (VEC == 4) {
+            if (!((bits[j] >> q) & 1)) w[q] = static_cast<int>(0xff800000u);
+          } else {                                     // a pair of bf16: all ones over what stays, -inf over what does not
+            const int lo = static_cast<int>(bits[j] << (31 - 2 * q)) >> 31, hi = static_cast<int>(bits[j] << (30 - 2 * q)) >> 31;
+            const int keep = __byte_perm(lo, hi, 0x5410);
+            w[q] = (w[q] & keep) | (static_cast<int>(0xff80ff80u) & ~keep);
+          }
+        }
+      }
+      st_v4(out + v, x[j]);
+    }
   }
 }
 
-template <class T>
-static int run_rules(const RuleParams& p, cudaStream_t stream) {
-  const int chunks = (p.V + p.chunk - 1) / p.chunk;
-  const int64_t blocks = static_cast<int64_t>(p.rows) * chunks;
-  if (blocks > 0x7fffffff) return -3;
-  constexpr int VEC = 16 / sizeof(T);
-  const bool inplace = p.z == p.out;
-  const bool wide = ((reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 && p.ldz % VEC == 0 && p.ldo % VEC == 0;
-  auto kern = wide ? inplace ? rules_kernel<T, VEC, true> : rules_kernel<T, VEC, false> : inplace ? rules_kernel<T, 1, true> : rules_kernel<T, 1, false>;
-  const size_t smem = p.chunk * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleMaxChunk * 4);
-    if (e != cudaSuccess) return static_cast<int>(e);
+template <class T, bool INPLACE, int BITS>
+__global__ void __launch_bounds__(kRuleThreads, 3) rules_kernel(RuleParams p, int parts, int part) {
+  constexpr int kAhead = 6;                            // tokens a thread has in flight
+  constexpr int kCounting = kRuleThreads / 2;
+  using Word = RuleWord<BITS>;
+  constexpr int kEach = 128 / BITS, kStep = 32 * kEach;          // tokens a lane and a warp look at together
+  extern __shared__ __align__(16) uint32_t words[];    // [part] words of BITS bits, the row's bias list
+  __shared__ uint16_t packed[kRuleThreads / 32][32 + kStep];     // a warp packs touched tokens until it has 32
+  int32_t* bias_ids = reinterpret_cast<int32_t*>(words + part * BITS / 32);
+  const int64_t row = blockIdx.x / parts;
+  const int tid = threadIdx.x, base = static_cast<int>(blockIdx.x % parts) * part, size = min(part, p.V - base);
+  grid_behind();
+  const T* z = static_cast<const T*>(p.z) + row * p.ldz + base;
+  T* out = static_cast<T*>(p.out) + row * p.ldo + base;
+  if (!INPLACE && tid == 0) {                          // on its way into L2 while the history is counted
+    const uintptr_t from = (reinterpret_cast<uintptr_t>(z) + 15) & ~uintptr_t(15), to = reinterpret_cast<uintptr_t>(z + size) & ~uintptr_t(15);
+    if (to > from) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(static_cast<uint32_t>(to - from)) : "memory");
   }
-  PRL_CUDA_CHECK(launch_behind(kern, static_cast<unsigned>(blocks), kRuleThreads, smem, stream, p, chunks));
+  // everything that has an address now is asked for now: a block is a few loads deep and little else
+  const int32_t* tok = p.tokens + row * p.ld_tokens;
+  int32_t token[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) token[u] = tid < kCounting && tid + u * kCounting < p.max_tokens ? __ldg(tok + tid + u * kCounting) : -1;
+  const int len = p.lens ? p.lens[row] : p.max_tokens, prompt = p.prompt_lens ? p.prompt_lens[row] : 0, least = p.num_stop > 0 ? p.min_lens[row] : 0;
+  const float rep = p.rep ? p.rep[row] : 1.f, pres = p.pres ? p.pres[row] : 0.f, freq = p.freq ? p.freq[row] : 0.f;
+  const uint32_t* mask = mask_of(p, row);
+  if (mask) mask += base >> 5;
+  const bool early = p.num_stop > 0 && len < least;
+  const int n = rep != 1.f || pres != 0.f || freq != 0.f ? min(len, p.max_tokens) : 0;
+  if (n <= 0 && !early && p.num_bias == 0) {
+    copy_part<T, INPLACE>(z, out, size, mask, tid, kRuleThreads);
+    return;
+  }
+  if (tid < kCounting) {                               // half of the warps count while the other half copies: both are latencies more than work
+    for (int j = tid; j < p.num_bias; j += kCounting) bias_ids[j] = p.bias_ids[row * p.ld_bias + j];
+    for (int i = tid; i < part * BITS / 128; i += kCounting) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("bar.sync 1, %0;" ::"n"(kCounting) : "memory");
+    for (int i0 = tid; i0 < n; i0 += kAhead * kCounting) {
+      if (i0 != tid) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) token[u] = i0 + u * kCounting < n ? __ldg(tok + i0 + u * kCounting) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t at = static_cast<uint32_t>(token[u] - base);
+        const int i = i0 + u * kCounting;
+        if (i < n && at < static_cast<uint32_t>(size)) {
+          if (i < prompt) Word::mark(words, at, Word::kPrompt);
+          else Word::add(words, at, 1u);
+        }
+      }
+    }
+    for (int j = tid; j < p.num_bias; j += kCounting) {
+      const uint32_t at = static_cast<uint32_t>(bias_ids[j] - base);
+      if (at < static_cast<uint32_t>(size)) Word::mark(words, at, Word::kBias);
+    }
+    if (early)
+      for (int j = tid; j < p.num_stop; j += kCounting) {
+        const uint32_t at = static_cast<uint32_t>(p.stop_ids[row * p.ld_stop + j] - base);
+        if (at < static_cast<uint32_t>(size)) Word::mark(words, at, Word::kBanned);
+      }
+  } else {
+    copy_part<T, INPLACE>(z, out, size, mask, tid - kCounting, kRuleThreads - kCounting);
+  }
+  __syncthreads();                                     // the words are complete, the copy is written
+
+  const int lane = tid & 31, warp = tid >> 5;
+  uint16_t* mine = packed[warp];
+  auto put = [&](int at) {                             // the token `at` of the part, a touched one
+    const uint32_t w = Word::get(words, at), bits = mask ? __ldg(mask + (at >> 5)) : ~0u;
+    float v = to_f32(z[at]);
+    if (w & (Word::kCount | Word::kPrompt)) v = v > 0.f ? v / rep : v * rep;
+    const uint32_t c = w & Word::kCount;
+    if (c) v = v - freq * static_cast<float>(c) - pres;
+    if (w & Word::kBias) {                             // of entries with the same token the last one counts
+      int j = p.num_bias - 1;
+      while (bias_ids[j] != base + at) --j;
+      v += p.bias_values[row * p.ld_bias + j];
+    }
+    T o;
+    from_f32((w & Word::kBanned) || !((bits >> (at & 31)) & 1) ? -INFINITY : v, o);
+    out[at] = o;
+  };
+  int count = 0;                                       // tokens packed and not yet written, the same for the whole warp
+  for (int i0 = warp * kStep; i0 < size; i0 += kRuleThreads * kEach) {            // (clear behind `size`)
+    uint32_t set = Word::set(*reinterpret_cast<const uint4*>(words + (i0 + lane * kEach) * BITS / 32));
+    if (!__any_sync(0xffffffffu, set)) continue;
+    int upto = __popc(set);
+    const int own = upto;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    for (int to = count + upto - own; set; set &= set - 1) mine[to++] = static_cast<uint16_t>(i0 + lane * kEach + __ffs(set) - 1);
+    count += __shfl_sync(0xffffffffu, upto, 31);
+    __syncwarp();
+    if (count < 32) continue;
+    int from = 0;
+    for (; count - from >= 32; from += 32) put(mine[from + lane]);
+    const int rest = count - from;
+    const uint16_t keep = lane < rest ? mine[from + lane] : 0;
+    __syncwarp();
+    if (lane < rest) mine[lane] = keep;
+    __syncwarp();
+    count = rest;
+  }
+  if (lane < count) put(mine[lane]);
+}
+
+template <class T, int BITS>
+static int run_rules(const RuleParams& p, cudaStream_t stream) {
+  // parts as wide as leave some blocks for every SM: each of them reads the row's history
+  int part = kRulePart;
+  while (part > 2048 && static_cast<int64_t>(p.rows) * ((p.V + part - 1) / part) < 2 * 148) part /= 2;
+  const int parts = (p.V + part - 1) / part;
+  const int64_t blocks = static_cast<int64_t>(p.rows) * parts;
+  if (blocks > 0x7fffffff) return -3;
+  auto kern = p.z == p.out ? rules_kernel<T, true, BITS> : rules_kernel<T, false, BITS>;
+  const size_t smem = part * BITS / 8 + 4 * static_cast<size_t>(p.num_bias);
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRulePart * BITS / 8 + 4 * kRuleMaxBias));
+  PRL_CUDA_CHECK(launch_behind(kern, static_cast<unsigned>(blocks), kRuleThreads, smem, stream, p, parts, part));
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
 }
 
 }  // namespace prl
 
-// p.chunk 0: chosen here.  A block reads the row's whole history, so long histories want wide chunks; few rows want many blocks.
 extern "C" int prl_adjust_logits(const prl::RuleParams* q, int fp32, cudaStream_t stream) {
   prl::RuleParams p = *q;
   if (p.rows <= 0 || p.V <= 0) return 0;
   if (p.num_bias > prl::kRuleMaxBias || p.max_tokens >= (1 << prl::kRuleCountBits)) return -1;
-  if (p.chunk <= 0) {
-    p.chunk = 16384;
-    while (p.chunk > 2048 && static_cast<int64_t>(p.rows) * ((p.V + p.chunk - 1) / p.chunk) < 2 * 148) p.chunk >>= 1;
-  }
-  if (p.chunk % 128 || p.chunk > prl::kRuleMaxChunk) return -2;
-  return fp32 ? prl::run_rules<float>(p, stream) : prl::run_rules<__nv_bfloat16>(p, stream);
+  if (!(p.rep || p.pres || p.freq)) p.max_tokens = 0;            // nothing counts the tokens
+  if (p.z == p.out && !p.masks && p.max_tokens + p.num_bias + p.num_stop == 0) return 0;
+  if (p.max_tokens < (1 << prl::kRuleShortBits)) return fp32 ? prl::run_rules<float, 16>(p, stream) : prl::run_rules<__nv_bfloat16, 16>(p, stream);
+  return fp32 ? prl::run_rules<float, 32>(p, stream) : prl::run_rules<__nv_bfloat16, 32>(p, stream);
 }

@@ -4,10 +4,11 @@
 
 namespace prl {
 
-constexpr int kRuleThreads = 256;
-constexpr int kRuleMaxChunk = 32768;
+constexpr int kRuleThreads = 512;
 constexpr int kRuleCountBits = 20;                  // a history is shorter than 2^20 tokens
+constexpr int kRuleShortBits = 13;                  // shorter than 2^13: 16 bits a token
 constexpr int kRuleMaxBias = 2046;                  // entries of a row's bias list
+constexpr int kRulePart = 16384;                    // most tokens of the vocabulary a block takes: their places are packed into 16 bits
 
 // Strides in elements.  A pointer that is null leaves its rule out.
 struct RuleParams {
@@ -32,7 +33,6 @@ struct RuleParams {
   int64_t ld_masks;
   int num_masks;
   const int32_t* mask_rows;        // [rows]: the row's mask, negative for none; null: mask b belongs to row b
-  int chunk;
 };
 
 }  // namespace prl

@@ -9,8 +9,8 @@ from dataclasses import dataclass, fields
 
 import torch
 
-MAX_HISTORY = 1 << 20          # tokens of a row's history, and entries of its bias list: what the kernel's table words hold
-MAX_BIAS = 2046
+MAX_HISTORY = 1 << 20          # tokens of a row's history: what the kernel's counters hold
+MAX_BIAS = 2046                # entries of a row's bias list
 
 
 @dataclass
@@ -92,13 +92,13 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | N
           -> -inf                                             where the mask, or the least length, does not let it come
 
     in fp32, rounded once.  The kernel may be captured; no gradient."""
-    _check(logits, rules, out)
-    if logits.is_cuda:
+    if logits.is_cuda:                   # (checks its arguments as _check does)
         from . import ext
 
         r = rules
         return ext().adjust_logits(logits, out, r.tokens, r.lens, r.prompt_lens, r.repetition, r.presence, r.frequency, r.bias_ids, r.bias_values, r.stop_ids,
                                    r.min_lens, r.masks, r.mask_rows)
+    _check(logits, rules, out)
     z = _adjust_reference(logits, rules)
     return z if out is None else out.copy_(z)
 

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 # ------------------------------------------------------------------------------------------------------------------ rules
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("rows,v,n,m", [(1, 1, 1, 1), (1, 31, 0, 0), (3, 32, 5, 3), (2, 2047, 300, 9), (5, 2048, 17, 40), (4, 4104, 1500, 7), (3, 16390, 999, 2046)])
+@pytest.mark.parametrize("rows,v,n,m", [(1, 1, 1, 1), (1, 31, 0, 0), (3, 32, 5, 3), (2, 2047, 300, 9), (5, 2048, 17, 40), (4, 4104, 1500, 7), (3, 16390, 999, 2046), (2, 33000, 8300, 30), (3, 100, 9000, 3)])
 def test_rules(rows, v, n, m, dtype):
     z, case = rules_case(rows, v, n, rows * 7 + v, dtype, "cuda", m)
     z0 = z.clone()
@@ -71,12 +71,23 @@ def test_rules_strides_views_and_odd_starts():
 
 def test_rules_refused_by_the_kernel_entry():
     z = torch.randn(4, 64, device="cuda")
-    with pytest.raises(ValueError, match="cuda"):
+    with pytest.raises(ValueError, match="device"):
         ops.adjust_logits(z, LogitRules(tokens=torch.zeros(4, 3, dtype=torch.int32)))
-    with pytest.raises(RuntimeError, match="apart"):
+    with pytest.raises(ValueError, match="apart"):
         ops.adjust_logits(z[:2], LogitRules(), out=z[1:3])
-    with pytest.raises(RuntimeError, match="unit inner stride"):
+    with pytest.raises(ValueError, match="unit inner stride"):
         ops.adjust_logits(z.t(), LogitRules())
+    _, c = rules_case(4, 64, 6, 0, torch.float32, "cuda")
+    for kw in [dict(lens=c["lens"][:2], tokens=c["tokens"]), dict(tokens=c["tokens"].long()), dict(repetition=c["repetition"].double(), tokens=c["tokens"]),
+               dict(presence=c["presence"]), dict(tokens=torch.zeros(4, 1, dtype=torch.int32, device="cuda").expand(4, 1 << 20)), dict(bias_ids=c["bias_ids"]),
+               dict(bias_ids=c["bias_ids"], bias_values=c["bias_values"][:, :2]), dict(bias_ids=c["bias_ids"].repeat(1, 500), bias_values=c["bias_values"].repeat(1, 500)),
+               dict(stop_ids=c["stop_ids"], lens=c["lens"]), dict(stop_ids=c["stop_ids"], min_lens=c["min_lens"]), dict(mask_rows=c["mask_rows"]),
+               dict(masks=c["masks"][:, :1], mask_rows=c["mask_rows"]), dict(masks=c["masks"][:2])]:
+        with pytest.raises(ValueError, match="adjust_logits"):
+            ops.adjust_logits(z, LogitRules(**kw))
+    for bad, out in ((z.half(), None), (z[0], None), (z, z[:2]), (z, z.bfloat16())):
+        with pytest.raises(ValueError, match="adjust_logits"):
+            ops.adjust_logits(bad, LogitRules(), out=out)
 
 
 def test_rules_stream_and_graph():
@@ -215,7 +226,7 @@ def test_adapters_views_streams_and_graph():
 def test_adapters_refused_by_the_kernel_entry():
     c = adapters_case(4, 64, (64,), 16, 2, 0, torch.bfloat16, "cuda")
     plan = ops.adapter_plan(c["ids"], 2)
-    with pytest.raises(RuntimeError, match="unit inner stride"):
+    with pytest.raises(ValueError, match="unit inner stride"):
         ops.adapter_linear(c["x"], c["w"], c["a"], c["b"].transpose(1, 2).contiguous().transpose(1, 2), c["scales"], plan)
     with pytest.raises(ValueError, match="plan is of"):
         ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"].cpu(), 2))

@@ -3,8 +3,9 @@
 //   out[i, n] = s_l * sum_r B_l[n, r] * t_i[p(n) * rank + r]  (+ bias[n]) (+ res[i, n]),     t_i = A_l x_i,   l = ids[i]
 //
 // p(n) is the part of the fused projection that column n belongs to (query / key / value, or gate / up in blocks of 128).  A row without
-// an adapter gets bias and residual alone.  The shared product adds `out` to its fp32 sums before it rounds, so a result is rounded once
-// more than without adapters only in the small term: t and out are bf16 (relative 2^-9 each of what the adapter adds).
+// an adapter gets bias and residual alone.  With few rows the shared product comes first and this is added to it (`onto`): a row without an adapter
+// then is what it is in a batch that has none, and any other is rounded twice, as bf16 2^-8 of the value at most each time.  With many rows this
+// comes first, and the shared product adds it to its fp32 sums before it rounds.  t is rounded to bf16, as an operand of the second product.
 //
 // plan   one block sorts the rows by adapter (stable, by counting) and cuts every adapter's rows into tiles.  One plan serves all
 //        projections of a step.
@@ -14,7 +15,9 @@
 //        The lanes' k-indices (and the columns of the second product) are permuted so that a lane's fragments are contiguous in memory:
 //        both operands of a product use the same permutation, and sums do not mind.
 //        Ranks are a few dozen, so the products are bound by their operands' bytes and mma.sync keeps up; tcgen05 would want 128 rows of
-//        one adapter and a round trip through tensor memory, longer than the whole kernel at decode.
+//        one adapter and a round trip through tensor memory, longer than the whole kernel at decode.  What bounds it is latency: loads, two
+//        cluster barriers and loads again, in 5.2 us for one row (K 896, N 1152), 9.8 for 128 rows of 24 adapters (4096, 6144, rank 16; 17 MB),
+//        18.5 for 45 rows of 9 (3584, 37888, rank 32; 30 MB), 50 for 5003 rows of 5 (2048, 2048, rank 64; 64 MB).
 #include "adapters.hpp"
 #include "common.cuh"
 
@@ -90,7 +93,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
 }
 
 // ------------------------------------------------------------------------------------------------------------ delta
-constexpr int kDeltaThreads = 256, kDeltaWarps = 8;
 constexpr int kLowChunk = 64;                        // low-rank columns whose sums a warp holds at a time
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -115,16 +117,18 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t a) {
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 
-// shared memory: partial sums [TM][R] fp32, those of the warps that split K [KW][TM][kLowChunk], t [TM][R + 8] bf16
+// TM rows a tile.  Shared memory: partial sums [TM][R] fp32, those of the KW warps that split K [KW][TM][kLowChunk], t [TM][R + 8] bf16 (rows an odd
+// number of 16-byte units apart)
 template <int TM>
-struct DeltaSmem {
-  static constexpr int KW = kDeltaWarps / (TM / 16);
-  static int bytes(int R) { return TM * R * 4 + KW * TM * kLowChunk * 4 + TM * (R + 8) * 2; }
+struct DeltaCfg {
+  static constexpr int MT = TM / 16, WARPS = 8, THREADS = 32 * WARPS, KW = WARPS / MT;
+  static int smem(int R) { return TM * R * 4 + KW * TM * kLowChunk * 4 + TM * (R + 8) * 2; }
 };
 
 template <int TM>
-__global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams p) {
-  constexpr int MT = TM / 16, KW = DeltaSmem<TM>::KW;
+__global__ void __launch_bounds__(DeltaCfg<TM>::THREADS, 2) delta_kernel(const DeltaParams p) {
+  using Cfg = DeltaCfg<TM>;
+  constexpr int MT = Cfg::MT, KW = Cfg::KW, kThreads = Cfg::THREADS;
   extern __shared__ __align__(16) uint8_t raw[];
   const int R = p.parts * p.rank, ldt = R + 8;
   float* part = reinterpret_cast<float*>(raw);
@@ -134,14 +138,25 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, grp = lane >> 2;
   const uint32_t cs = cluster_size(), rank = cluster_ctarank();
-  const int t = blockIdx.x / cs;
+  const int cluster = blockIdx.x / cs, t = cluster / p.shares, share = cluster % p.shares * cs + rank, shares = p.shares * cs;
   grid_behind();
   if (t >= *p.num_tiles) return;
   const AdapterTile tile = p.tiles[t];
   if (tid < TM) rows_sm[tid] = tid < tile.rows ? p.order[tile.first + tid] : -1;
   __syncthreads();
 
+  // this CTA's columns, 32 at a time, and its first weights of the second product, which can come while the first one runs
+  const int groups = p.N / 32, g0 = static_cast<int>(static_cast<int64_t>(groups) * share / shares),
+            g1 = static_cast<int>(static_cast<int64_t>(groups) * (share + 1) / shares);
+  // lane's place in the rows of b for 32 columns from `col`: a lane's columns of the four products are 8 consecutive ones
+  auto b_row = [&](int col) {
+    return static_cast<const __nv_bfloat16*>(p.b) + (static_cast<int64_t>(tile.adapter) * p.N + col + 8 * (grp >> 1) + (grp & 1)) * p.rank;
+  };
   if (tile.adapter >= 0) {
+    if (tid == 0 && g0 < g1)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const __nv_bfloat16*>(p.b) + (static_cast<int64_t>(tile.adapter) * p.N + g0 * 32) * p.rank),
+                   "r"((g1 - g0) * 64 * p.rank)
+                   : "memory");
     // ---- t = A x over this CTA's share of K
     const int mt = warp % MT, kw = warp / MT;
     const int steps = p.K / 32, s0 = steps * rank / cs, s1 = steps * (rank + 1) / cs;
@@ -153,8 +168,7 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
       const int nt = min(kLowChunk, R - c0) / 8;
       const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + (static_cast<int64_t>(tile.adapter) * R + c0 + grp) * p.K + quad * 8;
       float acc[8][4] = {};
-      const bool busy = mt * 16 < tile.rows;
-      if (busy) {
+      if (mt * 16 < tile.rows) {
 #pragma unroll 2
         for (int s = s0 + kw; s < s1; s += KW) {
           const int4 u = r0 >= 0 ? __ldg(reinterpret_cast<const int4*>(x0 + s * 32)) : zero;
@@ -179,12 +193,15 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
           *reinterpret_cast<float2*>(dst + 8 * kLowChunk + j * 8) = make_float2(acc[j][2], acc[j][3]);
         }
       __syncthreads();
-      for (int e = tid; e < TM * nt * 8; e += kDeltaThreads) {
-        const int m = e / (nt * 8), c = e % (nt * 8);
-        float v = 0.f;
+      for (int e = tid; e < tile.rows * nt * 4; e += kThreads) {
+        const int m = e / (nt * 4), c = e % (nt * 4) * 2;
+        float2 v = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < KW; ++k) v += red[(k * TM + m) * kLowChunk + c];
-        part[m * R + c0 + c] = v;
+        for (int k = 0; k < KW; ++k) {
+          const float2 q = *reinterpret_cast<const float2*>(red + (k * TM + m) * kLowChunk + c);
+          v.x += q.x; v.y += q.y;
+        }
+        *reinterpret_cast<float2*>(part + m * R + c0 + c) = v;
       }
       __syncthreads();
     }
@@ -192,16 +209,19 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
     const float scale = p.scales[tile.adapter];
     if (cs > 1) cluster_sync_all();
     const int pairs = tile.rows * (R / 2), e1 = pairs * (rank + 1) / cs;
-    for (int e = pairs * rank / cs + tid; e < e1; e += kDeltaThreads) {
+    for (int e = pairs * rank / cs + tid; e < e1; e += kThreads) {
       const int m = e / (R / 2), c = e % (R / 2) * 2;
       float2 v = make_float2(0.f, 0.f);
       if (cs == 1) {
         v = *reinterpret_cast<float2*>(part + m * R + c);
       } else {
-        for (uint32_t k = 0; k < cs; ++k) {
-          const float2 q = ld_cluster_f2(map_shared(part + m * R + c, k));
-          v.x += q.x; v.y += q.y;
-        }
+        float2 q[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+          if (k < cs) q[k] = ld_cluster_f2(map_shared(part + m * R + c, k));
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+          if (k < cs) { v.x += q[k].x; v.y += q[k].y; }
       }
       const uint32_t packed = pack_bf16(scale * v.x, scale * v.y);
       if (cs == 1) {
@@ -214,55 +234,68 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
     else __syncthreads();
   }
 
-  // ---- out = t B^T (+ bias) (+ res) over this CTA's share of the columns, 32 at a time: a lane ends up with 8 consecutive ones
-  const int groups = p.N / 32, g1 = groups * (rank + 1) / cs;
-  const int ksteps = p.rank / 16;
-  for (int g = groups * rank / cs + warp; g < g1; g += kDeltaWarps) {
+  // ---- out = t B^T (+ bias) (+ res) (+ base) over this CTA's share of the columns
+  for (int g = g0 + warp; g < g1; g += Cfg::WARPS) {
     const int col = g * 32;
     const int pt = p.interleaved ? (col >> 7) & 1 : (p.parts > 1 && col >= p.ends[0]) + (p.parts > 2 && col >= p.ends[1]);
-    int4 extra = make_int4(0, 0, 0, 0);
-    if (p.bias) extra = __ldg(reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.bias) + col + quad * 8));
-    int4 res[MT][2];
+    const int4 none = make_int4(0, 0, 0, 0);
+    const int4 extra = p.bias ? __ldg(reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.bias) + col + quad * 8)) : none;
+    int4 add[MT][2], own[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = rows_sm[m * 16 + grp + 8 * h];
-        res[m][h] = p.res && row >= 0 ? ld_nc_v4(static_cast<const __nv_bfloat16*>(p.res) + static_cast<int64_t>(row) * p.ldr + col + quad * 8) : make_int4(0, 0, 0, 0);
+        add[m][h] = p.res && row >= 0 ? ld_nc_v4(static_cast<const __nv_bfloat16*>(p.res) + static_cast<int64_t>(row) * p.ldr + col + quad * 8) : none;
+        own[m][h] = p.onto && row >= 0 ? ld_v4(static_cast<const __nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8) : none;
       }
     float acc[MT][4][4] = {};
     if (tile.adapter >= 0) {
-      const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b) + (static_cast<int64_t>(tile.adapter) * p.N + col + 8 * (grp >> 1) + (grp & 1)) * p.rank + quad * 4;
-      const __nv_bfloat16* tl = low + pt * p.rank + quad * 4;
+      const __nv_bfloat16* b = b_row(col);
+      const __nv_bfloat16* tl = low + pt * p.rank;
+      int k = 0;
 #pragma unroll 2
-      for (int k = 0; k < ksteps; ++k) {
-        uint2 w[4];
+      for (; k + 32 <= p.rank; k += 32) {            // 16 bytes a lane: two steps of 16
+        int4 w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint2*>(b + 2 * j * p.rank + k * 16));
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const int4*>(b + 2 * j * p.rank + k + quad * 8));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          if (MT > 1 && m * 16 >= tile.rows) break;
-          const uint2 u = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp) * ldt + k * 16);
-          const uint2 v = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp + 8) * ldt + k * 16);
+          const int4 u = *reinterpret_cast<const int4*>(tl + (m * 16 + grp) * ldt + k + quad * 8);
+          const int4 v = *reinterpret_cast<const int4*>(tl + (m * 16 + grp + 8) * ldt + k + quad * 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_bf16(acc[m][j], u.x, v.x, u.y, v.y, w[j].x, w[j].y);
+            mma_bf16(acc[m][j], u.z, v.z, u.w, v.w, w[j].z, w[j].w);
+          }
+        }
+      }
+      if (k < p.rank) {
+        uint2 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint2*>(b + 2 * j * p.rank + k + quad * 4));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint2 u = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp) * ldt + k + quad * 4);
+          const uint2 v = *reinterpret_cast<const uint2*>(tl + (m * 16 + grp + 8) * ldt + k + quad * 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_bf16(acc[m][j], u.x, v.x, u.y, v.y, w[j].x, w[j].y);
         }
       }
     }
-    const uint32_t ex[4] = {static_cast<uint32_t>(extra.x), static_cast<uint32_t>(extra.y), static_cast<uint32_t>(extra.z), static_cast<uint32_t>(extra.w)};
+    const uint32_t* ex = reinterpret_cast<const uint32_t*>(&extra);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = rows_sm[m * 16 + grp + 8 * h];
         if (row < 0) continue;
-        const uint32_t rv[4] = {static_cast<uint32_t>(res[m][h].x), static_cast<uint32_t>(res[m][h].y), static_cast<uint32_t>(res[m][h].z),
-                                static_cast<uint32_t>(res[m][h].w)};
+        const uint32_t *rv = reinterpret_cast<const uint32_t*>(&add[m][h]), *ov = reinterpret_cast<const uint32_t*>(&own[m][h]);
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 e = unpack_bf16(ex[j]), r = unpack_bf16(rv[j]);
-          o[j] = pack_bf16(acc[m][j][2 * h] + e.x + r.x, acc[m][j][2 * h + 1] + e.y + r.y);
+          const float2 e = unpack_bf16(ex[j]), r = unpack_bf16(rv[j]), y = unpack_bf16(ov[j]);
+          o[j] = pack_bf16(acc[m][j][2 * h] + e.x + r.x + y.x, acc[m][j][2 * h + 1] + e.y + r.y + y.y);
         }
         st_v4(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8,
               make_int4(static_cast<int>(o[0]), static_cast<int>(o[1]), static_cast<int>(o[2]), static_cast<int>(o[3])));
@@ -272,12 +305,12 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const DeltaParams 
 
 template <int TM>
 static int run_delta(const DeltaParams& p, int ctas, cudaStream_t stream) {
-  const int smem = DeltaSmem<TM>::bytes(p.parts * p.rank);
+  const int smem = DeltaCfg<TM>::smem(p.parts * p.rank);
   auto kern = delta_kernel<TM>;
-  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaSmem<TM>::bytes(kDeltaMaxLow)));
+  PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaCfg<TM>::smem(kDeltaMaxLow)));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles) * ctas);
-  cfg.blockDim = dim3(kDeltaThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles) * p.shares * ctas);
+  cfg.blockDim = dim3(DeltaCfg<TM>::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -305,18 +338,24 @@ extern "C" int prl_adapter_plan(const int32_t* ids, int T, int L, int tile_rows,
   return 0;
 }
 
-// tile_rows 16 or 64, as the plan was made; ctas: of a tile's cluster, 0 = as many (8 at most) as leave about four for every SM
-extern "C" int prl_adapter_delta(const prl::DeltaParams* q, int tile_rows, int ctas, cudaStream_t stream) {
-  const prl::DeltaParams& p = *q;
+// tile_rows 16 or 32, as the plan was made; ctas: of a cluster, shares: clusters that take a tile's columns between them, each with the whole first
+// product; 0 = as many CTAs (8 at most) as leave about four for every SM, and where that leaves fewer than one, more shares of at least 512 columns a CTA
+extern "C" int prl_adapter_delta(const prl::DeltaParams* q, int tile_rows, int ctas, int shares, cudaStream_t stream) {
+  prl::DeltaParams p = *q;
   if (p.max_tiles <= 0) return 0;
   if (p.K <= 0 || p.K % 32 || p.N <= 0 || p.N % 32 || p.rank < 16 || p.rank % 16 || p.parts < 1 || p.parts > 3 || p.parts * p.rank > prl::kDeltaMaxLow) return -1;
   if (ctas <= 0) {
     ctas = 8;
     while (ctas > 1 && static_cast<int64_t>(p.max_tiles) * ctas > 4 * 148) ctas >>= 1;
   }
+  if (shares <= 0) {
+    shares = 1;
+    while (static_cast<int64_t>(p.max_tiles) * ctas * shares < 148 && p.N / (2 * shares * ctas) >= 512) shares *= 2;
+  }
   if (ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) return -2;
-  if (static_cast<int64_t>(p.max_tiles) * ctas > 0x7fffffff) return -3;
+  p.shares = shares;
+  if (static_cast<int64_t>(p.max_tiles) * ctas * shares > 0x7fffffff) return -3;
   if (tile_rows == 16) return prl::run_delta<16>(p, ctas, stream);
-  if (tile_rows == 64) return prl::run_delta<64>(p, ctas, stream);
+  if (tile_rows == 32) return prl::run_delta<32>(p, ctas, stream);
   return -4;
 }

@@ -27,6 +27,8 @@ struct DeltaParams {
   int K, N, rank, parts, max_tiles;
   int ends[3];                     // column where each part ends; interleaved: parts alternate in blocks of 128 columns
   int interleaved;
+  int onto;                        // out holds the shared product: added to
+  int shares;                      // clusters a tile
 };
 
 }  // namespace prl

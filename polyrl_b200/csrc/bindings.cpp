@@ -616,6 +616,43 @@ std::vector<at::Tensor> lora_gemm_swiglu(const at::Tensor& x, const at::Tensor& 
   return {h};
 }
 
+// Forward of lora_linear and lora_linear_swiglu in one call: {y, A and B as the products take them, t, the projection (swiglu and save)}
+std::vector<at::Tensor> lora_fwd(const at::Tensor& x, const at::Tensor& w, const std::vector<OptT>& a, const std::vector<OptT>& b, const std::vector<int64_t>& widths,
+                                 double scale, bool swiglu, const OptT& bias, const OptT& residual, bool save) {
+  TORCH_CHECK(a.size() == widths.size() && b.size() == widths.size() && !a.empty(), "lora_fwd: parts");
+  at::Tensor pa, pb;
+  const auto fits = [](const at::Tensor& t) { return t.stride(-1) == 1 && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; };
+  if (a.size() == 1 && !bias.has_value() && a[0]->size(0) % 8 == 0 && fits(*a[0]) && fits(*b[0])) {
+    pa = *a[0];
+    pb = *b[0];
+  } else {
+    const std::vector<at::Tensor> p = lora_pack(a, b, widths, swiglu, bias);
+    pa = p[0];
+    pb = p[1];
+  }
+  const at::Tensor t = lora_thin(x, pa, 0, scale, 0, pb.size(1) - pa.size(0), 0);
+  if (!swiglu) return {lora_gemm(x, w, t, pb, false, residual), pa, pb, t};
+  std::vector<at::Tensor> y = lora_gemm_swiglu(x, w, t, pb, save);
+  if (save) return {y[0], pa, pb, t, y[1]};
+  return {y[0], pa, pb, t};
+}
+
+// and the backward: {dx, dA [R, K], dB [N, R]}, undefined where not asked for
+std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const at::Tensor& pa, const at::Tensor& pb, const at::Tensor& t, double scale,
+                           bool need_x, bool need_a, bool need_b) {
+  const int64_t r = pa.size(0);
+  OptT dx, da, db;
+  if (need_x || need_a) {
+    const at::Tensor dt = lora_thin(dy, pb, 1, scale, r, 0, 0);
+    if (need_b) db = lora_thin(dy, t, 2, 1.0, r, 0, 0);          // right behind the other product that reads dy
+    if (need_x) dx = lora_gemm(dy, w, dt, pa, true, c10::nullopt);
+    if (need_a) da = lora_thin(x, dt, 3, 1.0, 0, 0, 0);
+  } else if (need_b) {
+    db = lora_thin(dy, t, 2, 1.0, r, 0, 0);
+  }
+  return {dx, da, db};
+}
+
 // Row-parallel TP linear with the all-reduce fused into the GEMM epilogue over NVLink peer memory.
 at::Tensor skinny_gemm_tp(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& residual,
                           at::Tensor workspace, at::Tensor counters, int64_t splits, const std::vector<int64_t>& inbox_ptrs,
@@ -804,7 +841,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("force_bn") = 0);
   m.def("skinny_gemm", &skinny_gemm);
   m.def("skinny_gemm_tp", &skinny_gemm_tp);
-  m.def("lora_pack", &lora_pack);
+  m.def("lora_fwd", &lora_fwd);
+  m.def("lora_bwd", &lora_bwd);
   m.def("lora_thin", &lora_thin, py::arg("a"), py::arg("b"), py::arg("layout"), py::arg("scale") = 1.0, py::arg("rank") = 0, py::arg("pad") = 0,
         py::arg("split") = 0);
   m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("b"), py::arg("b_mn") = false, py::arg("residual") = py::none());

@@ -8,7 +8,7 @@
 extern "C" {
 int prl_adjust_logits(const prl::RuleParams*, int, cudaStream_t);
 int prl_adapter_plan(const int32_t*, int, int, int, int, int32_t*, void*, int32_t*, cudaStream_t);
-int prl_adapter_delta(const prl::DeltaParams*, int, int, cudaStream_t);
+int prl_adapter_delta(const prl::DeltaParams*, int, int, int, cudaStream_t);
 }
 
 namespace {
@@ -106,7 +106,8 @@ const void* delta_operand(const at::Tensor& t, const at::Tensor& x, const char* 
 
 // what the adapters of the rows add to x W^T, with bias and residual, as bf16 [T, N] (adapters.cu)
 at::Tensor adapter_delta(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scales, const at::Tensor& plan, int64_t tile_rows,
-                         int64_t max_tiles, const std::vector<int64_t>& widths, bool interleaved, const OptTensor& bias, const OptTensor& residual, int64_t ctas) {
+                         int64_t max_tiles, const std::vector<int64_t>& widths, bool interleaved, const OptTensor& bias, const OptTensor& residual, const OptTensor& onto, int64_t ctas,
+                         int64_t shares) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && a.dim() == 3 && b.dim() == 3, "adapter_delta: x [T, K], a [adapters, parts * rank, K], b [adapters, N, rank]");
   prl::DeltaParams p{};
   const int64_t T = x.size(0), K = x.size(1), L = a.size(0), N = b.size(1), rank = b.size(2), parts = widths.size();
@@ -134,13 +135,17 @@ at::Tensor adapter_delta(const at::Tensor& x, const at::Tensor& a, const at::Ten
     p.ldr = residual->stride(0);
   }
   c10::cuda::CUDAGuard g(x.device());
-  at::Tensor out = at::empty({T, N}, x.options());
+  if (onto.has_value())
+    TORCH_CHECK_VALUE(onto->dim() == 2 && onto->is_contiguous() && onto->size(0) == T && onto->size(1) == N && delta_operand(*onto, x, "adapter_delta: onto"),
+                      "adapter_delta: onto [T, N]");
+  at::Tensor out = onto.has_value() ? *onto : at::empty({T, N}, x.options());
   if (T == 0) return out;
+  p.onto = onto.has_value();
   const int32_t* pl = plan.data_ptr<int32_t>();
   p.scales = scales.data_ptr<float>(); p.out = out.data_ptr(); p.num_tiles = pl; p.tiles = reinterpret_cast<const prl::AdapterTile*>(pl + 4);
   p.order = pl + 4 + 4 * max_tiles; p.ldx = x.stride(0); p.ldo = N; p.K = K; p.N = N; p.rank = rank; p.parts = parts; p.max_tiles = max_tiles;
   p.interleaved = interleaved;
-  check(prl_adapter_delta(&p, tile_rows, ctas, cur_stream()), "adapter_delta");
+  check(prl_adapter_delta(&p, tile_rows, ctas, shares, cur_stream()), "adapter_delta");
   return out;
 }
 

@@ -1057,7 +1057,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_swiglu_add", &gemm_swiglu_add);
   m.def("adapter_plan", &adapter_plan);
   m.def("adapter_delta", &adapter_delta, py::arg("x"), py::arg("a"), py::arg("b"), py::arg("scales"), py::arg("plan"), py::arg("tile_rows"), py::arg("max_tiles"),
-        py::arg("widths"), py::arg("interleaved"), py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("ctas") = 0);
+        py::arg("widths"), py::arg("interleaved"), py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("onto") = py::none(),
+        py::arg("ctas") = 0, py::arg("shares") = 0);
   m.def("mix_embed", &mix_embed);
   m.def("mix_norm_add_", &mix_norm_add_);
   m.def("mix_rms", &mix_rms);

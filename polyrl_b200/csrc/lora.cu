@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  grid_behind();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -137,45 +138,45 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
     tmem_dealloc(tmem, tmem_cols);
   }
 
+  // four columns of a row, summed over the ranks
   const uint32_t base = smem_u32(smem);
-  auto peer = [&](uint32_t k) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base), "r"(k));
-    return a;
+  auto sum = [&](int row, int c) {
+    const uint32_t off = base + (row * (p.NR + 4) + c) * 4;
+    float4 q[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k)
+      if (k < S)
+        asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+                     : "=f"(q[k].x), "=f"(q[k].y), "=f"(q[k].z), "=f"(q[k].w)
+                     : "r"(off), "r"(k)
+                     : "memory");
+    float4 v = q[0];
+#pragma unroll
+    for (uint32_t k = 1; k < 8; ++k)
+      if (k < S) { v.x += q[k].x; v.y += q[k].y; v.z += q[k].z; v.w += q[k].w; }
+    return make_float4(v.x * p.scale, v.y * p.scale, v.z * p.scale, v.w * p.scale);
   };
+  const int cols = min(p.NR, p.R - r0);
   if constexpr (!TRANS) {                            // a share of the rows, four columns a thread
     const int rows0 = kBlockM * rank / S, rows1 = kBlockM * (rank + 1) / S;
-    const int cols = min(p.NR, p.R - r0), last = blockIdx.y + 1 == gridDim.y ? p.pad : 0, quads = (cols + last) / 4;
+    const int last = blockIdx.y + 1 == gridDim.y ? p.pad : 0, quads = (cols + last) / 4;
     for (int e = threadIdx.x; e < (rows1 - rows0) * quads; e += kThinThreads) {
       const int row = rows0 + e / quads, c = e % quads * 4;
       if (m0 + row >= p.M) break;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c < cols) {
-        const uint32_t off = (row * (p.NR + 4) + c) * 4;
-        for (uint32_t k = 0; k < S; ++k) {
-          float4 q;
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(peer(k) + off) : "memory");
-          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-        }
-        v.x *= p.scale; v.y *= p.scale; v.z *= p.scale; v.w *= p.scale;
-      } else if (c == cols) {
-        v.x = 1.f;
-      }
+      const float4 v = c < cols ? sum(row, c) : make_float4(c == cols ? 1.f : 0.f, 0.f, 0.f, 0.f);
       *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(m0 + row) * p.ldo + r0 + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     }
   } else {                                           // a share of the columns, lanes along the tile's rows
-    const int cols = min(p.NR, p.R - r0), c0 = cols * rank / S, c1 = cols * (rank + 1) / S;
-    for (int e = threadIdx.x; e < (c1 - c0) * kBlockM; e += kThinThreads) {
-      const int c = c0 + e / kBlockM, row = e % kBlockM;
+    const int quads = cols / 4, q0 = quads * rank / S, q1 = quads * (rank + 1) / S;
+    for (int e = threadIdx.x; e < (q1 - q0) * kBlockM; e += kThinThreads) {
+      const int c = (q0 + e / kBlockM) * 4, row = e % kBlockM;
       if (m0 + row >= p.M) continue;
-      const uint32_t off = (row * (p.NR + 4) + c) * 4;
-      float v = 0.f;
-      for (uint32_t k = 0; k < S; ++k) {
-        float q;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(peer(k) + off) : "memory");
-        v += q;
-      }
-      p.out[static_cast<int64_t>(r0 + c) * p.ldo + m0 + row] = __float2bfloat16(p.scale * v);
+      const float4 v = sum(row, c);
+      __nv_bfloat16* o = p.out + static_cast<int64_t>(r0 + c) * p.ldo + m0 + row;
+      o[0] = __float2bfloat16(v.x);
+      o[p.ldo] = __float2bfloat16(v.y);
+      o[2 * p.ldo] = __float2bfloat16(v.z);
+      o[3 * p.ldo] = __float2bfloat16(v.w);
     }
   }
   cluster_sync_all();                                // a peer may still read this CTA's sums
@@ -194,8 +195,13 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
   const int tiles = (p.M + kBlockM - 1) / kBlockM, blocks = (p.R + p.NR - 1) / p.NR, num_kb = (p.K + 63) / 64;
   int S = split;
   if (S <= 0) {
+    // CTAs for every SM; clusters of eight only where four leave half of the chip idle (they are harder to place, and sum over more CTAs).
+    // 64 tiles of 64 k-blocks, 48 columns, 1, 2, 4 and 8 CTAs: 26.7, 16.2, 12.1, 19.8 us; 32 tiles of 128 (dA): 49, 30, 24, 36; 224 tiles of 94: 57, 65,
+    // 78, 97; 16 tiles of 65, 64 columns: 27.8, 17.1, 11.4, 10.3.
+    const int64_t whole = static_cast<int64_t>(tiles) * blocks;
     S = 1;
-    while (S < 8 && static_cast<int64_t>(tiles) * blocks * S < 200 && num_kb / (2 * S) >= 4) S *= 2;
+    while (S < 4 && whole * S < 148 && num_kb >= 2 * S) S *= 2;
+    if (S == 4 && whole * S < 74 && num_kb >= 32) S = 8;
   }
   if (S > 8 || S > num_kb || (S & (S - 1))) return -4;
   auto kern = thin_kernel<A_MN, B_MN, TRANS>;
@@ -205,12 +211,14 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
   cfg.blockDim = dim3(kThinThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = S;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   PRL_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, static_cast<const ThinParams>(p)));
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
@@ -218,6 +226,7 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
 
 // ------------------------------------------------------------------------------------------------------------ pack
 __global__ void __launch_bounds__(256) lora_pack_kernel(const LoraPackParams p) {
+  grid_behind();
   const int64_t na = static_cast<int64_t>(p.R) * p.K, nb = static_cast<int64_t>(p.N) * p.ldb;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e * 8 < na + nb; e += static_cast<int64_t>(gridDim.x) * 256) {
     union { int4 v; __nv_bfloat16 h[8]; } o;
@@ -275,7 +284,7 @@ extern "C" int prl_lora_pack(const prl::LoraPackParams* q, cudaStream_t stream) 
   const int64_t units = (static_cast<int64_t>(q->R) * q->K + static_cast<int64_t>(q->N) * q->ldb) / 8;
   if (q->K % 8 || q->ldb % 8 || q->R % 8) return -1;
   const int64_t blocks = (units + 255) / 256;
-  lora_pack_kernel<<<static_cast<unsigned>(blocks < 8 * 148 ? blocks : 8 * 148), 256, 0, stream>>>(*q);
+  PRL_CUDA_CHECK(launch_behind(lora_pack_kernel, static_cast<unsigned>(blocks < 8 * 148 ? blocks : 8 * 148), 256, 0, stream, *q));
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
 }

@@ -46,7 +46,7 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     t = ids.shape[0]
     if not ids.is_cuda:
         return AdapterPlan(ids, num_adapters)
-    tile = 16 if t <= 256 else 64
+    tile = 16 if t <= 256 else 32
     groups = min(num_adapters + 1, t)
     most = (t - groups) // tile + groups           # tiles: the groups' rows, each rounded up
     return AdapterPlan(ids, num_adapters, tile, most, _C().adapter_plan(ids, num_adapters, tile, most))
@@ -77,9 +77,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else fn._aligned(t)
 
 
-def _delta(x, a, b, scales, plan, widths, interleaved, bias, residual):
+def _delta(x, a, b, scales, plan, widths, interleaved, bias=None, residual=None, onto=None):
     return _C().adapter_delta(_rows(x), a, b, scales, plan.buf, plan.tile_rows, plan.max_tiles, list(widths), interleaved,
-                              None if bias is None else fn._aligned(bias), None if residual is None else _rows(residual))
+                              None if bias is None else fn._aligned(bias), None if residual is None else _rows(residual), onto)
 
 
 def _delta_reference(x, a, b, scales, ids, widths, interleaved):
@@ -103,24 +103,19 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
 
         y_i = w x_i + scales[l] * b[l] (a[l] x_i)  (+ bias) (+ residual_i)
 
-    ``widths``: the columns of a fused projection's parts (query, key, value), each with ``rank`` rows of ``a`` [adapters, parts * rank, K] and its
-    rows of ``b`` [adapters, N, rank]; an adapter that leaves a part alone has zeros there.  Ranks are multiples of 16 (smaller ones are padded with
-    zeros).  What the adapters add is rounded to the rows' type before the product's sums are added to it.  Inference only."""
+    ``widths``: the columns of a fused projection's parts (query, key, value), each with ``rank`` rows of ``a`` [adapters, parts * rank, K] and
+    its rows of ``b`` [adapters, N, rank]; an adapter that leaves a part alone has zeros there.  Ranks are multiples of 16 (smaller ones are
+    padded with zeros).  Up to 256 rows the adapters add to what ``linear`` gives, so that a row without one is ``linear``'s bit for bit (without
+    a residual).  Inference only."""
     widths = (w.shape[0],) if widths is None else tuple(int(m) for m in widths)
     _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
     if not fn._is_kernel_tensor(x):
         y = fn.linear(x, w, bias, residual)
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
-    d, x = _delta(x, a, b, scales, plan, widths, False, bias, residual), _rows(x)
-    if isinstance(w, fn.Fp8Weight):
-        return fn._linear_fp8(x, w, None, d)
-    if fn._cublas() or w.dtype != x.dtype:
-        return d.addmm_(x, w.to(x.dtype).t())
-    # The framework's own products, which add the adapters' part to their fp32 sums.  (The library's, which plain decode products go to, may
-    # cut the reduction and round the pieces' sums to bf16 first.)
-    if 0 < x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._streams(w):
-        return fn.skinny_linear(x, w, None, d)
-    return _C().gemm_bf16(x, fn._g2_operand(w), d)
+    if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
+        return _delta(x, a, b, scales, plan, widths, False, None, residual, fn.linear(x, w, bias).contiguous())
+    d = _delta(x, a, b, scales, plan, widths, False, bias, residual)
+    return _C().gemm_bf16(_rows(x), fn._g2_operand(w.to(x.dtype)), d)
 
 
 @torch.no_grad()
@@ -134,7 +129,7 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
     if not fn._is_kernel_tensor(x):
         gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
         return ref.swiglu(gu).to(x.dtype)
-    d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True, None, None), _rows(x)
+    d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True), _rows(x)
     if isinstance(wgu, fn.Fp8Weight):
         xq, xs = fn.quantize_fp8_rowwise(x)
         if 0 < x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._stream_impl():
@@ -167,28 +162,14 @@ class _LoraFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias, residual, scale, widths, swiglu, *ab):
-        C = _C()
-        x = _rows(x)
-        w = fn._g2_operand(w)
-        a, b = ([None if t is None else t.contiguous() for t in ab[i::2]] for i in (0, 1))
+        x, w = _rows(x), fn._g2_operand(w)
+        a, b = ([None if t is None else fn._aligned(t) for t in ab[i::2]] for i in (0, 1))
         ranks = [0 if t is None else t.shape[0] for t in a]
-        if len(a) == 1 and bias is None and ranks[0] % 8 == 0 and a[0].data_ptr() % 16 == 0 and b[0].data_ptr() % 16 == 0:
-            pa, pb = a[0], b[0]
-        else:
-            pa, pb = C.lora_pack([None if t is None else fn._aligned(t) for t in a], b, list(widths), swiglu, bias)
-        t = C.lora_thin(x, pa, 0, scale, 0, pb.shape[1] - pa.shape[0])
         need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or any(ctx.needs_input_grad[7:])
-        gu = None
-        if swiglu:
-            y, *rest = C.lora_gemm_swiglu(x, w, t, pb, need)
-            gu = rest[0] if rest else None
-        else:
-            r = residual
-            if r is not None and not (r.is_contiguous() and r.data_ptr() % 16 == 0):
-                r = fn._aligned(r)
-            y = C.lora_gemm(x, w, t, pb, False, r)
+        y, pa, pb, t, *gu = _C().lora_fwd(x, w, a, b, widths, scale, swiglu, bias if bias is None else fn._aligned(bias),
+                                          residual if residual is None else fn._aligned(residual), need)
         if need:
-            ctx.save_for_backward(x, w, pa, pb, t, *([gu] if swiglu else []))
+            ctx.save_for_backward(x, w, pa, pb, t, *gu)
         ctx.meta = (scale, widths, swiglu, ranks)
         return y
 
@@ -203,16 +184,8 @@ class _LoraFn(torch.autograd.Function):
             return (None, None, dbias, dres, *[None] * (3 + 2 * len(ranks)))
         x, w, pa, pb, t, *gu = ctx.saved_tensors
         dy = C.swiglu_bwd(gu[0], fn._aligned(dy)) if swiglu else _rows(dy)
-        r = pa.shape[0]
-        dx = dw = da = db = None
-        if need[0] or any(need[7::2]):
-            dt = C.lora_thin(dy, pb, 1, scale, r)
-            if need[0]:
-                dx = C.lora_gemm(dy, w, dt, pa, True)
-            if any(need[7::2]):
-                da = C.lora_thin(x, dt, 3)
-        if any(need[8::2]):
-            db = C.lora_thin(dy, t, 2, 1.0, r)
+        r, dw = pa.shape[0], None
+        dx, da, db = C.lora_bwd(dy, x, w, pa, pb, t, scale, need[0], any(need[7::2]), any(need[8::2]))
         if need[1]:
             dw = fn.mm_tn(dy, x, out=fn._sink_for(w))
         grads, col, row = [], 0, 0

@@ -77,9 +77,10 @@ def part_of(n, widths, interleaved):
     return (torch.arange(n) // 128) % 2 if interleaved else torch.repeat_interleave(torch.arange(len(widths)), torch.tensor(widths))
 
 
-def adapters64(x, w, a, b, scales, ids, widths, interleaved=False, bias=None, residual=None):
+def adapters64(x, w, a, b, scales, ids, widths, interleaved=False, bias=None, residual=None, base=None):
     """(projection in 64 bits, bound of its error before the last rounding): low-rank values rounded to bf16, what the adapters add (with bias
-    and residual) rounded to bf16, all sums in fp32."""
+    and residual) rounded to bf16, all sums in fp32.  `base`: the projection (with its bias) as it is; what the adapters and the residual add goes on
+    top in fp32."""
     dev = x.device
     x, w, a, b, s = (t.double() for t in (x, w, a, b, scales))
     n, k, r = w.shape[0], w.shape[1], b.shape[2]
@@ -97,10 +98,12 @@ def adapters64(x, w, a, b, scales, ids, widths, interleaved=False, bias=None, re
             et = u * t.abs() + (k + 3) * U32 * mag
             d[rows[:, None], cols] = t @ bi.t()
             err[rows[:, None], cols] = et @ bi.abs().t() + (r + 1) * U32 * ((t.abs() + et) @ bi.abs().t())
-    for extra in (bias, residual):
+    for extra in (bias, residual) if base is None else (residual,):
         if extra is not None:
             d = d + extra.double()
-            err = err + 2 * U32 * d.abs()
+            err = err + 2 * U32 * (d.abs() + extra.double().abs())
+    if base is not None:
+        return base.double() + d, err + 2 * U32 * (base.double().abs() + d.abs())
     base = x @ w.t()
     err = err + u * (d.abs() + err) + (k + 2) * U32 * (x.abs() @ w.abs().t() + d.abs())
     return base + d, err

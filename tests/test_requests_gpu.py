@@ -112,6 +112,11 @@ def test_rules_stream_and_graph():
 
 
 # ------------------------------------------------------------------------------------------------------------------ adapters
+def near64(c, widths):
+    """Up to 256 rows the adapters add to `linear`'s result."""
+    return adapters64(**c, widths=widths, base=ops.linear(c["x"], c["w"], c["bias"]) if c["x"].shape[0] <= 256 else None)
+
+
 def run_adapters(c, widths, num):
     plan = ops.adapter_plan(c["ids"], num)
     return ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], plan, widths, c["bias"], c["residual"])
@@ -142,16 +147,16 @@ def test_plan_sorts_rows(t, num, kind):
     (300, 896, (896,), 64, 6), (1000, 224, (64, 32, 32), 128, 2), (1531, 64, (64,), 16, 9)])
 def test_adapters(t, k, widths, rank, num):
     c = adapters_case(t, k, widths, rank, num, t + k, torch.bfloat16, "cuda")
-    check_near(run_adapters(c, widths, num), *adapters64(**c, widths=widths))
+    check_near(run_adapters(c, widths, num), *near64(c, widths))
     c = dict(c, bias=None, residual=None, ids=torch.sort(c["ids"])[0])
-    check_near(run_adapters(c, widths, num), *adapters64(**c, widths=widths))
+    check_near(run_adapters(c, widths, num), *near64(c, widths))
 
 
 @pytest.mark.parametrize("value", [-1, 0, 2, 2 ** 31 - 1])
 @pytest.mark.parametrize("t", [3, 80, 333])
 def test_adapters_all_rows_alike(value, t):
     c = adapters_case(t, 128, (64, 64), 16, 3, t, torch.bfloat16, "cuda", ids=torch.full((t,), value, dtype=torch.int32))
-    check_near(run_adapters(c, (64, 64), 3), *adapters64(**c, widths=(64, 64)))
+    check_near(run_adapters(c, (64, 64), 3), *near64(c, (64, 64)))
 
 
 @pytest.mark.parametrize("t,k,f,rank,num", [(1, 64, 128, 16, 1), (45, 896, 4864, 32, 9), (128, 256, 512, 16, 3), (129, 256, 512, 16, 3), (600, 256, 1280, 64, 2),
@@ -172,8 +177,7 @@ def test_adapters_over_fp8_weights():
         base = ops.adapter_linear(*args, ops.adapter_plan(none, 3)).double()
         y = ops.adapter_linear(*args, ops.adapter_plan(c["ids"], 3))
         assert torch.equal(base.bfloat16(), ops.linear(c["x"], w))
-        ref, err = adapters64(**dict(c, w=torch.zeros_like(c["w"])), widths=(512,))
-        check_near(y, base + ref, err + 2.0 ** -8 * base.abs())               # base is rounded too
+        check_near(y, *adapters64(**c, widths=(512,), base=base))
         c = adapters_case(t, 256, (256, 256), 16, 3, t, torch.bfloat16, "cuda", extra=False)
         w = ops.quantize_weight_fp8(c["w"])
         gu = ops.linear(c["x"], w).double()
@@ -181,6 +185,14 @@ def test_adapters_over_fp8_weights():
         y = ops.adapter_linear_swiglu(c["x"], w, c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], 3))
         # sums rounded to bf16 before the activation where the rows are many (twice), and in `gu` here
         check_near(y, *swiglu64(gu + ref, err + 3 * 2.0 ** -8 * (gu.abs() + ref.abs())))
+
+
+def test_rows_without_an_adapter_are_linears():
+    for t in (1, 30, 256):
+        c = dict(adapters_case(t, 256, (256, 64, 64), 16, 4, t, torch.bfloat16, "cuda"), residual=None)
+        y, base = run_adapters(c, (256, 64, 64), 4), ops.linear(c["x"], c["w"], c["bias"])
+        none = (c["ids"] < 0) | (c["ids"] >= 4)
+        assert torch.equal(y[none], base[none])
 
 
 def test_adapters_rows_are_their_own():
@@ -199,7 +211,7 @@ def test_adapters_rows_are_their_own():
 
 def test_adapters_views_streams_and_graph():
     c = adapters_case(21, 128, (128, 64), 16, 3, 5, torch.bfloat16, "cuda")
-    ref = adapters64(**c, widths=(128, 64))
+    ref = near64(c, (128, 64))
     wide = torch.randn(21, 400, device="cuda").bfloat16()
     for x in (wide[:, 8:136], wide[:, 3:131]):                               # a pitch, and rows that start on an odd element
         x.copy_(c["x"])
@@ -220,7 +232,7 @@ def test_adapters_views_streams_and_graph():
         c["ids"].copy_((c["ids"] + shift) % 4)
         c["x"].mul_(0.5)
         graph.replay()
-        check_near(y, *adapters64(**c, widths=(128, 64)))
+        check_near(y, *near64(c, (128, 64)))
 
 
 def test_adapters_refused_by_the_kernel_entry():

@@ -193,15 +193,7 @@ def load_peft_adapter(engine, path: str) -> int:
         ac = json.loads(cfg_file.read_text())
         if engine.lora is not None and int(ac.get("r", engine.lora.rank)) != engine.lora.rank:
             raise ValueError(f"adapter rank {ac.get('r')} != model.lora_rank {engine.lora.rank}")
-    if (p / "adapter_model.safetensors").exists():
-        from safetensors.torch import load_file
-
-        sd = load_file(str(p / "adapter_model.safetensors"))
-    elif (p / "adapter_model.bin").exists():
-        sd = torch.load(p / "adapter_model.bin", map_location="cpu", weights_only=True)
-    else:
-        raise FileNotFoundError(f"no adapter_model.safetensors / adapter_model.bin in {path!r}")
-    ours = import_peft_state_dict(sd)
+    ours = import_peft_state_dict(read_peft_adapter(path)[0])
     n = 0
     for i, unit in enumerate(engine.lora_layers):
         pre = f"layers.{i}.lora."
@@ -213,3 +205,136 @@ def load_peft_adapter(engine, path: str) -> int:
             unit.load_full_state(named)
             n += len(named)
     return n
+
+
+# --------------------------------------------------------------------------------------------
+# adapters of requests: many beside one model (rollout engine)
+# --------------------------------------------------------------------------------------------
+def read_peft_adapter(path: str) -> tuple[dict[str, torch.Tensor], dict]:
+    """(peft tensors, adapter_config.json or {}) of a peft adapter directory."""
+    import json
+    from pathlib import Path
+
+    p = Path(path)
+    if (p / "adapter_model.safetensors").exists():
+        from safetensors.torch import load_file
+
+        sd = load_file(str(p / "adapter_model.safetensors"))
+    elif (p / "adapter_model.bin").exists():
+        sd = torch.load(p / "adapter_model.bin", map_location="cpu", weights_only=True)
+    else:
+        raise FileNotFoundError(f"no adapter_model.safetensors / adapter_model.bin in {path!r}")
+    return sd, json.loads((p / "adapter_config.json").read_text()) if (p / "adapter_config.json").exists() else {}
+
+
+class LayerAdapters:
+    """The bank's adapters of one block beside its weights, for the rows of one step."""
+
+    def __init__(self, bank: "AdapterBank", layer: int, plan):
+        self.bank, self.stacks, self.plan = bank, bank.layers[layer], plan
+
+    def linear(self, name: str, x: torch.Tensor, w, bias=None, residual=None) -> torch.Tensor:
+        a, b = self.stacks[name]
+        return ops.adapter_linear(x, w, a, b, self.bank.scales, self.plan, self.bank.widths[name], bias, residual)
+
+    def swiglu(self, x: torch.Tensor, wgu) -> torch.Tensor:
+        a, b = self.stacks["gate_up"]
+        return ops.adapter_linear_swiglu(x, wgu, a, b, self.bank.scales, self.plan)
+
+
+class AdapterBank:
+    """Up to ``capacity`` adapters of a rank up to ``max_rank`` for the blocks of one model, stacked as ``ops.adapter_linear`` reads them:
+    a [capacity, parts * rank, in], b [capacity, out, rank] for every fused projection.  An adapter's place is its row in the stacks; what it
+    does not adapt, and the columns that its rank does not fill, are zeros.  Addresses are fixed, so captured steps see what is loaded."""
+
+    PARTS = {"qkv": ("q_proj", "k_proj", "v_proj"), "o": ("o_proj",), "gate_up": ("gate_proj", "up_proj"), "down": ("down_proj",)}
+
+    def __init__(self, cfg: ModelConfig, capacity: int, max_rank: int, device, dtype):
+        from .transformer import rope_feature_perm
+
+        if cfg.family != "llama" or cfg.attn_type != "mha" or cfg.num_experts or cfg.mlp_act != "swiglu":
+            raise NotImplementedError("adapters of requests are implemented for dense llama / qwen blocks")
+        if rope_feature_perm(cfg) is not None:
+            raise NotImplementedError("adapters of requests for checkpoints whose rotary layout is permuted at load time")
+        if not 1 <= capacity <= 1024 or not 1 <= max_rank <= 128:
+            raise ValueError("1 to 1024 adapters of rank 1 to 128")
+        self.cfg, self.capacity, self.rank = cfg, capacity, -(-max_rank // 16) * 16
+        self.dims = _proj_dims(cfg)
+        self.widths = {n: tuple(self.dims[p][0] for p in parts) for n, parts in self.PARTS.items()}
+        if any(m % 32 for ws in self.widths.values() for m in ws) or any(k % 32 for _, k in self.dims.values()):
+            raise NotImplementedError("adapters of requests need widths that are multiples of 32")
+        self.scales = torch.zeros(capacity, dtype=torch.float32, device=device)
+        zeros = lambda *s: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
+        self.layers = [{n: (zeros(capacity, len(parts) * self.rank, self.dims[parts[0]][1]), zeros(capacity, sum(self.widths[n]), self.rank))
+                        for n, parts in self.PARTS.items()} for _ in range(cfg.num_layers)]
+        self.names: dict[str, int] = {}
+
+    def place(self, name: str) -> int:
+        if name not in self.names:
+            raise ValueError(f"no adapter {name!r} is loaded")
+        return self.names[name]
+
+    def load(self, name: str, source, alpha: float | None = None) -> int:
+        """``source``: a peft adapter directory, or tensors by name (with ``alpha``, default the rank).  Returns the adapter's place."""
+        if name in self.names:
+            raise ValueError(f"adapter {name!r} is loaded already")
+        free = sorted(set(range(self.capacity)) - set(self.names.values()))
+        if not free:
+            raise ValueError(f"all {self.capacity} places for adapters are taken")
+        root = False
+        if not isinstance(source, dict):
+            source, ac = read_peft_adapter(source)
+            odd = [k for k in ("use_dora", "alpha_pattern", "rank_pattern", "modules_to_save") if ac.get(k)]
+            if odd or ac.get("bias", "none") != "none":
+                raise NotImplementedError(f"adapter {name!r}: {', '.join(odd) or 'trained biases'} (adapter_config.json)")
+            root = bool(ac.get("use_rslora"))
+            alpha = float(ac["lora_alpha"]) if alpha is None and "lora_alpha" in ac else alpha
+        ours = {k for k in source if ".lora.lora_" in k}
+        sd = {k: source[k] for k in ours} if ours else import_peft_state_dict(source)
+        if len(sd) != len(source):
+            raise ValueError(f"adapter {name!r}: {len(source) - len(sd)} of its {len(source)} tensors belong to no module that is adapted here")
+        ranks = {t.shape[0] for n, t in sd.items() if n.endswith("_A")}
+        if len(ranks) != 1:
+            raise ValueError(f"adapter {name!r}: one rank for all of its modules expected, not {sorted(ranks)}")
+        (rank,) = ranks
+        if rank > self.rank:
+            raise ValueError(f"adapter {name!r} has rank {rank}, the bank holds up to {self.rank}")
+        known = {f"layers.{i}.lora.lora_{p}_{m}": (p, m) for i in range(self.cfg.num_layers) for p in self.dims for m in "AB"}
+        for n, t in sd.items():
+            if n not in known:
+                raise ValueError(f"adapter {name!r}: {n} is no module of {self.cfg.name}")
+            p, m = known[n]
+            want = (rank, self.dims[p][1]) if m == "A" else (self.dims[p][0], rank)
+            if tuple(t.shape) != want or n[:-1] + "AB"[m == "A"] not in sd:
+                raise ValueError(f"adapter {name!r}: {n} is {tuple(t.shape)}, {want} and its partner expected")
+        at = free[0]
+        self._write(at, sd, rank)
+        self.scales[at] = (rank if alpha is None else float(alpha)) / (rank ** 0.5 if root else rank)
+        self.names[name] = at
+        return at
+
+    @torch.no_grad()
+    def _write(self, at: int, sd: dict, rank: int) -> None:
+        for i, stacks in enumerate(self.layers):
+            for n, parts in self.PARTS.items():
+                a, b = stacks[n]
+                a[at].zero_()
+                b[at].zero_()
+                for k, (p, m) in enumerate(zip(parts, self.widths[n])):
+                    ta, tb = (sd.get(f"layers.{i}.lora.lora_{p}_{x}") for x in "AB")
+                    if ta is None:
+                        continue
+                    a[at, k * self.rank:k * self.rank + rank].copy_(ta)
+                    if n == "gate_up":          # rows in blocks of 128 of gate and up, as the fused weight has them
+                        b[at].view(m // 128, 2, 128, self.rank)[:, k, :, :rank].copy_(tb.view(m // 128, 128, rank))
+                    else:
+                        lo = sum(self.widths[n][:k])
+                        b[at, lo:lo + m, :rank].copy_(tb)
+
+    def unload(self, name: str) -> None:
+        self.scales[self.place(name)] = 0.0
+        del self.names[name]
+
+    def beside(self, layers: list[dict], plan) -> list[dict]:
+        """The blocks' weights with the bank's adapters beside them, for rows whose adapters the plan holds."""
+        return [{**w, "_adapters": LayerAdapters(self, i, plan)} for i, w in enumerate(layers)]

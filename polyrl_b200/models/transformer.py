@@ -440,6 +440,40 @@ def _mlp_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, aux_out: list | Non
     return ops.linear(ops.linear_swiglu(h, w["wgu"]), w["wd"], residual=x)
 
 
+def _qkv(cfg: ModelConfig, w: dict, h: torch.Tensor) -> torch.Tensor:
+    """The fused query / key / value projection, with the adapters that stand beside it: one that is trained (``_lora_scale``), or those of
+    the batch's requests (``_adapters``, models/lora.py)."""
+    if "_adapters" in w:
+        return w["_adapters"].linear("qkv", h, w["wqkv"], bias=w.get("bqkv"))
+    if "_lora_scale" in w:
+        from . import lora
+
+        return lora.qkv_linear(cfg, w, h)
+    return ops.linear(h, w["wqkv"], bias=w.get("bqkv"))
+
+
+def _proj(w: dict, x: torch.Tensor, name: str, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Projection ``wo`` or ``wd``, in the same way."""
+    if "_adapters" in w:
+        return w["_adapters"].linear("o" if name == "wo" else "down", x, w[name], residual=residual)
+    if "_lora_scale" in w:
+        from . import lora
+
+        return lora.single_linear(w, x, name, "o_proj" if name == "wo" else "down_proj", residual)
+    return ops.linear(x, w[name], residual=residual)
+
+
+def _gate_up(w: dict, h: torch.Tensor) -> torch.Tensor:
+    """silu(gate) * up of the fused projection, in the same way."""
+    if "_adapters" in w:
+        return w["_adapters"].swiglu(h, w["wgu"])
+    if "_lora_scale" in w:
+        from . import lora
+
+        return lora.gate_up_swiglu(w, h)
+    return ops.linear_swiglu(h, w["wgu"])
+
+
 def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, kv_sink=None, aux_out: list | None = None) -> torch.Tensor:
     """One decoder block on packed activations x:[T,H].  ``kv_sink`` = (k_cache, v_cache, slot_mapping)
     makes this a prefill step that also fills the paged KV cache (rollout engine)."""
@@ -458,8 +492,6 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
             y = dense_block(x, w, pos, cos, sin, inp.cu_seqlens, nq, nkv, d, cfg.rms_norm_eps)
             if y is not None:
                 return y
-        if lora:
-            from . import lora as L
         h, x = ops.rmsnorm_residual(x, w["ln1"], cfg.rms_norm_eps)
         if cfg.attn_type == "mla":
             from . import mla
@@ -468,7 +500,7 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
                 raise NotImplementedError("LoRA adapters are not implemented for MLA attention")
             x = ops.linear(mla.attention_forward(cfg, w, h, inp, kv_sink), w["wo"], residual=x)
             return x if w.get("_skip_mlp") else _mlp_forward(cfg, w, x, aux_out)
-        qkv = L.qkv_linear(cfg, w, h) if lora else ops.linear(h, w["wqkv"], bias=w.get("bqkv"))
+        qkv = _qkv(cfg, w, h)
         pos, cos, sin = inp.rope_inputs(cfg, x.device)
         a = None
         if kv_sink is not None:
@@ -496,10 +528,10 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
             a = attention_varlen(q, k, v, inp.cu_seqlens, inp.max_seqlen, causal=True)
         a = a.reshape(t, nq * d)
         if cfg.sandwich_norm:
-            o = L.single_linear(w, a, "wo", "o_proj") if lora else ops.linear(a, w["wo"])
+            o = _proj(w, a, "wo")
             x = x + ops.rmsnorm(o, w["ln_attn"], cfg.rms_norm_eps)
         else:
-            x = L.single_linear(w, a, "wo", "o_proj", residual=x) if lora else ops.linear(a, w["wo"], residual=x)
+            x = _proj(w, a, "wo", x)
         if w.get("_skip_mlp"):              # callers that supply their own MLP (expert parallelism, parallel/expert.py)
             return x
         h, x = ops.rmsnorm_residual(x, w["ln2"], cfg.rms_norm_eps)
@@ -510,11 +542,11 @@ def layer_forward(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: PackedInput, 
             if lora:
                 raise NotImplementedError("LoRA adapters are not implemented for the xIELU MLP")
             return xielu_mlp(w, h, x)
-        a = L.gate_up_swiglu(w, h) if lora else ops.linear_swiglu(h, w["wgu"])
+        a = _gate_up(w, h)
         if cfg.sandwich_norm:
-            y = L.single_linear(w, a, "wd", "down_proj") if lora else ops.linear(a, w["wd"])
+            y = _proj(w, a, "wd")
             return x + ops.rmsnorm(y, w["ln_mlp"], cfg.rms_norm_eps)
-        return L.single_linear(w, a, "wd", "down_proj", residual=x) if lora else ops.linear(a, w["wd"], residual=x)
+        return _proj(w, a, "wd", x)
     # ---- gpt2 block (library ops; plumbing / CPU config)
     h = F.layer_norm(x, (cfg.hidden_size,), w["ln1_w"], w["ln1_b"], cfg.rms_norm_eps)
     qkv = F.linear(h, w["wqkv"], w["bqkv"])
@@ -584,24 +616,24 @@ def layer_decode(cfg: ModelConfig, w: dict, x: torch.Tensor, inp: DecodeInput, k
     if cfg.family == "llama":
         h = ops.rmsnorm(x, w["ln1"], cfg.rms_norm_eps)
         cos, sin = rope_tables(cfg, x.device)
-        qkv = qk_norm_rope_and_cache_(cfg, w, ops.linear(h, w["wqkv"], bias=w.get("bqkv")), inp.position_ids, cos, sin, k_cache, v_cache,
+        qkv = qk_norm_rope_and_cache_(cfg, w, _qkv(cfg, w, h), inp.position_ids, cos, sin, k_cache, v_cache,
                                       inp.slot_mapping)
         a = ops.paged_decode_attention(qkv[:, : nq * d], k_cache, v_cache, inp.block_table, inp.seq_lens, nq, nkv, d,
                                        scale, max_len=inp.max_len)
         if cfg.sandwich_norm:
-            x = x + ops.rmsnorm(ops.linear(a, w["wo"]), w["ln_attn"], cfg.rms_norm_eps)
+            x = x + ops.rmsnorm(_proj(w, a, "wo"), w["ln_attn"], cfg.rms_norm_eps)
         else:
-            x = ops.linear(a, w["wo"], residual=x)
+            x = _proj(w, a, "wo", x)
         h = ops.rmsnorm(x, w["ln2"], cfg.rms_norm_eps)
         if "router" in w:
             y = moe_mlp_static(cfg, w, h) if _MOE_STATIC_DECODE() else moe_mlp(cfg, w, h)
             return x + (ops.rmsnorm(y, w["ln_mlp"], cfg.rms_norm_eps) if cfg.sandwich_norm else y)
         if "wup" in w:
             return xielu_mlp(w, h, x)
-        a = ops.linear_swiglu(h, w["wgu"])
+        a = _gate_up(w, h)
         if cfg.sandwich_norm:
-            return x + ops.rmsnorm(ops.linear(a, w["wd"]), w["ln_mlp"], cfg.rms_norm_eps)
-        return ops.linear(a, w["wd"], residual=x)
+            return x + ops.rmsnorm(_proj(w, a, "wd"), w["ln_mlp"], cfg.rms_norm_eps)
+        return _proj(w, a, "wd", x)
     h = F.layer_norm(x, (cfg.hidden_size,), w["ln1_w"], w["ln1_b"], cfg.rms_norm_eps)
     qkv = F.linear(h, w["wqkv"], w["bqkv"])
     page = k_cache.shape[2]
@@ -626,13 +658,13 @@ def layer_decode_fused(cfg: ModelConfig, w: dict, x: torch.Tensor, delta: torch.
     nq, nkv, d = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
     h = ops.rmsnorm(x, w["ln1"], cfg.rms_norm_eps) if delta is None else C.add_rmsnorm_(x, delta, w["ln1"], cfg.rms_norm_eps)
     cos, sin = rope_tables(cfg, x.device)
-    qkv = qk_norm_rope_and_cache_(cfg, w, ops.linear(h, w["wqkv"], bias=w.get("bqkv")), inp.position_ids, cos, sin, k_cache, v_cache, inp.slot_mapping)
+    qkv = qk_norm_rope_and_cache_(cfg, w, _qkv(cfg, w, h), inp.position_ids, cos, sin, k_cache, v_cache, inp.slot_mapping)
     a = ops.paged_decode_attention(qkv[:, : nq * d], k_cache, v_cache, inp.block_table, inp.seq_lens, nq, nkv, d, d ** -0.5,
                                    max_len=inp.max_len)
-    o = ops.linear(a, w["wo"])
+    o = _proj(w, a, "wo")
     h = C.add_rmsnorm_(x, o, w["ln2"], cfg.rms_norm_eps)
-    g = ops.linear_swiglu(h, w["wgu"])
-    return x, ops.linear(g, w["wd"])
+    g = _gate_up(w, h)
+    return x, _proj(w, g, "wd")
 
 
 # --------------------------------------------------------------------------------------------

@@ -107,9 +107,9 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     its rows of ``b`` [adapters, N, rank]; an adapter that leaves a part alone has zeros there.  Ranks are multiples of 16 (smaller ones are
     padded with zeros).  Up to 256 rows the adapters add to what ``linear`` gives, so that a row without one is ``linear``'s bit for bit (without
     a residual).  Inference only."""
-    widths = (w.shape[0],) if widths is None else tuple(int(m) for m in widths)
-    _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
-    if not fn._is_kernel_tensor(x):
+    widths = (w.shape[0],) if widths is None else tuple(widths)
+    if not fn._is_kernel_tensor(x) or plan.buf is None:          # (the kernel's binding checks as much)
+        _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
         y = fn.linear(x, w, bias, residual)
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
     if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
@@ -123,10 +123,10 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
     """``linear_swiglu`` with an adapter for every row: ``a`` [adapters, 2 * rank, K] (gate, up), ``b`` [adapters, 2 F, rank] with its rows in the
     order of ``wgu``'s (blocks of 128 gate and 128 up rows); the adapters act before the activation.  Inference only."""
     n = wgu.shape[0]
-    _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
     if n % 256:
         raise ValueError("adapter_linear_swiglu: gate and up in blocks of 128 rows each")
-    if not fn._is_kernel_tensor(x):
+    if not fn._is_kernel_tensor(x) or plan.buf is None:
+        _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
         gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
         return ref.swiglu(gu).to(x.dtype)
     d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True), _rows(x)

@@ -41,6 +41,18 @@ class SamplingParams:
     stop_token_ids: tuple = ()
     ignore_eos: bool = False
     seed: int | None = None
+    # rules on the logits (rollout/rules.py); log-probs are those of the distribution that results
+    repetition_penalty: float = 1.0        # of tokens in the prompt or the output: z / r if z > 0 else z * r
+    presence_penalty: float = 0.0          # off the logits of tokens in the output
+    frequency_penalty: float = 0.0         # the same for every time that they are there
+    min_new_tokens: int = 0                # stop tokens may not come before
+    logit_bias: dict | None = None         # {token: number added to its logit}
+    allowed_token_ids: tuple | None = None # no other token may come
+
+    @property
+    def has_rules(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0 or self.min_new_tokens != 0
+                or bool(self.logit_bias) or self.allowed_token_ids is not None)
 
     @classmethod
     def from_dict(cls, d: dict | None) -> "SamplingParams":
@@ -48,6 +60,13 @@ class SamplingParams:
         keep = {k: d[k] for k in ("max_new_tokens", "temperature", "top_p", "top_k", "n", "ignore_eos", "seed") if k in d}
         if "stop_token_ids" in d and d["stop_token_ids"]:
             keep["stop_token_ids"] = tuple(d["stop_token_ids"])
+        keep |= {k: float(d[k]) for k in ("repetition_penalty", "presence_penalty", "frequency_penalty") if d.get(k) is not None}
+        if d.get("min_new_tokens") is not None:
+            keep["min_new_tokens"] = int(d["min_new_tokens"])
+        if d.get("logit_bias"):
+            keep["logit_bias"] = {int(t): float(v) for t, v in d["logit_bias"].items()}
+        if d.get("allowed_token_ids") is not None:
+            keep["allowed_token_ids"] = tuple(int(t) for t in d["allowed_token_ids"])
         return cls(**keep)
 
 
@@ -77,6 +96,7 @@ class Request:
     h: int = -1                            # handle inside the native scheduler (csrc/scheduler.hpp), -1 = not registered
     state_slot: int = 0                    # recurrent-state slot (mixer stacks), 0 = none
     fed: bool = False                      # tokens are supplied step by step (RolloutEngine.extend), nothing is sampled
+    adapter: int = -1                      # place in the engine's adapter bank (models/lora.py), -1 = the plain model
 
     @property
     def decoding(self) -> bool:
@@ -278,7 +298,7 @@ class RolloutEngine:
                  kv_cache_tokens: int | None = None, gpu_memory_utilization: float = 0.5, dtype=None,
                  use_cuda_graph: bool = True, max_prefill_tokens: int = 16384, seed: int = 0, tp=None,
                  weight_dtype: str = "bf16", steps_per_sync: int | None = None, enable_prefix_cache: bool = False,
-                 kv_vmm: bool | None = None):
+                 kv_vmm: bool | None = None, max_adapters: int = 0, max_adapter_rank: int = 16):
         if cfg.sliding_window and max_model_len > cfg.sliding_window:
             raise NotImplementedError(f"max_model_len {max_model_len} exceeds the model's attention window {cfg.sliding_window}: "
                                       "windowed decode attention is not implemented (full-causal only)")
@@ -295,6 +315,14 @@ class RolloutEngine:
         self._kv_blocks = 0
         self.enable_prefix_cache = enable_prefix_cache and tp is None and cfg.family == "llama"
         self.prefix_cache: PrefixCache | None = None
+        self.adapters = None                       # bank of low-rank adapters that requests name (load_adapter)
+        if max_adapters:
+            from ..models.lora import AdapterBank
+
+            if tp is not None:
+                raise NotImplementedError("adapters of requests with tensor parallelism")
+            self.adapters = AdapterBank(cfg, max_adapters, max_adapter_rank, device, dtype or (torch.bfloat16 if str(device).startswith("cuda") else torch.float32))
+        self.rules = None                          # rules of requests on their logits, per slot (created by the first one that has any)
         if weight_dtype not in ("bf16", "fp8"):
             raise ValueError("weight_dtype must be 'bf16' or 'fp8'")
         if weight_dtype == "fp8" and tp is not None:
@@ -341,6 +369,7 @@ class RolloutEngine:
         self._base_seed = seed
         self._step_count = 0
         self._top_k, self._top_p = -1, 1.0
+        self._with_rules = self._with_adapters = False
         self.vision_w = None                         # VLM tower weights (set_vision_weights)
         self.stats = {"prefill_tokens": 0, "decode_tokens": 0, "steps": 0, "last_gen_throughput": 0.0}
         self._alloc_static()
@@ -522,6 +551,7 @@ class RolloutEngine:
         self.st_seq_lens = torch.zeros(s, dtype=torch.int32, device=dev)
         self.st_active = torch.zeros(s, dtype=torch.long, device=dev)
         self.st_state = torch.zeros(s, dtype=torch.long, device=dev)           # recurrent-state slot of a batch slot
+        self.st_adapter = torch.full((s,), -1, dtype=torch.int32, device=dev)
         self.arange32 = torch.arange(s + 1, dtype=torch.int32, device=dev)
         self.st_block_table = torch.zeros(s, self.max_blocks_per_seq + 2, dtype=torch.int32, device=dev)   # + overshoot slack -> scratch page 0
         self.st_temp = torch.ones(s, dtype=torch.float32, device=dev)
@@ -538,10 +568,42 @@ class RolloutEngine:
         """Tower weights (models.vision.VisionWeights-like: ``.stem`` dict + ``.blocks`` list) for image prompts."""
         self.vision_w = vision_w
 
+    def _stop_ids(self, p: SamplingParams) -> set[int]:
+        """Tokens that end a request."""
+        return set() if p.ignore_eos else {t for t in (self.cfg.eos_token_id, *p.stop_token_ids, *self.cfg.extra_eos_token_ids) if t is not None and t >= 0}
+
+    def check_request(self, params: SamplingParams, adapter: str | None = None) -> None:
+        """ValueError for parameters or an adapter that ``add_request`` refuses."""
+        if params.has_rules:
+            from .rules import check_params
+
+            check_params(params, self.cfg.vocab_size, self._stop_ids(params))
+        if adapter is not None:
+            if self.adapters is None:
+                raise ValueError("this engine serves no adapters (max_adapters)")
+            self.adapters.place(adapter)
+
+    def load_adapter(self, name: str, source, alpha: float | None = None) -> None:
+        """Take a low-rank adapter into the bank under ``name``: a peft adapter directory, or its tensors by name (peft's, or
+        ``layers.{i}.lora.lora_{proj}_{A|B}``) with ``alpha`` (default: the rank).  Requests name it in ``add_request``."""
+        if self.adapters is None:
+            raise ValueError("this engine serves no adapters (max_adapters)")
+        self.adapters.load(name, source, alpha)
+
+    def unload_adapter(self, name: str) -> None:
+        """Forget an adapter that no request uses."""
+        if self.adapters is None:
+            raise ValueError("this engine serves no adapters (max_adapters)")
+        at = self.adapters.place(name)
+        if any(r.adapter == at for r in (*self.waiting, *self.running.values())):
+            raise ValueError(f"adapter {name!r} is in use")
+        self.adapters.unload(name)
+
     def add_request(self, prompt_ids: list[int], params: SamplingParams | dict | None = None, rid: str | None = None,
-                    group=None, mm: dict | None = None) -> Request:
+                    group=None, mm: dict | None = None, adapter: str | None = None) -> Request:
         if not isinstance(params, SamplingParams):
             params = SamplingParams.from_dict(params)
+        self.check_request(params, adapter)
         mrope_pos, mrope_delta = None, 0
         if mm is not None:
             from ..models import vision as V
@@ -561,7 +623,7 @@ class RolloutEngine:
         if params.max_new_tokens > budget:
             params = SamplingParams(**{**params.__dict__, "max_new_tokens": budget})
         r = Request(rid or f"r{next(self._rid)}", list(prompt_ids), params, t_arrival=time.time(), group=group, mm=mm,
-                    mrope_pos=mrope_pos, mrope_delta=mrope_delta)
+                    mrope_pos=mrope_pos, mrope_delta=mrope_delta, adapter=-1 if adapter is None else self.adapters.place(adapter))
         self.waiting.append(r)
         return r
 
@@ -596,6 +658,16 @@ class RolloutEngine:
         total = len(r.prompt_ids) + r.params.max_new_tokens
         return (total + PAGE - 1) // PAGE
 
+    @staticmethod
+    def _group_key(r: Request) -> int:
+        """Requests with the same key may share their prompt's pages: one group, one adapter; -1: none."""
+        return -1 if r.group is None else id(r.group) if r.adapter < 0 else (id(r.group) * 1021 + r.adapter + 1) & (2 ** 62 - 1)
+
+    @staticmethod
+    def _cacheable(r: Request) -> bool:
+        """The tokens alone say what its keys and values are."""
+        return r.mm is None and r.adapter < 0
+
     def _admit(self) -> list[Request]:
         """Pop waiting requests that fit (slots, KV pages reserved up front, prefill token budget)."""
         admitted = self._admit_native() if self.sched is not None else self._admit_python()
@@ -611,10 +683,10 @@ class RolloutEngine:
             r = self.waiting[0]
             need = self._blocks_needed(r)
             full_prompt_pages = len(r.prompt_ids) // PAGE
-            donor = shared.get(id(r.group)) if r.group is not None else None
+            donor = shared.get(self._group_key(r)) if r.group is not None else None
             cached: list[int] = []
             keys: list[int] = []
-            if donor is None and self.prefix_cache is not None and r.mm is None:     # placeholder ids do not identify an image
+            if donor is None and self.prefix_cache is not None and self._cacheable(r):     # placeholder ids do not identify an image
                 # at least the last prompt token must be recomputed (its logits seed the first sampled token)
                 keys = self.prefix_cache.page_keys(r.prompt_ids, (len(r.prompt_ids) - 1) // PAGE)
                 cached = self.prefix_cache.match(keys)
@@ -642,7 +714,7 @@ class RolloutEngine:
                 r.blocks = cached + self.alloc.alloc(fresh)
                 r.cached_tokens = r.prefilled = len(cached) * PAGE
                 if r.group is not None:
-                    shared[id(r.group)] = r
+                    shared[self._group_key(r)] = r
             r.slot = self.free_slots.pop()
             self.running[r.slot] = r
             admitted.append(r)
@@ -653,7 +725,7 @@ class RolloutEngine:
         """``_admit`` through the C++ scheduler: same decisions, the per-request results are mirrored onto the Request objects."""
         for r in self.waiting:                     # registration is lazy so the native queue always has the order of self.waiting
             if r.h < 0:
-                r.h = self.sched.add(r.prompt_ids, r.params.max_new_tokens, id(r.group) if r.group is not None else -1, r.mm is None)
+                r.h = self.sched.add(r.prompt_ids, r.params.max_new_tokens, self._group_key(r), self._cacheable(r))
         admitted, by_h = [], {}
         for h in self.sched.admit(self.max_prefill_tokens):
             r = self.waiting.popleft()
@@ -676,18 +748,22 @@ class RolloutEngine:
             self.running.pop(r.slot, None)
             self.st_active[r.slot] = 0
             self.st_seq_lens[r.slot] = 0
+            if r.adapter >= 0:
+                self.st_adapter[r.slot] = -1
+            if r.params.has_rules and self.rules is not None:
+                self.rules.clear(r.slot)
             self.free_slots.append(r.slot)
             r.slot = -1
         if self.state is not None:
             self.state.release(r.state_slot)
             r.state_slot = 0
         if r.h >= 0 and self.sched is not None:
-            to_cache = self.prefix_cache is not None and reason != "abort" and r.mm is None
+            to_cache = self.prefix_cache is not None and reason != "abort" and self._cacheable(r)
             self.sched.finish(r.h, (r.prompt_ids + r.output_ids) if to_cache else [], to_cache)
             r.h, r.blocks = -1, []
             return
         if r.blocks and self.alloc is not None:
-            if self.prefix_cache is not None and reason != "abort" and r.mm is None:
+            if self.prefix_cache is not None and reason != "abort" and self._cacheable(r):
                 # every FULL page whose KV is final: prompt + generated tokens except the last one (never fed back)
                 toks = r.prompt_ids + r.output_ids
                 n_full = max(0, (len(toks) - 1)) // PAGE
@@ -768,7 +844,13 @@ class RolloutEngine:
         temps = torch.tensor([r.params.temperature for r in reqs], dtype=torch.float32, device=dev)
         seeds = torch.tensor([self._seed_for(r, 0) for r in reqs], dtype=torch.long, device=dev)
         p0 = reqs[0].params
+        ruled = [r for r in reqs if r.params.has_rules]
+        if ruled:
+            at = self._set_rules(reqs, ruled)
+            self.rules.apply_to(logits, torch.tensor([r.slot for r in reqs], dtype=torch.long, device=dev))
         tok, lp = ops.sample_tokens(logits, temps, seeds, greedy=False, top_k=p0.top_k, top_p=p0.top_p)
+        if ruled:
+            self.rules.append(torch.tensor([r.slot for r in ruled], dtype=torch.long, device=dev), tok.index_select(0, at))
         tok_c, lp_c = tok.tolist(), lp.tolist()
         if self.hybrid and self.is_cuda:
             from ..ops import mixers
@@ -782,7 +864,7 @@ class RolloutEngine:
             if r.finished:
                 continue
             n = r.num_tokens            # tokens so far; the new token sits at position n-1 (+ the M-RoPE offset of image prompts)
-            live.append((r.slot, t, n - 1 + r.mrope_delta, n, 1, r.params.temperature, self._seed_for(r, 1), r.state_slot))
+            live.append((r.slot, t, n - 1 + r.mrope_delta, n, 1, r.params.temperature, self._seed_for(r, 1), r.state_slot, r.adapter))
             rows.append(r)
         if live:
             cols = list(zip(*live))
@@ -794,12 +876,28 @@ class RolloutEngine:
             self.st_temp[sl] = torch.tensor(cols[5], dtype=torch.float32, device=dev)
             self.st_seeds[sl] = torch.tensor(cols[6], dtype=torch.long, device=dev)
             self.st_state[sl] = torch.tensor(cols[7], dtype=torch.long, device=dev)
+            if self.adapters is not None:
+                self.st_adapter[sl] = torch.tensor(cols[8], dtype=torch.int32, device=dev)
             width = self.st_block_table.shape[1]
             if self.sched is not None and all(r.h >= 0 for r in rows):
                 table = self.sched.block_rows([r.h for r in rows], width)
             else:
                 table = torch.tensor([r.blocks + [0] * (width - len(r.blocks)) for r in rows], dtype=torch.int32)
             self.st_block_table[sl] = table.to(dev)
+
+    def _set_rules(self, reqs: list[Request], ruled: list[Request]) -> torch.Tensor:
+        """Rules of requests whose first token is sampled next; returns which rows of ``reqs`` have any."""
+        if self.rules is None:
+            from .rules import RequestRules
+
+            vocab = tf.lm_head_weight(self.cfg, self.head_w, self.embed_w).shape[0]
+            self.rules = RequestRules(self.max_num_seqs, self.max_model_len, vocab, self.device)
+        version = self.rules.version
+        for r in ruled:
+            self.rules.set(r.slot, r.params, r.prompt_ids + r.output_ids, len(r.prompt_ids), self._stop_ids(r.params))
+        if self.rules.version != version:                    # steps captured over tensors that have been replaced
+            self._graphs = {k: g for k, g in self._graphs.items() if "rules" not in k}
+        return torch.tensor([i for i, r in enumerate(reqs) if r.params.has_rules], dtype=torch.long, device=self.device)
 
     def _forward_spans(self, donors: list[Request], spans: list[tuple[int, int]]) -> tuple[torch.Tensor, torch.Tensor]:
         """Run the tokens [c, e) of every request as ONE packed step over the cache and state that earlier steps left.  Returns the
@@ -839,7 +937,11 @@ class RolloutEngine:
             inp.kv_gather = (g_blk.to(dev), g_off.to(dev), cu_k.to(dev), max(klens))
         slot_t = slots_t.to(dev)
         x = tf.embed_forward(cfg, self.embed_w, inp).to(self.dtype)
-        for i, w in enumerate(self.layer_w):
+        layers = self.layer_w
+        if any(r.adapter >= 0 for r in donors):
+            ids = torch.repeat_interleave(torch.tensor([r.adapter for r in donors], dtype=torch.int32), torch.tensor(lens))
+            layers = self.adapters.beside(layers, ops.adapter_plan(ids.to(dev), self.adapters.capacity))
+        for i, w in enumerate(layers):
             if self.tp is not None:
                 from .tp import layer_prefill_tp
 
@@ -981,7 +1083,10 @@ class RolloutEngine:
         fused = (self.tp is None and cfg.family == "llama" and self.is_cuda and self.dtype == torch.bfloat16 and not cfg.num_experts
                  and cfg.attn_type == "mha" and cfg.mlp_act == "swiglu")
         delta = None
-        for i, w in enumerate(self.layer_w):
+        layers = self.layer_w
+        if self._with_adapters:
+            layers = self.adapters.beside(layers, ops.adapter_plan(self.st_adapter[:bs], self.adapters.capacity))
+        for i, w in enumerate(layers):
             if self.tp is not None:
                 from .tp import layer_decode_tp
 
@@ -1012,7 +1117,11 @@ class RolloutEngine:
 
     def _decode_sample(self, bs: int, logits: torch.Tensor) -> None:
         act = self.st_active[:bs]
+        if self._with_rules:
+            self.rules.apply(logits)
         tok, lp = ops.sample_tokens(logits, self.st_temp[:bs], self.st_seeds[:bs], top_k=self._top_k, top_p=self._top_p)
+        if self._with_rules:
+            self.rules.advance(tok, act)
         self.st_out_tok[:bs].copy_(tok)
         self.st_out_lp[:bs].copy_(lp)
         # on-device bookkeeping for the next step
@@ -1029,15 +1138,21 @@ class RolloutEngine:
 
     def _run_decode(self, bs: int, sample: bool = True) -> torch.Tensor:
         """One decode step, through its CUDA graph where there is one; returns the step's logits (overwritten by the next step)."""
+        # what some request of the batch brings is part of the step, and of the graph; a batch without is the step without
+        self._with_rules = sample and any(r.params.has_rules for r in self.running.values())
+        self._with_adapters = sample and any(r.adapter >= 0 for r in self.running.values())
         if not self.use_cuda_graph or (sample and (self._top_k > 0 or self._top_p < 1.0)):
             # top-k / top-p go through the sort-based library sampler (host-seeded RNG): not captured into a graph
             return self._decode_body(bs, sample)
         key = (bs, self._top_k, self._top_p) if sample else (bs, "logits")
+        key += ("rules",) * self._with_rules + ("adapters",) * self._with_adapters
         g = self._graphs.get(key)
         if g is None:
             # warm-up on a side stream (also sets kernel attributes), then capture.  The warm-up step is real work: with every slot
             # idle it leaves caches and recurrent states alone.
             keep = (self.st_input_ids, self.st_positions, self.st_seq_lens, self.st_seeds, self.st_active)
+            if self._with_rules:
+                keep += (self.rules.lens,)
             snap = [t.clone() for t in keep]
             if self.hybrid:
                 self.st_active.zero_()
@@ -1076,8 +1191,12 @@ class RolloutEngine:
         for src, dst in zip(high, low_free):
             r = self.running.pop(src)
             for t in (self.st_input_ids, self.st_positions, self.st_seq_lens, self.st_active, self.st_temp,
-                      self.st_seeds, self.st_state):
+                      self.st_seeds, self.st_state, self.st_adapter):
                 t[dst] = t[src]
+            if self.adapters is not None:
+                self.st_adapter[src] = -1
+            if self.rules is not None:
+                self.rules.move(src, dst)
             self.st_block_table[dst] = self.st_block_table[src]
             self.st_active[src] = 0
             self.st_seq_lens[src] = 0
@@ -1265,16 +1384,17 @@ class RolloutEngine:
     # ------------------------------------------------------------------ batch API
     @torch.no_grad()
     def generate(self, prompts: list[list[int]], params: SamplingParams | dict | None = None,
-                 on_finish=None, mm: list[dict | None] | None = None) -> list[list[Request]]:
+                 on_finish=None, mm: list[dict | None] | None = None, adapter: str | list[str | None] | None = None) -> list[list[Request]]:
         """Generate ``params.n`` samples for every prompt; returns, per prompt, its list of requests.  ``mm[i]`` carries the image
-        inputs of prompt i (vision-language models)."""
+        inputs of prompt i (vision-language models); ``adapter``: the loaded adapter of all prompts, or of each."""
         if not isinstance(params, SamplingParams):
             params = SamplingParams.from_dict(params)
         groups: list[list[Request]] = []
         for pi, p in enumerate(prompts):
             tag = object()
             m = mm[pi] if mm is not None else None
-            groups.append([self.add_request(p, params, group=tag if params.n > 1 else None, mm=m) for _ in range(params.n)])
+            ad = adapter[pi] if isinstance(adapter, (list, tuple)) else adapter
+            groups.append([self.add_request(p, params, group=tag if params.n > 1 else None, mm=m, adapter=ad) for _ in range(params.n)])
         t0 = time.time()
         ntok0 = self.stats["decode_tokens"]
         while self.has_work():

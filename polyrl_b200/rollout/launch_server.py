@@ -41,6 +41,9 @@ def main(argv=None) -> int:
                                                            "and /v1/chat/completions routes; default: --model-path when it holds a tokenizer")
     ap.add_argument("--served-model-name", default=None)
     ap.add_argument("--tool-call-parser", default=None, help="hermes | gpt-oss | json_block: parse tool calls of chat completions into tool_calls")
+    ap.add_argument("--max-adapters", type=int, default=0, help="low-rank adapters that requests can name (/load_lora_adapter, then lora_path or model)")
+    ap.add_argument("--max-adapter-rank", type=int, default=16)
+    ap.add_argument("--lora-paths", nargs="*", default=[], metavar="NAME=PATH", help="peft adapters to load at start")
     ap.add_argument("--tp-size", type=int, default=1, help="tensor-parallel degree; launch with torchrun --nproc-per-node TP")
     a = ap.parse_args(argv)
     cfg = get_model_config(a.model_path)
@@ -84,8 +87,12 @@ def main(argv=None) -> int:
             vw.load_state_dict(sd)
         print(f"[engine] loaded weights from {mp}", flush=True)
     eng = RolloutEngine(cfg, a.device, max_num_seqs=a.max_num_seqs, max_model_len=a.max_model_len,
-                        gpu_memory_utilization=a.mem_fraction_static, tp=tp_ctx, enable_prefix_cache=a.enable_prefix_cache)
+                        gpu_memory_utilization=a.mem_fraction_static, tp=tp_ctx, enable_prefix_cache=a.enable_prefix_cache,
+                        max_adapters=max(a.max_adapters, len(a.lora_paths)), max_adapter_rank=a.max_adapter_rank)
     eng.set_weights(w.embed, w.layers, w.head)
+    for entry in a.lora_paths:
+        name, _, path = entry.partition("=")
+        eng.load_adapter(name, path or name)
     if vw is not None:
         eng.set_vision_weights(vw)
     if tp_rank > 0:

@@ -5,8 +5,10 @@ Why it exists: the reference's rollout servers (SGLang / vLLM) speak this API na
 ``verl/trainer/main_generation_server.py`` (offline generation through stand-alone servers, one ``/v1/chat/completions`` call per
 sample), generative reward models and evaluation harnesses that point at a served policy.  Supported request fields: ``messages`` /
 ``prompt`` (text, list of texts, or token ids), ``max_tokens`` / ``max_completion_tokens``, ``temperature``, ``top_p``, ``top_k``,
-``n``, ``seed``, ``stop`` (strings, applied to the decoded text), ``stop_token_ids``, ``ignore_eos``, ``logprobs``, ``tools``
-(rendered by the chat template; calls in the output are parsed into ``tool_calls`` when the server has a tool parser), ``stream``.
+``n``, ``seed``, ``stop`` (strings, applied to the decoded text), ``stop_token_ids``, ``ignore_eos``, ``presence_penalty``,
+``frequency_penalty``, ``repetition_penalty``, ``logit_bias``, ``min_tokens``, ``allowed_token_ids``, ``logprobs``, ``tools``
+(rendered by the chat template; calls in the output are parsed into ``tool_calls`` when the server has a tool parser), ``stream``.  A ``model``
+that is the name of a loaded adapter is served with it.
 """
 from __future__ import annotations
 
@@ -21,7 +23,11 @@ from .engine import SamplingParams
 def _sampling(body: dict) -> SamplingParams:
     mx = body.get("max_completion_tokens") or body.get("max_tokens") or 128
     temp = body.get("temperature")
-    return SamplingParams(max_new_tokens=int(mx), temperature=1.0 if temp is None else float(temp),
+    rules = {ours: body[k] for k, ours in (("presence_penalty", "presence_penalty"), ("frequency_penalty", "frequency_penalty"), ("min_tokens", "min_new_tokens"),
+                                           ("repetition_penalty", "repetition_penalty"), ("logit_bias", "logit_bias"), ("allowed_token_ids", "allowed_token_ids"))
+             if body.get(k) is not None}
+    rules = {k: v for k, v in SamplingParams.from_dict(rules).__dict__.items() if k in rules}
+    return SamplingParams(**rules, max_new_tokens=int(mx), temperature=1.0 if temp is None else float(temp),
                           top_p=float(body.get("top_p") if body.get("top_p") is not None else 1.0),
                           top_k=int(body.get("top_k") if body.get("top_k") is not None else -1),
                           stop_token_ids=tuple(int(t) for t in (body.get("stop_token_ids") or ())),
@@ -97,7 +103,9 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
         prompts = _prompts(srv, body, chat)
         sp = _sampling(body)
         n = max(1, int(body.get("n") or 1))
-    except (ValueError, TypeError, KeyError) as e:
+        adapter = srv.adapter_of(body.get("model"))
+        srv.engine.check_request(sp, adapter)
+    except (ValueError, TypeError, KeyError, AttributeError) as e:
         h._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})
         return
     room = srv.engine.max_model_len - 1
@@ -110,7 +118,7 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
     rid = ("chatcmpl-" if chat else "cmpl-") + uuid.uuid4().hex[:24]
     obj = "chat.completion" if chat else "text_completion"
     base = {"id": rid, "created": int(time.time()), "model": body.get("model") or srv.model_name}
-    keys_qs = [srv.submit([p] * n, sp) for p in prompts]          # one engine group per prompt: its n samples share the prefill
+    keys_qs = [srv.submit([p] * n, sp, adapter=adapter) for p in prompts]          # one engine group per prompt: its n samples share the prefill
     stream = bool(body.get("stream", False))
     if stream:
         h.send_response(200)
@@ -140,6 +148,8 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
                     if delta and final[ci] is None:
                         ch = {"index": ci, "delta": {"content": delta}, "finish_reason": None} if chat else {"index": ci, "text": delta, "finish_reason": None}
                         write({**base, "object": obj + ".chunk" if chat else obj, "choices": [ch]})
+                if "error" in payload:                              # refused by the engine after it was queued
+                    raise ConnectionAbortedError(payload["error"])
                 if fin and final[ci] is None:
                     final[ci] = payload
                     pending[pi] -= 1

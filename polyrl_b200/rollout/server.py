@@ -76,8 +76,8 @@ class EngineServer:
                     info = srv.engine.server_info()
                     self._json(200, {"internal_states": [info], "weight_version": srv.weight_version})
                 elif path == "/v1/models":
-                    self._json(200, {"object": "list", "data": [{"id": srv.model_name, "object": "model", "owned_by": "polyrl_b200",
-                                                                  "max_model_len": srv.engine.max_model_len}]})
+                    self._json(200, {"object": "list", "data": [{"id": name, "object": "model", "owned_by": "polyrl_b200",
+                                                                  "max_model_len": srv.engine.max_model_len} for name in (srv.model_name, *srv.adapter_names())]})
                 else:
                     self._json(404, {"error": "not found"})
 
@@ -115,6 +115,9 @@ class EngineServer:
                     self._json(200, {"success": True})
                 elif path == "/flush_cache":
                     self._json(200, {"success": True})
+                elif path in ("/load_lora_adapter", "/unload_lora_adapter"):
+                    ok, msg = srv._adapter(path[1:].split("_", 1)[0], body)
+                    self._json(200 if ok else 400, {"success": ok, "message": msg})
                 else:
                     self._json(404, {"error": "not found"})
 
@@ -173,12 +176,32 @@ class EngineServer:
         done.wait(timeout=600)
         return result.get("ok", False), result.get("msg", "timeout")
 
-    def submit(self, prompts: list[list[int]], sp: SamplingParams, mm=None) -> tuple[str, "queue.Queue"]:
+    def adapter_names(self) -> list[str]:
+        bank = getattr(self.engine, "adapters", None)
+        return list(bank.names) if bank is not None else []
+
+    def adapter_of(self, name) -> str | None:
+        """The adapter that a request means by its model's name."""
+        return name if name in self.adapter_names() else None
+
+    def _adapter(self, what: str, body: dict):
+        """Load (``lora_name``, ``lora_path``) or unload (``lora_name``) an adapter on the engine thread."""
+        if not body.get("lora_name") or (what == "load" and not body.get("lora_path")):
+            return False, "lora_name" + (" and lora_path" if what == "load" else "") + " required"
+        if self.tp_cmd_group is not None:
+            return False, "adapters with tensor parallelism are not implemented"
+        done, result = threading.Event(), {}
+        with self._lock:
+            self._inbox.append(("adapter", (what, body, result), done))
+        done.wait(timeout=600)
+        return result.get("ok", False), result.get("msg", "timeout")
+
+    def submit(self, prompts: list[list[int]], sp: SamplingParams, mm=None, adapter: str | None = None) -> tuple[str, "queue.Queue"]:
         """Queue token-id prompts for the engine thread; events (index, payload, finished) arrive on the returned queue."""
         q: queue.Queue = queue.Queue()
         key = f"g{id(q)}"
         with self._lock:
-            self._inbox.append(("generate", (key, prompts, sp, q, mm), None))
+            self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter), None))
         return key, q
 
     def _handle_generate(self, h, body: dict):
@@ -188,7 +211,13 @@ class EngineServer:
             return
         batch = bool(ids) and isinstance(ids[0], list)
         prompts = ids if batch else [ids]
-        sp = SamplingParams.from_dict(body.get("sampling_params") or {})
+        adapter = body.get("lora_path")                 # the name that an adapter was loaded under
+        try:
+            sp = SamplingParams.from_dict(body.get("sampling_params") or {})
+            self.engine.check_request(sp, adapter)
+        except (ValueError, TypeError, AttributeError) as e:
+            h._json(400, {"error": str(e)})
+            return
         stream = bool(body.get("stream", False))
         mm = None
         if body.get("image_data") is not None:          # one entry for the whole request, or one per prompt
@@ -196,7 +225,7 @@ class EngineServer:
 
             img = body["image_data"]
             mm = [decode_mm_wire(d) if d is not None else None for d in img] if isinstance(img, list) else [decode_mm_wire(img)] * len(prompts)
-        key, q = self.submit(prompts, sp, mm)
+        key, q = self.submit(prompts, sp, mm, adapter)
         n = len(prompts)
         latest = [None] * n
         if stream:
@@ -257,14 +286,24 @@ class EngineServer:
             for kind, payload, done in cmds:
                 try:
                     if kind == "generate":
-                        key, prompts, sp, q, mm = payload
+                        key, prompts, sp, q, mm, adapter = payload
                         rids = []
                         for _ in prompts:
                             self._rid += 1
                             rids.append(f"s{self._rid}")
                         wire.append(("generate", {"prompts": prompts, "sp": sp.__dict__, "rids": rids, "mm": mm}))
-                        tracked = [_Tracked(r, i) for i, r in enumerate(_add_group(eng, prompts, sp, rids, mm))]
+                        tracked = [_Tracked(r, i) for i, r in enumerate(_add_group(eng, prompts, sp, rids, mm, adapter))]
                         self._streams[key] = (q, tracked)
+                    elif kind == "adapter":
+                        what, body, result = payload
+                        try:
+                            if what == "load":
+                                eng.load_adapter(body["lora_name"], body["lora_path"])
+                            else:
+                                eng.unload_adapter(body["lora_name"])
+                            result["ok"], result["msg"] = True, "ok"
+                        except Exception as e:  # noqa: BLE001  (a bad path or a full bank is the caller's to hear)
+                            result["ok"], result["msg"] = False, str(e)
                     elif kind == "abort_key":
                         ent = self._streams.pop(payload, None)
                         rids = [t.req.rid for t in ent[1]] if ent else []
@@ -295,6 +334,9 @@ class EngineServer:
                 except Exception as e:  # keep the engine thread alive
                     if kind == "update_weights":
                         payload[1]["ok"], payload[1]["msg"] = False, repr(e)
+                    elif kind == "generate" and payload[0] not in self._streams:      # refused: the caller must not wait for it
+                        for i in range(len(payload[1])):
+                            payload[3].put((i, {"index": i, "error": str(e), "output_ids": [], "meta_info": {"finish_reason": {"type": "abort"}}}, True))
                 finally:
                     if done is not None:
                         done.set()
@@ -328,11 +370,12 @@ class EngineServer:
 
 
 # ---------------------------------------------------------------------------------------------- TP lock-step helpers
-def _add_group(eng: RolloutEngine, prompts, sp: SamplingParams, rids, mm=None) -> list[Request]:
+def _add_group(eng: RolloutEngine, prompts, sp: SamplingParams, rids, mm=None, adapter: str | None = None) -> list[Request]:
     """Requests of one HTTP call; identical prompts (with the same image inputs) share their prompt KV as an n-sample group."""
     same_mm = mm is None or all(m is mm[0] for m in mm)
     tag = object() if len(prompts) > 1 and same_mm and all(p == prompts[0] for p in prompts) else None
-    return [eng.add_request(list(map(int, p)), sp, rid=rid, group=tag, mm=mm[i] if mm is not None else None)
+    kw = {} if adapter is None else {"adapter": adapter}
+    return [eng.add_request(list(map(int, p)), sp, rid=rid, group=tag, mm=mm[i] if mm is not None else None, **kw)
             for i, (p, rid) in enumerate(zip(prompts, rids))]
 
 

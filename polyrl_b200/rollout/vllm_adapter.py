@@ -69,6 +69,10 @@ class VLLMRollout:
         kw = dict(n=p.n, temperature=p.temperature, top_p=p.top_p, top_k=p.top_k if p.top_k and p.top_k > 0 else -1,
                   max_tokens=p.max_new_tokens, logprobs=0, ignore_eos=p.ignore_eos, seed=p.seed, detokenize=False,
                   stop_token_ids=[self.cfg.eos_token_id, *self.cfg.extra_eos_token_ids, *p.stop_token_ids])
+        if p.has_rules:
+            kw |= dict(repetition_penalty=p.repetition_penalty, presence_penalty=p.presence_penalty, frequency_penalty=p.frequency_penalty,
+                       min_tokens=p.min_new_tokens, logit_bias=p.logit_bias or None,
+                       allowed_token_ids=None if p.allowed_token_ids is None else list(p.allowed_token_ids))
         try:
             from vllm import SamplingParams as VSP
         except Exception:                              # adapter tests inject a fake ``llm`` without vLLM installed

@@ -14,7 +14,7 @@ int64_t prl_gemm2_ws_floats(int, int, int);
 int64_t prl_gemm2_tail_ws_floats(int, int, int, int);
 int prl_gemm2_tail_bf16(const void*, const void*, const void*, const void*, void*, const void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int, float*, cudaStream_t);
 int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
-int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, cudaStream_t);
+int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, int, int, cudaStream_t);
 int prl_lora_pack(const prl::LoraPackParams*, cudaStream_t);
 int prl_gemm2_grads_joint(int, int, int);
 int prl_gemm2_grads(const void*, const void*, const void*, void*, float*, float, void*, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, cudaStream_t);
@@ -562,18 +562,20 @@ std::vector<at::Tensor> lora_pack(const std::vector<OptT>& a, const std::vector<
 }
 
 // layout 0: scale a [M, K] b [R, K]^T; 1: scale a [M, K] b [K, R]; 2: scale a [K, M]^T b [K, R]; 3: the transpose of that, [R, M].  `rank` columns of
-// b take part (0: all); pad: further columns, ones in the first
-at::Tensor lora_thin(const at::Tensor& a, const at::Tensor& b, int64_t layout, double scale, int64_t rank, int64_t pad, int64_t split) {
-  TORCH_CHECK(a.is_cuda() && layout >= 0 && layout <= 3 && pad >= 0 && pad % 8 == 0 && (layout != 3 || pad == 0), "lora_thin: layout");
+// b take part (0: all); pad: further columns, ones in the first.  halves: out [M, R + pad + R] ends with what rounding to bf16 left of the first R columns.
+// lo: b has such halves from column lo
+at::Tensor lora_thin(const at::Tensor& a, const at::Tensor& b, int64_t layout, double scale, int64_t rank, int64_t pad, bool halves, int64_t lo, int64_t split) {
+  TORCH_CHECK(a.is_cuda() && layout >= 0 && layout <= 3 && pad >= 0 && pad % 8 == 0 && (layout != 3 || (pad == 0 && !halves)) && lo >= 0 && lo % 8 == 0 &&
+              (lo == 0 || layout != 0), "lora_thin: layout");
   const void *pa = lora_operand(a, a, "lora_thin: a"), *pb = lora_operand(b, a, "lora_thin: b");
   const int64_t M = layout >= 2 ? a.size(1) : a.size(0), K = layout >= 2 ? a.size(0) : a.size(1), Kb = layout == 0 ? b.size(1) : b.size(0),
                 width = layout == 0 ? b.size(0) : b.size(1), R = rank > 0 ? rank : width;
-  TORCH_CHECK(K == Kb && R <= width && R % 8 == 0 && M <= 0x7fffffff && K <= 0x7fffffff, "lora_thin: sizes");
+  TORCH_CHECK(K == Kb && R + lo <= width && (lo == 0 || R <= lo) && R % 8 == 0 && M <= 0x7fffffff && K <= 0x7fffffff, "lora_thin: sizes");
   c10::cuda::CUDAGuard g(a.device());
-  at::Tensor out = layout == 3 ? at::empty({R, M}, a.options()) : at::empty({M, R + pad}, a.options());
+  at::Tensor out = layout == 3 ? at::empty({R, M}, a.options()) : at::empty({M, R + pad + (halves ? R : 0)}, a.options());
   if (K == 0) return out.zero_();
   check(prl_lora_thin(pa, pb, out.data_ptr(), M, R, K, a.stride(0), b.stride(0), out.stride(0), static_cast<float>(scale), static_cast<int>(layout),
-                      static_cast<int>(pad), static_cast<int>(split), cur_stream()), "lora_thin");
+                      static_cast<int>(pad), halves ? static_cast<int>(R + pad) : 0, static_cast<int>(lo), static_cast<int>(split), cur_stream()), "lora_thin");
   return out;
 }
 
@@ -630,9 +632,9 @@ std::vector<at::Tensor> lora_fwd(const at::Tensor& x, const at::Tensor& w, const
     pa = p[0];
     pb = p[1];
   }
-  const at::Tensor t = lora_thin(x, pa, 0, scale, 0, pb.size(1) - pa.size(0), 0);
-  if (!swiglu) return {lora_gemm(x, w, t, pb, false, residual), pa, pb, t};
-  std::vector<at::Tensor> y = lora_gemm_swiglu(x, w, t, pb, save);
+  const at::Tensor t = lora_thin(x, pa, 0, scale, 0, pb.size(1) - pa.size(0), save, 0, 0), t1 = t.narrow(1, 0, pb.size(1));
+  if (!swiglu) return {lora_gemm(x, w, t1, pb, false, residual), pa, pb, t};
+  std::vector<at::Tensor> y = lora_gemm_swiglu(x, w, t1, pb, save);
   if (save) return {y[0], pa, pb, t, y[1]};
   return {y[0], pa, pb, t};
 }
@@ -642,14 +644,11 @@ std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::
                            bool need_x, bool need_a, bool need_b) {
   const int64_t r = pa.size(0);
   OptT dx, da, db;
-  if (need_x || need_a) {
-    const at::Tensor dt = lora_thin(dy, pb, 1, scale, r, 0, 0);
-    if (need_b) db = lora_thin(dy, t, 2, 1.0, r, 0, 0);          // right behind the other product that reads dy
-    if (need_x) dx = lora_gemm(dy, w, dt, pa, true, c10::nullopt);
-    if (need_a) da = lora_thin(x, dt, 3, 1.0, 0, 0, 0);
-  } else if (need_b) {
-    db = lora_thin(dy, t, 2, 1.0, r, 0, 0);
-  }
+  at::Tensor dt;
+  if (need_x || need_a) dt = lora_thin(dy, pb, 1, scale, r, 0, need_a, 0, 0);
+  if (need_b) db = lora_thin(dy, t, 2, 1.0, r, 0, false, pb.size(1), 0);              // right behind the other product that reads dy
+  if (need_x) dx = lora_gemm(dy, w, dt.narrow(1, 0, r), pa, true, c10::nullopt);
+  if (need_a) da = lora_thin(x, dt, 3, 1.0, r, 0, false, r, 0);
   return {dx, da, db};
 }
 
@@ -844,7 +843,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lora_fwd", &lora_fwd);
   m.def("lora_bwd", &lora_bwd);
   m.def("lora_thin", &lora_thin, py::arg("a"), py::arg("b"), py::arg("layout"), py::arg("scale") = 1.0, py::arg("rank") = 0, py::arg("pad") = 0,
-        py::arg("split") = 0);
+        py::arg("halves") = false, py::arg("lo") = 0, py::arg("split") = 0);
   m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("b"), py::arg("b_mn") = false, py::arg("residual") = py::none());
   m.def("lora_gemm_swiglu", &lora_gemm_swiglu);
   m.def("stream_gemm", &stream_gemm, py::arg("x"), py::arg("w"), py::arg("residual") = py::none(), py::arg("bias") = py::none(),

@@ -6,7 +6,9 @@
 // R is a few dozen (all parts of a fused projection side by side, B block-diagonal), the other two sides are thousands, so each product reads
 // its one large operand (x or dy) once and is bound by that.  y += t B^T and dx += dt A are not here: t and dt are further k-blocks of the
 // large products (gemm2_sm100.cuh, Gemm2Tail), so what the adapter adds is summed in fp32 with the rest, rounds nothing of its own and moves
-// no [T, N] or [T, K] array.  t and dt are rounded to bf16 (2^-8 relative at most), as every operand of a product is.
+// no [T, N] or [T, K] array.  There t and dt are bf16, as every operand of a product is (2^-8 at most of what the adapter adds).  The gradients dA and
+// dB are all adapter, so for them t and dt come in two bf16 halves, the rounded value and what rounding left (2^-16): twice the columns of a product
+// that is bound by its other operand.
 //
 // thin   D[m, r] = scale * sum_k A(m, k) B(r, k), 128 rows of D a tile: tcgen05.mma 128 x R x 16, both operands by TMA (K-major, or MN-major
 //        where the sum runs over tokens: dA is computed as x^T dt and stored transposed).  A cluster of S CTAs shares a tile's reduction,
@@ -24,8 +26,10 @@ constexpr int kThinThreads = 192;                    // warp 0 TMA, warp 1 MMA, 
 constexpr int kThinStageA = kBlockM * 128;
 constexpr int kThinSmemMax = 201 * 1024;
 
+// columns of the accumulator: NR, or twice that with the second half behind a whole number of 64-column boxes
+__host__ __device__ constexpr int thin_lo(int NR) { return (NR + 63) / 64 * 64; }
 template <bool MN>
-__host__ __device__ constexpr int thin_b_bytes(int NR) { return MN ? (NR + 63) / 64 * 8192 : NR * 128; }
+__host__ __device__ constexpr int thin_b_bytes(int NR, bool halves) { return MN ? (halves ? 2 : 1) * ((NR + 63) / 64) * 8192 : NR * 128; }
 
 struct ThinParams {
   __nv_bfloat16* out;
@@ -33,6 +37,8 @@ struct ThinParams {
   int M, R, K, NR, stages;
   float scale;
   int pad;                                           // columns after the last one: the first is 1, the rest 0 (row-major output)
+  int lo_out;                                        // > 0: column of the outputs' second halves (row-major output)
+  int lo_in;                                         // > 0: the same of B (MN-major)
 };
 
 // grid (tiles * S, blocks of NR columns); A_MN / B_MN: the reduction runs over the operand's rows in memory; TRANS: out is [R, M]
@@ -42,14 +48,15 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[8], empty_bar[8], done_bar;
   __shared__ uint32_t tmem_slot;
-  const int b_bytes = thin_b_bytes<B_MN>(p.NR), stage_bytes = kThinStageA + b_bytes;
+  const int b_bytes = thin_b_bytes<B_MN>(p.NR, p.lo_in > 0), stage_bytes = kThinStageA + b_bytes;
+  const int cols_acc = B_MN && p.lo_in > 0 ? thin_lo(p.NR) + p.NR : p.NR, ld_acc = cols_acc + 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t S;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
   const uint32_t rank = cluster_ctarank();
   const int m0 = blockIdx.x / S * kBlockM, r0 = blockIdx.y * p.NR;
   const int num_kb = (p.K + 63) / 64, kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
-  const uint32_t tmem_cols = p.NR <= 32 ? 32 : p.NR <= 64 ? 64 : p.NR <= 128 ? 128 : 256;
+  const uint32_t tmem_cols = cols_acc <= 32 ? 32 : cols_acc <= 64 ? 64 : cols_acc <= 128 ? 128 : 256;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
@@ -87,7 +94,10 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
           tma_load_2d(&tmA, &full_bar[stage], sa, kb * 64, m0);
         }
         if constexpr (B_MN) {
-          for (int c = 0; c < p.NR; c += 64) tma_load_2d(&tmB, &full_bar[stage], sb + c / 64 * 8192, r0 + c, kb * 64);
+          for (int c = 0; c < p.NR; c += 64) {
+            tma_load_2d(&tmB, &full_bar[stage], sb + c / 64 * 8192, r0 + c, kb * 64);
+            if (p.lo_in > 0) tma_load_2d(&tmB, &full_bar[stage], sb + (thin_lo(p.NR) + c) / 64 * 8192, p.lo_in + r0 + c, kb * 64);
+          }
         } else {
           tma_load_2d(&tmB, &full_bar[stage], sb, kb * 64, r0);
         }
@@ -96,7 +106,7 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = umma_idesc_major(kBlockM, p.NR, 1, 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
+      const uint32_t idesc = umma_idesc_major(kBlockM, cols_acc, 1, 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
       constexpr uint32_t a_step = A_MN ? (16 * 128) >> 4 : 32 >> 4, b_step = B_MN ? (16 * 128) >> 4 : 32 >> 4;
       int stage = 0;
       uint32_t phase = 0;
@@ -115,13 +125,13 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
       umma_commit(&done_bar);
     }
   } else {
-    // every load has landed and every product has read its stage: the pipeline's memory takes the sums, rows of NR + 4 floats (an odd number
+    // every load has landed and every product has read its stage: the pipeline's memory takes the sums, rows of cols_acc + 4 floats (an odd number
     // of 16-byte units, so that 8 lanes' rows start in different banks)
     mbar_wait(&done_bar, 0);
     tc_fence_after();
     const int quad = warp & 3, row = quad * 32 + lane;
-    float* dst = reinterpret_cast<float*>(smem) + row * (p.NR + 4);
-    for (int c = 0; c < p.NR; c += 16) {
+    float* dst = reinterpret_cast<float*>(smem) + row * ld_acc;
+    for (int c = 0; c < cols_acc; c += 16) {
       uint32_t r[16];
       __syncwarp();
       tmem_ld_32x16(tmem + c + (static_cast<uint32_t>(quad * 32) << 16), r);
@@ -140,8 +150,8 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
 
   // four columns of a row, summed over the ranks
   const uint32_t base = smem_u32(smem);
-  auto sum = [&](int row, int c) {
-    const uint32_t off = base + (row * (p.NR + 4) + c) * 4;
+  auto ranks = [&](int row, int c) {
+    const uint32_t off = base + (row * ld_acc + c) * 4;
     float4 q[8];
 #pragma unroll
     for (uint32_t k = 0; k < 8; ++k)
@@ -154,6 +164,14 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
 #pragma unroll
     for (uint32_t k = 1; k < 8; ++k)
       if (k < S) { v.x += q[k].x; v.y += q[k].y; v.z += q[k].z; v.w += q[k].w; }
+    return v;
+  };
+  auto sum = [&](int row, int c) {
+    float4 v = ranks(row, c);
+    if (B_MN && p.lo_in > 0) {
+      const float4 l = ranks(row, thin_lo(p.NR) + c);
+      v.x += l.x; v.y += l.y; v.z += l.z; v.w += l.w;
+    }
     return make_float4(v.x * p.scale, v.y * p.scale, v.z * p.scale, v.w * p.scale);
   };
   const int cols = min(p.NR, p.R - r0);
@@ -164,7 +182,13 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
       const int row = rows0 + e / quads, c = e % quads * 4;
       if (m0 + row >= p.M) break;
       const float4 v = c < cols ? sum(row, c) : make_float4(c == cols ? 1.f : 0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(m0 + row) * p.ldo + r0 + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      const uint2 hi = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      __nv_bfloat16* o = p.out + static_cast<int64_t>(m0 + row) * p.ldo + r0 + c;
+      *reinterpret_cast<uint2*>(o) = hi;
+      if (p.lo_out > 0 && c < cols) {
+        const float2 a = unpack_bf16(hi.x), b = unpack_bf16(hi.y);
+        *reinterpret_cast<uint2*>(o + p.lo_out) = make_uint2(pack_bf16(v.x - a.x, v.y - a.y), pack_bf16(v.z - b.x, v.w - b.y));
+      }
     }
   } else {                                           // a share of the columns, lanes along the tile's rows
     const int quads = cols / 4, q0 = quads * rank / S, q1 = quads * (rank + 1) / S;
@@ -184,14 +208,17 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
 
 template <bool A_MN, bool B_MN, bool TRANS>
 static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int64_t ldb, int split, cudaStream_t stream) {
-  p.NR = p.R >= 256 ? 256 : (p.R + 15) / 16 * 16;
-  const int stage = kThinStageA + thin_b_bytes<B_MN>(p.NR), sums = kBlockM * (p.NR + 4) * 4;
-  const int budget = p.NR <= 128 ? 100 * 1024 : 200 * 1024;           // two CTAs an SM where two fit
+  const bool halves = B_MN && p.lo_in > 0;
+  const int most = halves ? 128 : 256;
+  p.NR = p.R >= most ? most : (p.R + 15) / 16 * 16;
+  const int cols = halves ? thin_lo(p.NR) + p.NR : p.NR;
+  const int stage = kThinStageA + thin_b_bytes<B_MN>(p.NR, halves), sums = kBlockM * (cols + 4) * 4;
+  const int budget = cols <= 128 ? 100 * 1024 : 200 * 1024;           // two CTAs an SM where two fit
   p.stages = budget / stage > 8 ? 8 : budget / stage;
   const int smem = (p.stages * stage > sums ? p.stages * stage : sums) + 1024;
   CUtensorMap tmA, tmB;
   if (A_MN ? make_tmap_kmajor(&tmA, A, p.K, p.M, lda * 2, 64, 2) : make_tmap_kmajor(&tmA, A, p.M, p.K, lda * 2, kBlockM, 2)) return -2;
-  if (B_MN ? make_tmap_kmajor(&tmB, B, p.K, p.R, ldb * 2, 64, 2) : make_tmap_kmajor(&tmB, B, p.R, p.K, ldb * 2, p.NR, 2)) return -3;
+  if (B_MN ? make_tmap_kmajor(&tmB, B, p.K, halves ? p.lo_in + p.R : p.R, ldb * 2, 64, 2) : make_tmap_kmajor(&tmB, B, p.R, p.K, ldb * 2, p.NR, 2)) return -3;
   const int tiles = (p.M + kBlockM - 1) / kBlockM, blocks = (p.R + p.NR - 1) / p.NR, num_kb = (p.K + 63) / 64;
   int S = split;
   if (S <= 0) {
@@ -265,12 +292,13 @@ __global__ void __launch_bounds__(256) lora_pack_kernel(const LoraPackParams p) 
 using namespace prl;
 
 // layout 0: A [M, K], B [R, K]; 1: A [M, K], B [K, R]; 2: A [K, M], B [K, R]; 3: as 2, out [R, M].  Pitches in elements, multiples of 8.
-// pad > 0 (layouts 0 to 2): so many more columns of out, ones in the first.
+// pad > 0 (layouts 0 to 2): so many more columns of out, ones in the first.  lo_out > 0 (0 to 2): out gets what rounding left in columns lo_out on;
+// lo_in > 0 (1 to 3): B has such halves from column lo_in.
 extern "C" int prl_lora_thin(const void* A, const void* B, void* out, int M, int R, int K, int64_t lda, int64_t ldb, int64_t ldo, float scale, int layout, int pad,
-                             int split, cudaStream_t stream) {
+                             int lo_out, int lo_in, int split, cudaStream_t stream) {
   if (M <= 0 || R <= 0 || K <= 0) return 0;
-  if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || (layout != 3 && ldo % 4)) return -1;
-  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad};
+  if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || lo_out % 8 || lo_in % 8 || (layout != 3 && ldo % 4) || (layout == 3 && lo_out) || (layout == 0 && lo_in)) return -1;
+  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad, lo_out, lo_in};
   switch (layout) {
     case 0: return run_thin<false, false, false>(A, B, p, lda, ldb, split, stream);
     case 1: return run_thin<false, true, false>(A, B, p, lda, ldb, split, stream);

@@ -152,9 +152,9 @@ def lora_value64(x, w, parts, widths, scale, dy, bias=None, residual=None, swigl
 
 
 def lora64(x, w, parts, widths, scale, dy, bias=None, residual=None, swiglu=False):
-    """{name: (value, bound before the last rounding)} of y, dx and of every part's da, db: low-rank values, their gradients and, with swiglu, the
-    projection and its gradient are rounded to bf16; sums in fp32."""
-    u = 2.0 ** -8
+    """{name: (value, bound before the last rounding)} of y, dx and of every part's da, db: low-rank values and their gradients are rounded to bf16
+    (for da and db to two bf16 numbers, 2^-8 of 2^-8 of the value), with swiglu the projection and its gradient too; sums in fp32."""
+    u, u2 = 2.0 ** -8, 2.0 ** -16
     x, w, dy = x.double(), w.double(), dy.double()
     (t_rows, k), n, dev = x.shape, w.shape[0], x.device
     part = part_of(n, widths, swiglu).to(dev)
@@ -168,11 +168,12 @@ def lora64(x, w, parts, widths, scale, dy, bias=None, residual=None, swiglu=Fals
             continue
         a, b = p
         t = scale * (x @ a.t())
-        et = u * t.abs() + (k + 3) * U32 * abs(scale) * (x.abs() @ a.abs().t())
+        sums = (k + 3) * U32 * abs(scale) * (x.abs() @ a.abs().t())
+        et = u * t.abs() + sums
         z[:, c] += t @ b.t()
         mag[:, c] += t.abs() @ b.abs().t()
         err[:, c] += et @ b.abs().t()
-        low.append((t, et))
+        low.append((t, u2 * t.abs() + 2 * sums))
     for extra in (bias, residual):
         if extra is not None:
             z, mag = z + extra.double(), mag + extra.double().abs()
@@ -199,9 +200,10 @@ def lora64(x, w, parts, widths, scale, dy, bias=None, residual=None, swiglu=Fals
         (a, b), (t, et), d, e = p, l, dy[:, c], ed[:, c]
         dt = scale * (d @ b)
         edt = abs(scale) * (e @ b.abs())
-        edt = edt + u * (dt.abs() + edt) + (n + 3) * U32 * abs(scale) * ((d.abs() + e) @ b.abs())
-        dx, edx, mdx = dx + dt @ a, edx + edt @ a.abs(), mdx + dt.abs() @ a.abs()
-        out[f"da{i}"] = (dt.t() @ x, edt.t() @ x.abs() + (t_rows + 8) * U32 * (dt.abs().t() @ x.abs()))
-        out[f"db{i}"] = (d.t() @ t, e.t() @ (t.abs() + et) + d.abs().t() @ et + (t_rows + 8) * U32 * (d.abs().t() @ t.abs()))
+        edt = edt + (n + 3) * U32 * abs(scale) * ((d.abs() + e) @ b.abs())
+        dx, edx, mdx = dx + dt @ a, edx + (edt + u * (dt.abs() + edt)) @ a.abs(), mdx + dt.abs() @ a.abs()
+        edt = edt + u2 * (dt.abs() + edt)
+        out[f"da{i}"] = (dt.t() @ x, edt.t() @ x.abs() + (2 * t_rows + 8) * U32 * (dt.abs().t() @ x.abs()))
+        out[f"db{i}"] = (d.t() @ t, e.t() @ (t.abs() + et) + d.abs().t() @ et + (2 * t_rows + 8) * U32 * (d.abs().t() @ t.abs()))
     out["dx"] = (dx, edx + (n + 400) * U32 * (mdx + edx))
     return out

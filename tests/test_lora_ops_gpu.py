@@ -19,13 +19,31 @@ def test_thin_products(layout, m, r, k, split):
     a, b = torch.randn(m8, k, generator=g).to(BF).cuda(), torch.randn(r, k, generator=g).to(BF).cuda()
     ref, mag = 0.5 * (a.double() @ b.double().t()), 0.5 * (a.double().abs() @ b.double().abs().t())
     pad = 8 if layout < 3 else 0
-    got = ops.ext().lora_thin(a.t().contiguous() if layout >= 2 else a, b if layout == 0 else b.t().contiguous(), layout, 0.5, 0, pad, split)
+    got = ops.ext().lora_thin(a.t().contiguous() if layout >= 2 else a, b if layout == 0 else b.t().contiguous(), layout, 0.5, 0, pad, False, 0, split)
     if layout == 3:
         got = got.t()
     else:
         assert (got[:, r] == 1).all() and (got[:, r + 1:] == 0).all()
         got = got[:, :r]
     check_near(got, ref, (k + 2) * 2.0 ** -24 * mag)
+
+
+@pytest.mark.parametrize("t,r,k,n,pad", [(70, 8, 64, 72, 0), (130, 48, 200, 136, 8), (515, 64, 512, 128, 8), (300, 136, 264, 200, 0), (257, 264, 136, 72, 8)])
+def test_halves(t, r, k, n, pad):
+    """A thin product in two bf16 halves, and the products over tokens that read both: as if it had 16 bits of mantissa."""
+    g = torch.Generator().manual_seed(t)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    x, a, dy = rnd(t, k), rnd(r, k), rnd(t, n)
+    C = ops.ext()
+    low = C.lora_thin(x, a, 0, 0.5, 0, pad, True)
+    ref, mag = 0.5 * (x.double() @ a.double().t()), 0.5 * (x.double().abs() @ a.double().abs().t())
+    both = low[:, :r].double() + low[:, r + pad:].double()
+    assert low.shape[1] == 2 * r + pad and ((both - ref).abs() <= 2.0 ** -16 * ref.abs() + (k + 2) * 2.0 ** -24 * mag).all()
+    assert torch.equal(low[:, :r + pad], C.lora_thin(x, a, 0, 0.5, 0, pad))
+    want, most = dy.double().t() @ both, dy.double().abs().t() @ (both.abs() * (1 + 2.0 ** -7))
+    for split in (0, 1, 2):
+        check_near(C.lora_thin(dy, low, 2, 1.0, r, 0, False, r + pad, split), want, (2 * t + 4) * 2.0 ** -24 * most)
+        check_near(C.lora_thin(dy, low, 3, 1.0, r, 0, False, r + pad, split).t(), want, (2 * t + 4) * 2.0 ** -24 * most)
 
 
 @pytest.mark.parametrize("t,k,widths,ranks", [

@@ -80,6 +80,7 @@ at::Tensor adjust_logits(const at::Tensor& z, OptTensor out, const OptTensor& to
     p.num_masks = masks->size(0);
     TORCH_CHECK_VALUE(masks->size(1) >= (V + 31) / 32 && (p.mask_rows || p.num_masks == rows), "adjust_logits: masks [masks, ceil(vocabulary / 32)], one a row or mask_rows");
   }
+  if (out.has_value() && !o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
   check(prl_adjust_logits(&p, z.scalar_type() == at::kFloat, cur_stream()), "adjust_logits");
   return o;
 }
@@ -135,9 +136,10 @@ at::Tensor adapter_delta(const at::Tensor& x, const at::Tensor& a, const at::Ten
     p.ldr = residual->stride(0);
   }
   c10::cuda::CUDAGuard g(x.device());
-  if (onto.has_value())
-    TORCH_CHECK_VALUE(onto->dim() == 2 && onto->is_contiguous() && onto->size(0) == T && onto->size(1) == N && delta_operand(*onto, x, "adapter_delta: onto"),
-                      "adapter_delta: onto [T, N]");
+  if (onto.has_value()) {
+    TORCH_CHECK_VALUE(onto->dim() == 2 && onto->is_contiguous() && onto->size(0) == T && onto->size(1) == N, "adapter_delta: onto [T, N]");
+    delta_operand(*onto, x, "adapter_delta: onto");
+  }
   at::Tensor out = onto.has_value() ? *onto : at::empty({T, N}, x.options());
   if (T == 0) return out;
   p.onto = onto.has_value();

@@ -74,7 +74,10 @@ def _check_adapters(name: str, x, w, a, b, scales, plan: AdapterPlan, widths, bi
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows as the kernels read them: unit inner stride, pitch and base on 16 bytes."""
-    return t if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else fn._aligned(t)
+    if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    t = fn._aligned(t)
+    return t if t.shape[0] != 1 else t.as_strided(t.shape, (t.shape[1], 1))      # a single row counts as contiguous whatever its pitch is
 
 
 def _delta(x, a, b, scales, plan, widths, interleaved, bias=None, residual=None, onto=None):

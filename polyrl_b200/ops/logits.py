@@ -36,11 +36,6 @@ class LogitRules:
     masks: torch.Tensor | None = None          # [M, ceil(V / 32)] int32
     mask_rows: torch.Tensor | None = None      # [B] int32
 
-    def rows(self, b: int) -> "LogitRules":
-        """The rules of the first ``b`` rows."""
-        return LogitRules(**{f.name: getattr(self, f.name) if f.name == "masks" and self.mask_rows is not None or getattr(self, f.name) is None
-                             else getattr(self, f.name)[:b] for f in fields(self)})
-
 
 _FLOATS = {"repetition", "presence", "frequency", "bias_values"}
 _MATRICES = {"tokens", "bias_ids", "bias_values", "stop_ids", "masks"}
@@ -91,7 +86,7 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | N
           -> z + bias
           -> -inf                                             where the mask, or the least length, does not let it come
 
-    in fp32, rounded once.  The kernel may be captured; no gradient."""
+    in fp32, rounded once.  The kernel may be captured; no gradient (writing in place counts as a change of the tensor)."""
     if logits.is_cuda:                   # (checks its arguments as _check does)
         from . import ext
 

@@ -104,7 +104,7 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
         sp = _sampling(body)
         n = max(1, int(body.get("n") or 1))
         adapter = srv.adapter_of(body.get("model"))
-        srv.engine.check_request(sp, adapter)
+        srv.check_request(sp, adapter)
     except (ValueError, TypeError, KeyError, AttributeError) as e:
         h._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})
         return

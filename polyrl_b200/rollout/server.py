@@ -176,6 +176,12 @@ class EngineServer:
         done.wait(timeout=600)
         return result.get("ok", False), result.get("msg", "timeout")
 
+    def check_request(self, sp: SamplingParams, adapter: str | None) -> None:
+        """ValueError for what the engine would refuse (engines of other kinds say so themselves)."""
+        check = getattr(self.engine, "check_request", None)
+        if check is not None:
+            check(sp, adapter)
+
     def adapter_names(self) -> list[str]:
         bank = getattr(self.engine, "adapters", None)
         return list(bank.names) if bank is not None else []
@@ -214,7 +220,7 @@ class EngineServer:
         adapter = body.get("lora_path")                 # the name that an adapter was loaded under
         try:
             sp = SamplingParams.from_dict(body.get("sampling_params") or {})
-            self.engine.check_request(sp, adapter)
+            self.check_request(sp, adapter)
         except (ValueError, TypeError, AttributeError) as e:
             h._json(400, {"error": str(e)})
             return

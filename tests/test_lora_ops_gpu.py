@@ -105,6 +105,11 @@ def test_views_and_odd_starts():
         v.copy_(t)
         return v
 
+    one = {k: (v[:1] if k in ("x", "dy", "residual") else v) for k, v in c.items()}
+    wide = torch.empty(3, 77, dtype=BF, device="cuda")[1:2, 5:69]             # a single row of an odd pitch
+    wide.copy_(one["x"])
+    for (n, t), u in zip(run_lora(dict(one, x=wide)).items(), run_lora(one).values()):
+        assert torch.equal(t, u), n
     for by in (8, 3):
         o = dict(c, x=shifted(c["x"], by), w=shifted(c["w"], by), dy=shifted(c["dy"], by), residual=shifted(c["residual"], by),
                  parts=[tuple(shifted(m, by) for m in p) for p in c["parts"]])

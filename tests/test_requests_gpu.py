@@ -235,6 +235,28 @@ def test_adapters_views_streams_and_graph():
         check_near(y, *near64(c, (128, 64)))
 
 
+def test_no_rows_and_one_row_of_an_odd_pitch():
+    c = adapters_case(0, 64, (256,), 16, 2, 0, torch.bfloat16, "cuda")
+    assert run_adapters(c, (256,), 2).shape == (0, 256)
+    c["b"], c["a"] = c["b"], torch.cat([c["a"], c["a"]], 1)
+    assert ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], 2)).shape == (0, 128)
+    wide = torch.randn(5, 77, device="cuda").bfloat16()
+    for t in (1, 2):
+        c = adapters_case(t, 64, (64,), 16, 2, 1, torch.bfloat16, "cuda")
+        for x in (wide[2:2 + t, 1:65], wide[2:2 + t, 8:72]):
+            x.copy_(c["x"])
+            check_near(run_adapters(dict(c, x=x, residual=x), (64,), 2), *near64(dict(c, residual=x), (64,)))
+
+
+def test_rules_in_place_count_as_a_change():
+    z, case = rules_case(2, 40, 5, 0, torch.float32, "cuda")
+    before = z._version
+    ops.adjust_logits(z, LogitRules(**case))
+    assert z._version == before
+    ops.adjust_logits(z, LogitRules(**case), out=z)
+    assert z._version > before
+
+
 def test_adapters_refused_by_the_kernel_entry():
     c = adapters_case(4, 64, (64,), 16, 2, 0, torch.bfloat16, "cuda")
     plan = ops.adapter_plan(c["ids"], 2)

@@ -125,7 +125,8 @@ struct DeltaCfg {
   static int smem(int R) { return TM * R * 4 + KW * TM * kLowChunk * 4 + TM * (R + 8) * 2; }
 };
 
-template <int TM>
+// ADD: bias, res or onto are there
+template <int TM, bool ADD>
 __global__ void __launch_bounds__(DeltaCfg<TM>::THREADS, 2) delta_kernel(const DeltaParams p) {
   using Cfg = DeltaCfg<TM>;
   constexpr int MT = Cfg::MT, KW = Cfg::KW, kThreads = Cfg::THREADS;
@@ -239,16 +240,18 @@ __global__ void __launch_bounds__(DeltaCfg<TM>::THREADS, 2) delta_kernel(const D
     const int col = g * 32;
     const int pt = p.interleaved ? (col >> 7) & 1 : (p.parts > 1 && col >= p.ends[0]) + (p.parts > 2 && col >= p.ends[1]);
     const int4 none = make_int4(0, 0, 0, 0);
-    const int4 extra = p.bias ? __ldg(reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.bias) + col + quad * 8)) : none;
-    int4 add[MT][2], own[MT][2];
+    int4 extra = none, add[MT][2], own[MT][2];
+    if constexpr (ADD) {
+      if (p.bias) extra = __ldg(reinterpret_cast<const int4*>(static_cast<const __nv_bfloat16*>(p.bias) + col + quad * 8));
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = rows_sm[m * 16 + grp + 8 * h];
-        add[m][h] = p.res && row >= 0 ? ld_nc_v4(static_cast<const __nv_bfloat16*>(p.res) + static_cast<int64_t>(row) * p.ldr + col + quad * 8) : none;
-        own[m][h] = p.onto && row >= 0 ? ld_v4(static_cast<const __nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8) : none;
-      }
+        for (int h = 0; h < 2; ++h) {
+          const int row = rows_sm[m * 16 + grp + 8 * h];
+          add[m][h] = p.res && row >= 0 ? ld_nc_v4(static_cast<const __nv_bfloat16*>(p.res) + static_cast<int64_t>(row) * p.ldr + col + quad * 8) : none;
+          own[m][h] = p.onto && row >= 0 ? ld_v4(static_cast<const __nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8) : none;
+        }
+    }
     float acc[MT][4][4] = {};
     if (tile.adapter >= 0) {
       const __nv_bfloat16* b = b_row(col);
@@ -283,22 +286,26 @@ __global__ void __launch_bounds__(DeltaCfg<TM>::THREADS, 2) delta_kernel(const D
         }
       }
     }
-    const uint32_t* ex = reinterpret_cast<const uint32_t*>(&extra);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = rows_sm[m * 16 + grp + 8 * h];
         if (row < 0) continue;
-        const uint32_t *rv = reinterpret_cast<const uint32_t*>(&add[m][h]), *ov = reinterpret_cast<const uint32_t*>(&own[m][h]);
-        uint32_t o[4];
+        int4 o;
+        int* ow = reinterpret_cast<int*>(&o);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 e = unpack_bf16(ex[j]), r = unpack_bf16(rv[j]), y = unpack_bf16(ov[j]);
-          o[j] = pack_bf16(acc[m][j][2 * h] + e.x + r.x + y.x, acc[m][j][2 * h + 1] + e.y + r.y + y.y);
+          float2 v = make_float2(acc[m][j][2 * h], acc[m][j][2 * h + 1]);
+          if constexpr (ADD) {
+            const float2 e = unpack_bf16(reinterpret_cast<const uint32_t*>(&extra)[j]), r = unpack_bf16(reinterpret_cast<const uint32_t*>(&add[m][h])[j]),
+                         y = unpack_bf16(reinterpret_cast<const uint32_t*>(&own[m][h])[j]);
+            v.x += e.x + r.x + y.x;
+            v.y += e.y + r.y + y.y;
+          }
+          ow[j] = static_cast<int>(pack_bf16(v.x, v.y));
         }
-        st_v4(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8,
-              make_int4(static_cast<int>(o[0]), static_cast<int>(o[1]), static_cast<int>(o[2]), static_cast<int>(o[3])));
+        st_v4(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col + quad * 8, o);
       }
   }
 }
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(DeltaCfg<TM>::THREADS, 2) delta_kernel(const D
 template <int TM>
 static int run_delta(const DeltaParams& p, int ctas, cudaStream_t stream) {
   const int smem = DeltaCfg<TM>::smem(p.parts * p.rank);
-  auto kern = delta_kernel<TM>;
+  auto kern = p.bias || p.res || p.onto ? delta_kernel<TM, true> : delta_kernel<TM, false>;
   PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaCfg<TM>::smem(kDeltaMaxLow)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles) * p.shares * ctas);

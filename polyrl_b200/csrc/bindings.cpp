@@ -639,17 +639,33 @@ std::vector<at::Tensor> lora_fwd(const at::Tensor& x, const at::Tensor& w, const
   return {y[0], pa, pb, t};
 }
 
-// and the backward: {dx, dA [R, K], dB [N, R]}, undefined where not asked for
+// and the backward: {dx, dA and dB of part 0, of part 1, ..}, undefined where not asked for (`want`: one entry for each).  Parts are views of two results.
 std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const at::Tensor& pa, const at::Tensor& pb, const at::Tensor& t, double scale,
-                           bool need_x, bool need_a, bool need_b) {
+                           const std::vector<int64_t>& ranks, const std::vector<int64_t>& widths, bool swiglu, const std::vector<bool>& want) {
+  TORCH_CHECK(ranks.size() == widths.size() && want.size() == 1 + 2 * ranks.size(), "lora_bwd: parts");
   const int64_t r = pa.size(0);
-  OptT dx, da, db;
-  at::Tensor dt;
-  if (need_x || need_a) dt = lora_thin(dy, pb, 1, scale, r, 0, need_a, 0, 0);
+  bool need_a = false, need_b = false;
+  for (size_t i = 0; i < ranks.size(); ++i) {
+    need_a |= ranks[i] > 0 && want[1 + 2 * i];
+    need_b |= ranks[i] > 0 && want[2 + 2 * i];
+  }
+  std::vector<OptT> out(want.size());
+  at::Tensor dt, da, db;
+  if (want[0] || need_a) dt = lora_thin(dy, pb, 1, scale, r, 0, need_a, 0, 0);
   if (need_b) db = lora_thin(dy, t, 2, 1.0, r, 0, false, pb.size(1), 0);              // right behind the other product that reads dy
-  if (need_x) dx = lora_gemm(dy, w, dt.narrow(1, 0, r), pa, true, c10::nullopt);
+  if (want[0]) out[0] = lora_gemm(dy, w, dt.narrow(1, 0, r), pa, true, c10::nullopt);
   if (need_a) da = lora_thin(x, dt, 3, 1.0, r, 0, false, r, 0);
-  return {dx, da, db};
+  int64_t col = 0, row = 0;
+  for (size_t i = 0; i < ranks.size(); ++i) {
+    if (ranks[i] > 0 && want[1 + 2 * i]) out[1 + 2 * i] = da.narrow(0, col, ranks[i]);
+    if (ranks[i] > 0 && want[2 + 2 * i]) {
+      const at::Tensor rows = swiglu ? db.view({-1, 2, 128, r}).select(1, i).reshape({widths[i], r}) : db.narrow(0, row, widths[i]);
+      out[2 + 2 * i] = rows.narrow(1, col, ranks[i]);
+    }
+    col += (ranks[i] + 7) / 8 * 8;
+    row += widths[i];
+  }
+  return out;
 }
 
 // Row-parallel TP linear with the all-reduce fused into the GEMM epilogue over NVLink peer memory.

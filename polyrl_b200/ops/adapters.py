@@ -187,19 +187,8 @@ class _LoraFn(torch.autograd.Function):
             return (None, None, dbias, dres, *[None] * (3 + 2 * len(ranks)))
         x, w, pa, pb, t, *gu = ctx.saved_tensors
         dy = C.swiglu_bwd(gu[0], fn._aligned(dy)) if swiglu else _rows(dy)
-        r, dw = pa.shape[0], None
-        dx, da, db = C.lora_bwd(dy, x, w, pa, pb, t, scale, need[0], any(need[7::2]), any(need[8::2]))
-        if need[1]:
-            dw = fn.mm_tn(dy, x, out=fn._sink_for(w))
-        grads, col, row = [], 0, 0
-        for i, (rank, m) in enumerate(zip(ranks, widths)):
-            grads.append(da[col:col + rank] if rank and need[7 + 2 * i] else None)
-            if rank and need[8 + 2 * i]:
-                mine = db.view(-1, 2, 128, r)[:, i].reshape(m, r) if swiglu else db[row:row + m]
-                grads.append(mine[:, col:col + rank])
-            else:
-                grads.append(None)
-            col, row = col + -(-rank // 8) * 8, row + m
+        dx, *grads = C.lora_bwd(dy, x, w, pa, pb, t, scale, ranks, widths, swiglu, (need[0], *need[7:]))
+        dw = fn.mm_tn(dy, x, out=fn._sink_for(w)) if need[1] else None
         return (dx, dw, dbias, dres, None, None, None, *grads)
 
 
@@ -231,9 +220,11 @@ def _lora(x, w, parts, widths, scale, bias, residual, swiglu):
     if not kernel:
         y = _lora_reference(x, w, adapters, widths, scale, bias, residual, swiglu)
         return ref.swiglu(y) if swiglu else y
-    ab = [t for p in adapters for t in ((None, None) if p is None else (p[0].to(x.dtype), p[1].to(x.dtype)))]
+    ab = [t if t is None or t.dtype == x.dtype else t.to(x.dtype) for p in adapters for t in p or (None, None)]
+    if x.dim() == 2:
+        return _LoraFn.apply(x, w, bias, residual, float(scale), widths, swiglu, *ab)
     y = _LoraFn.apply(x.reshape(-1, x.shape[-1]), w, bias, None if residual is None else residual.reshape(-1, w.shape[0]), float(scale), widths, swiglu, *ab)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])
+    return y.reshape(*x.shape[:-1], y.shape[1])
 
 
 def lora_linear(x: torch.Tensor, w: torch.Tensor, parts, scale: float, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:

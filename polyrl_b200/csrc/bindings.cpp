@@ -16,6 +16,8 @@ int prl_gemm2_tail_bf16(const void*, const void*, const void*, const void*, void
 int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
 int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, int, int, cudaStream_t);
 int prl_lora_pack(const prl::LoraPackParams*, cudaStream_t);
+int prl_adapter_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, int, const int32_t*, const float*, int, cudaStream_t);
+int prl_adapter_pack(const void*, const void*, void*, const prl::LoraPackParams*, int, int, cudaStream_t);
 int prl_gemm2_grads_joint(int, int, int);
 int prl_gemm2_grads(const void*, const void*, const void*, void*, float*, float, void*, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, cudaStream_t);
 int prl_gemm2_bf16_accum_f32(const void*, const void*, float*, float, int, int, int, int64_t, int64_t, int64_t, int, int, float*, cudaStream_t);
@@ -668,6 +670,37 @@ std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::
   return out;
 }
 
+// Many rows whose adapters differ, through the large product: the low-rank values of all adapters side by side, a row's own kept, against all adapters' b
+// (adapters.cu says what it computes).  swiglu: gate and up interleaved, their activation returned.
+at::Tensor adapter_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scales, const at::Tensor& ids,
+                        const std::vector<int64_t>& widths, bool swiglu, const OptT& bias, const OptT& residual) {
+  TORCH_CHECK_VALUE(a.dim() == 3 && b.dim() == 3 && a.is_contiguous() && b.is_contiguous() && a.size(0) == b.size(0) && !widths.empty() && widths.size() <= 3,
+                    "adapter_gemm: a [adapters, parts * rank, K], b [adapters, N, rank]");
+  const int64_t L = a.size(0), each = a.size(1), K = a.size(2), N = b.size(1), rank = b.size(2), R = L * each, T = x.size(0), pad = bias.has_value() ? 8 : 0;
+  prl::LoraPackParams p{};
+  p.parts = widths.size();
+  int64_t end = 0;
+  for (int i = 0; i < p.parts; ++i) p.ends[i] = end += widths[i];
+  TORCH_CHECK_VALUE(end == N && each == p.parts * rank && rank % 8 == 0 && rank > 0 && K % 8 == 0 && R <= 0x7ffffff && N <= 0x7fffffff &&
+                    (!swiglu || (p.parts == 2 && widths[0] == widths[1] && N % 256 == 0)) && w.size(0) == N && w.size(1) == K && x.dim() == 2 && x.size(1) == K,
+                    "adapter_gemm: stacked adapters do not fit");
+  TORCH_CHECK_VALUE(scales.device() == x.device() && scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 1 && scales.size(0) == L,
+                    "adapter_gemm: one fp32 scale an adapter");
+  TORCH_CHECK_VALUE(ids.device() == x.device() && ids.scalar_type() == at::kInt && ids.is_contiguous() && ids.dim() == 1 && ids.size(0) == T, "adapter_gemm: one id a row");
+  const void* px = lora_operand(x, x, "adapter_gemm: x");
+  for (const at::Tensor& t : {a, b})
+    TORCH_CHECK_VALUE(t.device() == x.device() && t.scalar_type() == at::kBFloat16 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, "adapter_gemm: bf16 adapters");
+  if (bias.has_value())
+    TORCH_CHECK_VALUE(bias->device() == x.device() && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() && bias->numel() == N, "adapter_gemm: bf16 bias [N]");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor t = at::empty({T, R + pad}, x.options()), pb = at::empty({N, R + pad}, x.options());
+  p.interleaved = swiglu; p.N = N; p.ldb = R + pad;
+  check(prl_adapter_pack(b.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, pb.data_ptr(), &p, L, rank, cur_stream()), "adapter_pack");
+  check(prl_adapter_thin(px, a.data_ptr(), t.data_ptr(), T, R, K, x.stride(0), K, R + pad, pad, ids.data_ptr<int32_t>(), scales.data_ptr<float>(), each, cur_stream()),
+        "adapter_thin");
+  return swiglu ? lora_gemm_swiglu(x, w, t, pb, false)[0] : lora_gemm(x, w, t, pb, false, residual);
+}
+
 // Row-parallel TP linear with the all-reduce fused into the GEMM epilogue over NVLink peer memory.
 at::Tensor skinny_gemm_tp(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& residual,
                           at::Tensor workspace, at::Tensor counters, int64_t splits, const std::vector<int64_t>& inbox_ptrs,
@@ -858,6 +891,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("skinny_gemm_tp", &skinny_gemm_tp);
   m.def("lora_fwd", &lora_fwd);
   m.def("lora_bwd", &lora_bwd);
+  m.def("adapter_gemm", &adapter_gemm);
   m.def("lora_thin", &lora_thin, py::arg("a"), py::arg("b"), py::arg("layout"), py::arg("scale") = 1.0, py::arg("rank") = 0, py::arg("pad") = 0,
         py::arg("halves") = false, py::arg("lo") = 0, py::arg("split") = 0);
   m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("b"), py::arg("b_mn") = false, py::arg("residual") = py::none());

@@ -39,9 +39,14 @@ struct ThinParams {
   int pad;                                           // columns after the last one: the first is 1, the rest 0 (row-major output)
   int lo_out;                                        // > 0: column of the outputs' second halves (row-major output)
   int lo_in;                                         // > 0: the same of B (MN-major)
+  // rows of a batch with adapters of their own (row-major output): `each` columns belong to an adapter; a row keeps those of ids[row], times
+  // scales[ids[row]], and zeros elsewhere
+  const int32_t* ids;
+  const float* scales;
+  int each;
 };
 
-// grid (tiles * S, blocks of NR columns); A_MN / B_MN: the reduction runs over the operand's rows in memory; TRANS: out is [R, M]
+// grid (S, blocks of NR columns, tiles), so that the blocks that read the same rows of A run together; A_MN / B_MN: the reduction runs over the operand's rows in memory; TRANS: out is [R, M]
 template <bool A_MN, bool B_MN, bool TRANS>
 __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const ThinParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -54,7 +59,7 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
   uint32_t S;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
   const uint32_t rank = cluster_ctarank();
-  const int m0 = blockIdx.x / S * kBlockM, r0 = blockIdx.y * p.NR;
+  const int m0 = blockIdx.z * kBlockM, r0 = blockIdx.y * p.NR;
   const int num_kb = (p.K + 63) / 64, kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
   const uint32_t tmem_cols = cols_acc <= 32 ? 32 : cols_acc <= 64 ? 64 : cols_acc <= 128 ? 128 : 256;
 
@@ -181,7 +186,15 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
     for (int e = threadIdx.x; e < (rows1 - rows0) * quads; e += kThinThreads) {
       const int row = rows0 + e / quads, c = e % quads * 4;
       if (m0 + row >= p.M) break;
-      const float4 v = c < cols ? sum(row, c) : make_float4(c == cols ? 1.f : 0.f, 0.f, 0.f, 0.f);
+      float4 v = c < cols ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(c == cols ? 1.f : 0.f, 0.f, 0.f, 0.f);
+      const int owner = p.ids && c < cols ? (r0 + c) / p.each : -1;
+      if (c < cols && (!p.ids || p.ids[m0 + row] == owner)) {
+        v = sum(row, c);
+        if (p.ids) {
+          const float s = p.scales[owner];
+          v.x *= s; v.y *= s; v.z *= s; v.w *= s;
+        }
+      }
       const uint2 hi = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
       __nv_bfloat16* o = p.out + static_cast<int64_t>(m0 + row) * p.ldo + r0 + c;
       *reinterpret_cast<uint2*>(o) = hi;
@@ -230,11 +243,11 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
     while (S < 4 && whole * S < 148 && num_kb >= 2 * S) S *= 2;
     if (S == 4 && whole * S < 74 && num_kb >= 32) S = 8;
   }
-  if (S > 8 || S > num_kb || (S & (S - 1))) return -4;
+  if (S > 8 || S > num_kb || (S & (S - 1)) || tiles > 65535 || blocks > 65535) return -4;
   auto kern = thin_kernel<A_MN, B_MN, TRANS>;
   PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kThinSmemMax));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles * S, blocks);
+  cfg.gridDim = dim3(S, blocks, tiles);
   cfg.blockDim = dim3(kThinThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -298,7 +311,7 @@ extern "C" int prl_lora_thin(const void* A, const void* B, void* out, int M, int
                              int lo_out, int lo_in, int split, cudaStream_t stream) {
   if (M <= 0 || R <= 0 || K <= 0) return 0;
   if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || lo_out % 8 || lo_in % 8 || (layout != 3 && ldo % 4) || (layout == 3 && lo_out) || (layout == 0 && lo_in)) return -1;
-  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad, lo_out, lo_in};
+  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad, lo_out, lo_in, nullptr, nullptr, 1};
   switch (layout) {
     case 0: return run_thin<false, false, false>(A, B, p, lda, ldb, split, stream);
     case 1: return run_thin<false, true, false>(A, B, p, lda, ldb, split, stream);
@@ -306,6 +319,45 @@ extern "C" int prl_lora_thin(const void* A, const void* B, void* out, int M, int
     case 3: return run_thin<true, true, true>(A, B, p, lda, ldb, split, stream);
   }
   return -5;
+}
+
+// layout 0 for rows whose adapters differ: B [adapters * each, K], out [M, adapters * each (+ pad)], see ThinParams
+extern "C" int prl_adapter_thin(const void* A, const void* B, void* out, int M, int R, int K, int64_t lda, int64_t ldb, int64_t ldo, int pad, const int32_t* ids,
+                                const float* scales, int each, cudaStream_t stream) {
+  if (M <= 0 || R <= 0 || K <= 0) return 0;
+  if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || ldo % 4 || each < 4 || each % 4 || R % each) return -1;
+  return run_thin<false, false, false>(A, B, ThinParams{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, 1.f, pad, 0, 0, ids, scales, each}, lda, ldb, 0, stream);
+}
+
+namespace prl {
+// b [adapters, N, rank] -> [N, adapters * parts * rank (+ 8)]: row n holds every adapter's row n in the columns of its part, a bias behind them
+__global__ void __launch_bounds__(256) adapter_pack_kernel(const __nv_bfloat16* __restrict__ b, const __nv_bfloat16* __restrict__ bias, int4* __restrict__ out,
+                                                           const LoraPackParams p, int adapters, int rank) {
+  grid_behind();
+  const int units = p.ldb / 8, each = p.parts * rank;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < static_cast<int64_t>(p.N) * units; e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int n = static_cast<int>(e / units), c = static_cast<int>(e % units) * 8;
+    union { int4 v; __nv_bfloat16 h[8]; } o;
+    o.v = make_int4(0, 0, 0, 0);
+    if (c < adapters * each) {
+      const int part = p.interleaved ? (n >> 7) & 1 : (p.parts > 1 && n >= p.ends[0]) + (p.parts > 2 && n >= p.ends[1]);
+      const int l = c / each, k = c % each - part * rank;
+      if (k >= 0 && k < rank) o.v = __ldg(reinterpret_cast<const int4*>(b + (static_cast<int64_t>(l) * p.N + n) * rank + k));
+    } else if (bias) {
+      o.h[0] = bias[n];
+    }
+    out[e] = o.v;
+  }
+}
+}  // namespace prl
+
+extern "C" int prl_adapter_pack(const void* b, const void* bias, void* out, const prl::LoraPackParams* q, int adapters, int rank, cudaStream_t stream) {
+  if (q->N <= 0 || adapters <= 0 || rank % 8 || q->ldb % 8) return -1;
+  const int64_t blocks = (static_cast<int64_t>(q->N) * (q->ldb / 8) + 255) / 256;
+  PRL_CUDA_CHECK(launch_behind(adapter_pack_kernel, static_cast<unsigned>(blocks < 16 * 148 ? blocks : 16 * 148), 256, 0, stream, static_cast<const __nv_bfloat16*>(b),
+                               static_cast<const __nv_bfloat16*>(bias), static_cast<int4*>(out), *q, adapters, rank));
+  PRL_CUDA_CHECK(cudaGetLastError());
+  return 0;
 }
 
 extern "C" int prl_lora_pack(const prl::LoraPackParams* q, cudaStream_t stream) {

@@ -307,6 +307,8 @@ class AdapterBank:
             want = (rank, self.dims[p][1]) if m == "A" else (self.dims[p][0], rank)
             if tuple(t.shape) != want or n[:-1] + "AB"[m == "A"] not in sd:
                 raise ValueError(f"adapter {name!r}: {n} is {tuple(t.shape)}, {want} and its partner expected")
+            if not torch.isfinite(t).all():
+                raise ValueError(f"adapter {name!r}: {n} is not finite")
         at = free[0]
         self._write(at, sd, rank)
         self.scales[at] = (rank if alpha is None else float(alpha)) / (rank ** 0.5 if root else rank)

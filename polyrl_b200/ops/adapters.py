@@ -85,6 +85,16 @@ def _delta(x, a, b, scales, plan, widths, interleaved, bias=None, residual=None,
                               None if bias is None else fn._aligned(bias), None if residual is None else _rows(residual), onto)
 
 
+def _together(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Many rows: whether the adapters' part goes through the large product as further k-blocks, the low-rank values of all adapters side by
+    side with a row's own kept (lora.cu).  That is LR (K + N) products a row for LR = adapters * parts * rank, whichever adapters the rows have;
+    a pass of its own is bound by the array of N values a row that it leaves.  The line is where both took as long, at about 1300 LR values' worth
+    of products for one of the array's.  Apart and together, rows, K, N, LR, us: 5003, 2048, 2048, 320: 85 and 66; 2900, 3584, 37888, 640: 892 and
+    732, with 1024 897 and 800; 3000, 896, 9728, 512: 178 and 106; 8000, 4096, 6144, 384: 396 and 381, with 1536 468 and 555; 4000, 14336, 4096, 512:
+    424 and 485."""
+    return a.shape[0] * a.shape[1] * (a.shape[2] + b.shape[1]) <= 1300 * b.shape[1]
+
+
 def _delta_reference(x, a, b, scales, ids, widths, interleaved):
     out = torch.zeros(x.shape[0], b.shape[1], dtype=torch.float32, device=x.device)
     n, r = b.shape[1], b.shape[2]
@@ -109,7 +119,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     ``widths``: the columns of a fused projection's parts (query, key, value), each with ``rank`` rows of ``a`` [adapters, parts * rank, K] and
     its rows of ``b`` [adapters, N, rank]; an adapter that leaves a part alone has zeros there.  Ranks are multiples of 16 (smaller ones are
     padded with zeros).  Up to 256 rows the adapters add to what ``linear`` gives, so that a row without one is ``linear``'s bit for bit (without
-    a residual).  Inference only."""
+    a residual).  With more rows ``b`` must be finite: rows of other adapters may be multiplied by it and zero.  Inference only."""
     widths = (w.shape[0],) if widths is None else tuple(widths)
     if not fn._is_kernel_tensor(x) or plan.buf is None:          # (the kernel's binding checks as much)
         _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
@@ -117,8 +127,12 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
     if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
         return _delta(x, a, b, scales, plan, widths, False, None, residual, fn.linear(x, w, bias).contiguous())
+    w = fn._g2_operand(w.to(x.dtype))
+    if _together(a, b):
+        return _C().adapter_gemm(_rows(x), w, a, b, scales, plan.ids, widths, False, bias if bias is None else fn._aligned(bias),
+                                 residual if residual is None else fn._aligned(residual))
     d = _delta(x, a, b, scales, plan, widths, False, bias, residual)
-    return _C().gemm_bf16(_rows(x), fn._g2_operand(w.to(x.dtype)), d)
+    return _C().gemm_bf16(_rows(x), w, d)
 
 
 @torch.no_grad()
@@ -132,6 +146,8 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
         _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
         gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
         return ref.swiglu(gu).to(x.dtype)
+    if x.shape[0] > 256 and not isinstance(wgu, fn.Fp8Weight) and not fn._cublas() and wgu.dtype == x.dtype and _together(a, b):
+        return _C().adapter_gemm(_rows(x), fn._g2_operand(wgu), a, b, scales, plan.ids, (n // 2, n // 2), True, None, None)
     d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True), _rows(x)
     if isinstance(wgu, fn.Fp8Weight):
         xq, xs = fn.quantize_fp8_rowwise(x)

@@ -203,6 +203,7 @@ def test_adapters_refused(tmp_path):
                       ("partner", lambda: eng.load_adapter("b", {k: v for k, v in sd.items() if not k.endswith("layers.1.lora.lora_o_proj_B")})),
                       ("no module", lambda: eng.load_adapter("b", {k.replace("layers.1", "layers.7"): v for k, v in sd.items()})),
                       ("belong to no module", lambda: eng.load_adapter("b", {**export_peft_state_dict(sd), "lm_head.lora_A.weight": torch.zeros(8, 256)})),
+                      ("not finite", lambda: eng.load_adapter("b", {k: torch.full_like(v, float("inf")) if k.endswith("1.lora.lora_o_proj_B") else v for k, v in sd.items()})),
                       ("no adapter", lambda: eng.unload_adapter("b"))]:
         with pytest.raises(ValueError, match=match):
             fn()

@@ -152,6 +152,36 @@ def test_adapters(t, k, widths, rank, num):
     check_near(run_adapters(c, widths, num), *near64(c, widths))
 
 
+@pytest.mark.parametrize("t,k,widths,rank,num,together", [
+    (257, 64, (64,), 16, 2, True), (300, 896, (896, 128, 128), 16, 8, True), (515, 2048, (1024,), 64, 9, False), (1300, 256, (512, 64, 64), 32, 20, False),
+    (2049, 512, (1536,), 128, 3, True)])
+def test_adapters_many_rows_both_ways(t, k, widths, rank, num, together, monkeypatch):
+    """Through the large product, or in a pass of its own: the rule's choice and the other one, each within its bound."""
+    c = adapters_case(t, k, widths, rank, num, t, torch.bfloat16, "cuda")
+    assert ops.adapters._together(c["a"], c["b"]) == together
+    ref = adapters64(**c, widths=widths)
+    for way in (True, False):
+        monkeypatch.setattr(ops.adapters, "_together", lambda a, b, way=way: way)
+        for d in (c, dict(c, residual=None), dict(c, bias=None)):
+            check_near(run_adapters(d, widths, num), *(ref if d is c else adapters64(**d, widths=widths)))
+    c = adapters_case(t, k, (256, 256), rank, num, t, torch.bfloat16, "cuda", extra=False)
+    for way in (True, False):
+        monkeypatch.setattr(ops.adapters, "_together", lambda a, b, way=way: way)
+        y = ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], num))
+        check_near(y, *swiglu64(*adapters64(**c, widths=(256, 256), interleaved=True)))
+
+
+def test_many_rows_that_are_not_finite_stay_alone(monkeypatch):
+    c = adapters_case(400, 256, (256, 64, 64), 16, 4, 0, torch.bfloat16, "cuda")
+    bad = c["x"].clone()
+    bad[13], bad[340] = float("nan"), float("inf")
+    rest = torch.ones(400, dtype=torch.bool, device="cuda")
+    rest[[13, 340]] = False
+    for way in (True, False):
+        monkeypatch.setattr(ops.adapters, "_together", lambda a, b, way=way: way)
+        assert torch.equal(run_adapters(dict(c, x=bad), (256, 64, 64), 4)[rest], run_adapters(c, (256, 64, 64), 4)[rest])
+
+
 @pytest.mark.parametrize("value", [-1, 0, 2, 2 ** 31 - 1])
 @pytest.mark.parametrize("t", [3, 80, 333])
 def test_adapters_all_rows_alike(value, t):

@@ -89,13 +89,17 @@ __device__ __forceinline__ void copy_part(const T* z, T* out, int size, const ui
       if constexpr (!INPLACE) x[j] = ld_nc_v4(z + v);
       bits[j] = mask ? __funnelshift_r(__ldg(mask + (v >> 5)), __ldg(mask + ((v + VEC - 1) >> 5)), v & 31) & kAll : kAll;
     }
+    if constexpr (INPLACE) {                           // what is neither kept nor banned as a whole
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) {
+        const int v = v0 + j * threads * VEC;
+        if (v < tail && bits[j] != kAll && bits[j] != 0) x[j] = ld_v4(z + v);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       const int v = v0 + j * threads * VEC;
       if (v >= tail || (INPLACE && bits[j] == kAll)) continue;
-      if constexpr (INPLACE) {
-        if (bits[j] != 0) x[j] = ld_v4(z + v);
-      }
       if (bits[j] != kAll) {
         int* w = reinterpret_cast<int*>(&x[j]);
 #pragma unroll

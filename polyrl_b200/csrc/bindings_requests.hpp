@@ -151,4 +151,12 @@ at::Tensor adapter_delta(const at::Tensor& x, const at::Tensor& a, const at::Ten
   return out;
 }
 
+// x w^T (+ bias) by the library, as a decode step's plain products, and what the adapters add to it
+at::Tensor adapter_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scales, const at::Tensor& plan,
+                          int64_t tile_rows, int64_t max_tiles, const std::vector<int64_t>& widths, const OptTensor& bias, const OptTensor& residual) {
+  TORCH_CHECK_VALUE(w.dim() == 2 && x.dim() == 2 && w.size(1) == x.size(1) && b.dim() == 3 && w.size(0) == b.size(1), "adapter_linear: the projection does not fit");
+  c10::cuda::CUDAGuard g(x.device());
+  return adapter_delta(x, a, b, scales, plan, tile_rows, max_tiles, widths, false, c10::nullopt, residual, at::linear(x, w, bias), 0, 0);
+}
+
 }  // namespace

@@ -1055,6 +1055,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("inverse") = true);
   m.def("adjust_logits", &adjust_logits);
   m.def("gemm_swiglu_add", &gemm_swiglu_add);
+  m.def("adapter_linear", &adapter_linear);
   m.def("adapter_plan", &adapter_plan);
   m.def("adapter_delta", &adapter_delta, py::arg("x"), py::arg("a"), py::arg("b"), py::arg("scales"), py::arg("plan"), py::arg("tile_rows"), py::arg("max_tiles"),
         py::arg("widths"), py::arg("interleaved"), py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("onto") = py::none(),

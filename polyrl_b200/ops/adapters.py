@@ -125,6 +125,8 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
         y = fn.linear(x, w, bias, residual)
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
+    if fn._is_decode_shape(x, w) and fn._plain_decode(x, w):
+        return _C().adapter_linear(_rows(x), w, a, b, scales, plan.buf, plan.tile_rows, plan.max_tiles, widths, bias, None if residual is None else _rows(residual))
     if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
         return _delta(x, a, b, scales, plan, widths, False, None, residual, fn.linear(x, w, bias).contiguous())
     w = fn._g2_operand(w.to(x.dtype))

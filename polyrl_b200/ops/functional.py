@@ -234,6 +234,11 @@ class _LinearFn(torch.autograd.Function):
         return dx, dw, dres
 
 
+def _plain_decode(x: torch.Tensor, w) -> bool:
+    """Rows whose product, when their number is a decode step's, is the library's."""
+    return _is_kernel_tensor(x) and w.dtype == torch.bfloat16 and x.dim() == 2 and _decode_policy() in ("auto", "cublas")
+
+
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
            residual: torch.Tensor | None = None) -> torch.Tensor:
     """y = x @ w.T (+ bias) (+ residual).  w is [out, in] (nn.Linear layout)."""
@@ -241,8 +246,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
         return _linear_fp8(x, w, bias, residual)
     if _is_kernel_tensor(x) and w.dtype == torch.bfloat16 and x.dim() == 2 and _use_skinny(x, w):
         return skinny_linear(x, w, bias, residual, 0)
-    if _is_kernel_tensor(x) and w.dtype == torch.bfloat16 and x.dim() == 2 and _decode_policy() in ("auto", "cublas") \
-            and _is_decode_shape(x, w):
+    if _plain_decode(x, w) and _is_decode_shape(x, w):
         y = torch.nn.functional.linear(x, w, bias)
         return y.add_(residual) if residual is not None else y
     if _is_kernel_tensor(x) and w.dtype == torch.bfloat16 and w.shape[0] % 8 == 0 and w.shape[1] % 8 == 0:

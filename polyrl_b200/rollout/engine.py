@@ -1139,8 +1139,8 @@ class RolloutEngine:
     def _run_decode(self, bs: int, sample: bool = True) -> torch.Tensor:
         """One decode step, through its CUDA graph where there is one; returns the step's logits (overwritten by the next step)."""
         # what some request of the batch brings is part of the step, and of the graph; a batch without is the step without
-        self._with_rules = sample and any(r.params.has_rules for r in self.running.values())
-        self._with_adapters = sample and any(r.adapter >= 0 for r in self.running.values())
+        self._with_rules = sample and any(r.params.has_rules and r.decoding for r in self.running.values())
+        self._with_adapters = sample and any(r.adapter >= 0 and r.decoding for r in self.running.values())
         if not self.use_cuda_graph or (sample and (self._top_k > 0 or self._top_p < 1.0)):
             # top-k / top-p go through the sort-based library sampler (host-seeded RNG): not captured into a graph
             return self._decode_body(bs, sample)

@@ -120,6 +120,19 @@ def test_rules_of_samples_of_one_prompt_and_of_moved_slots():
     check_ruled(cfg, w, reqs, eng, 1e-3)
 
 
+def test_rules_of_a_request_whose_prompt_is_not_in_yet():
+    cfg, w, eng = make_engine(max_prefill_tokens=16)
+    prompt, late = [5, 6, 7], list(range(9, 90))
+    first = eng.add_request(prompt, SamplingParams(max_new_tokens=30, temperature=0.0))
+    while not first.output_ids:
+        eng.step()
+    second = eng.add_request(late, SamplingParams(max_new_tokens=12, temperature=0.0, presence_penalty=2.0, frequency_penalty=0.5))
+    while eng.has_work():
+        eng.step()
+    check_ruled(cfg, w, [first, second], eng, 1e-3)
+    assert len(second.output_ids) > 1
+
+
 def test_rules_refused():
     cfg, w, eng = make_engine()
     for kw in [dict(repetition_penalty=0.0), dict(repetition_penalty=float("nan")), dict(presence_penalty=float("inf")), dict(min_new_tokens=-1),

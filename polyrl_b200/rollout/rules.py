@@ -92,8 +92,9 @@ class RequestRules:
         """A slot whose request has no rules."""
         self.repetition[slot], self.presence[slot], self.frequency[slot] = 1.0, 0.0, 0.0
         self.lens[slot], self.min_lens[slot], self.mask_rows[slot] = 0, 0, -1
-        if self.bias_ids is not None:
-            self.bias_ids[slot] = -1
+        for t in (self.bias_ids, self.stop_ids):
+            if t is not None:
+                t[slot] = -1
 
     def move(self, src: int, dst: int) -> None:
         for t in (self.tokens, self.lens, self.prompt_lens, self.repetition, self.presence, self.frequency, self.min_lens, self.bias_ids, self.bias_values,

@@ -133,6 +133,15 @@ def test_rules_of_a_request_whose_prompt_is_not_in_yet():
     assert len(second.output_ids) > 1
 
 
+def test_stop_tokens_of_a_slots_last_request_are_forgotten():
+    cfg, w, eng = make_engine(max_num_seqs=1)
+    many = tuple(range(40, 52))
+    eng.generate([[5, 6]], SamplingParams(max_new_tokens=4, temperature=0.0, min_new_tokens=3, stop_token_ids=many))
+    r = eng.generate([[5, 6]], SamplingParams(max_new_tokens=6, temperature=0.0, min_new_tokens=5, logit_bias={45: 1e4}))[0][0]
+    assert r.output_ids == [45] * 6
+    check_ruled(cfg, w, [r], eng, 1e-3)
+
+
 def test_rules_refused():
     cfg, w, eng = make_engine()
     for kw in [dict(repetition_penalty=0.0), dict(repetition_penalty=float("nan")), dict(presence_penalty=float("inf")), dict(min_new_tokens=-1),

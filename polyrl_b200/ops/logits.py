@@ -21,7 +21,8 @@ class LogitRules:
     The repetition penalty falls on tokens of the whole history, presence and frequency on output tokens.  Ids outside the vocabulary
     (padding) count for nothing, in ``tokens``, ``bias_ids`` and ``stop_ids``; of bias entries with the same id the last one counts.
     ``masks`` hold a bit a token, 32 to a word, lowest bit first; ``mask_rows`` says which mask a row has (negative: none; absent: row b has
-    mask b).  Stop tokens may not come while ``lens[b] < min_lens[b]``.  Where nothing is allowed the row is -inf throughout."""
+    mask b).  Stop tokens may not come while ``lens[b] < min_lens[b]``.  Where nothing is allowed the row is -inf throughout,
+    and there is no token in it that ``sample_tokens`` could choose."""
 
     tokens: torch.Tensor | None = None         # [B, n] int32, n < 2^20
     lens: torch.Tensor | None = None           # [B] int32

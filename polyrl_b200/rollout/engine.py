@@ -577,7 +577,7 @@ class RolloutEngine:
         if params.has_rules:
             from .rules import check_params
 
-            check_params(params, self.cfg.vocab_size, self._stop_ids(params))
+            check_params(params, self.cfg.vocab_size, self._stop_ids(params), self.max_model_len)
         if adapter is not None:
             if self.adapters is None:
                 raise ValueError("this engine serves no adapters (max_adapters)")

@@ -5,35 +5,38 @@ sampled token joins its row's history) is captured once.  Reference capability: 
 reference's rollout workers (rlboost/verl_stream/workers/rollout/sglang_rollout/sglang_rollout_remote.py:103-182)."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import ops
-from ..ops.logits import MAX_BIAS, LogitRules
+from ..ops.logits import MAX_BIAS, MAX_HISTORY, LogitRules
 
 OVERSHOOT = 8            # tokens that a sequence may ride along after it has ended (engine: steps_per_sync)
+LARGEST = 1e20           # of a penalty or a bias: a logit stays finite with all of them, 2^20 times the frequency penalty and a small temperature
 
 
-def check_params(p, vocab: int, stop_ids) -> None:
-    """Refuse what the rules cannot mean.  ``stop_ids``: the tokens that end the request."""
-    import math
-
-    if not (math.isfinite(p.repetition_penalty) and p.repetition_penalty > 0):
+def check_params(p, vocab: int, stop_ids, max_len: int) -> None:
+    """Refuse what the rules cannot mean, and what could leave a step without a token to sample.  ``stop_ids``: the tokens that end the request;
+    ``max_len``: of the engine's sequences."""
+    if max_len + OVERSHOOT >= MAX_HISTORY:
+        raise ValueError(f"rules on logits need a history of less than {MAX_HISTORY} tokens")
+    if not 1 / LARGEST <= p.repetition_penalty <= LARGEST:
         raise ValueError(f"repetition_penalty must be positive, not {p.repetition_penalty}")
-    if not (math.isfinite(p.presence_penalty) and math.isfinite(p.frequency_penalty)):
-        raise ValueError("presence_penalty and frequency_penalty must be finite")
+    if not (abs(p.presence_penalty) <= LARGEST and abs(p.frequency_penalty) <= LARGEST):
+        raise ValueError(f"presence_penalty and frequency_penalty must be finite, up to {LARGEST:g}")
     if p.min_new_tokens < 0:
         raise ValueError("min_new_tokens must not be negative")
     if p.logit_bias:
         if len(p.logit_bias) > MAX_BIAS:
             raise ValueError(f"logit_bias: at most {MAX_BIAS} tokens")
-        if any(not 0 <= int(t) < vocab for t in p.logit_bias) or any(math.isnan(float(v)) or float(v) == math.inf for v in p.logit_bias.values()):
-            raise ValueError(f"logit_bias: tokens below {vocab} and numbers (-inf bans a token)")
-    if p.allowed_token_ids is not None:
-        if not p.allowed_token_ids or any(not 0 <= int(t) < vocab for t in p.allowed_token_ids):
-            raise ValueError(f"allowed_token_ids: at least one token, all below {vocab}")
-        banned = {int(t) for t, v in (p.logit_bias or {}).items() if float(v) == -math.inf} | (set(stop_ids) if p.min_new_tokens > 0 else set())
-        if set(map(int, p.allowed_token_ids)) <= banned:
-            raise ValueError("allowed_token_ids: nothing is left before min_new_tokens")
+        if any(not 0 <= int(t) < vocab for t in p.logit_bias) or not all(abs(float(v)) <= LARGEST or float(v) == -math.inf for v in p.logit_bias.values()):
+            raise ValueError(f"logit_bias: tokens below {vocab} and numbers up to {LARGEST:g} (-inf bans a token)")
+    if p.allowed_token_ids is not None and (not p.allowed_token_ids or any(not 0 <= int(t) < vocab for t in p.allowed_token_ids)):
+        raise ValueError(f"allowed_token_ids: at least one token, all below {vocab}")
+    banned = {int(t) for t, v in (p.logit_bias or {}).items() if float(v) == -math.inf} | (set(stop_ids) if p.min_new_tokens > 0 else set())
+    if set(range(vocab) if p.allowed_token_ids is None and len(banned) >= vocab else map(int, p.allowed_token_ids or (-1,))) <= banned:
+        raise ValueError("allowed_token_ids, logit_bias and min_new_tokens leave no token to sample")
 
 
 class RequestRules:
@@ -80,7 +83,7 @@ class RequestRules:
         if p.min_new_tokens > 0 and stops:
             self.stop_ids = self._wide(self.stop_ids, len(stops), -1)
             self.stop_ids[slot, :len(stops)] = torch.tensor(stops, dtype=torch.int32).to(self.device)
-            self.min_lens[slot] = prompt_len + p.min_new_tokens
+            self.min_lens[slot] = prompt_len + min(p.min_new_tokens, p.max_new_tokens)
         if p.allowed_token_ids is not None:
             if self.masks is None:
                 self.masks = torch.zeros(self.slots, (self.vocab + 31) // 32, dtype=torch.int32, device=self.device)

@@ -154,6 +154,24 @@ def test_rules_refused():
     assert not eng.has_work()
 
 
+def test_no_rules_leave_nothing_to_sample():
+    """Numbers that could take every allowed logit to -inf, and lists that ban every token, are refused; what is let in keeps a finite one."""
+    cfg, w, eng = make_engine()
+    ban = {t: -float("inf") for t in range(512)}
+    for kw in [dict(repetition_penalty=1e-30), dict(repetition_penalty=1e30), dict(presence_penalty=1e30), dict(frequency_penalty=-1e30), dict(logit_bias={3: -1e30}),
+               dict(logit_bias=ban), dict(logit_bias={t: v for t, v in ban.items() if t != 1}, min_new_tokens=1)]:
+        with pytest.raises(ValueError):
+            eng.add_request([5], SamplingParams(**kw))
+    reqs = [eng.add_request([5, 6], SamplingParams(max_new_tokens=8, temperature=t, **kw)) for t in (0.0, 1.0, 1e-6)
+            for kw in [dict(allowed_token_ids=(5,), frequency_penalty=1e20, presence_penalty=1e20, repetition_penalty=1e20), dict(allowed_token_ids=(5,), logit_bias={5: -1e20})]]
+    late = eng.add_request([5, 6], SamplingParams(max_new_tokens=8, min_new_tokens=2 ** 40, logit_bias={1: 1e4}))
+    while eng.has_work():
+        eng.step()
+    assert all(r.output_ids == [5] * 8 for r in reqs) and len(late.output_ids) == 8 and 1 not in late.output_ids
+    with pytest.raises(ValueError, match="history"):
+        RolloutEngine.check_request(type("E", (), dict(cfg=cfg, max_model_len=1 << 20, _stop_ids=lambda self, p: set()))(), SamplingParams(presence_penalty=1.0))
+
+
 def check_adapted(cfg, reqs, weights, slack):
     """Greedy tokens of every request are those of its adapter's merged model, up to near-ties."""
     for r, m in zip(reqs, weights):

@@ -72,6 +72,12 @@ def _check_adapters(name: str, x, w, a, b, scales, plan: AdapterPlan, widths, bi
         raise ValueError(f"{name}: bias [N], residual [T, N]")
 
 
+def _of_plan(name: str, a: torch.Tensor, plan: AdapterPlan) -> None:
+    """The plan holds places in the stacks: of other stacks it could point behind these."""
+    if a.shape[0] != plan.num_adapters:
+        raise ValueError(f"{name}: a plan for {plan.num_adapters} adapters, the stacks hold {a.shape[0]}")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows as the kernels read them: unit inner stride, pitch and base on 16 bytes."""
     if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
@@ -121,10 +127,11 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     padded with zeros).  Up to 256 rows the adapters add to what ``linear`` gives, so that a row without one is ``linear``'s bit for bit (without
     a residual).  With more rows ``b`` must be finite: rows of other adapters may be multiplied by it and zero.  Inference only."""
     widths = (w.shape[0],) if widths is None else tuple(widths)
-    if not fn._is_kernel_tensor(x) or plan.buf is None:          # (the kernel's binding checks as much)
+    if not fn._is_kernel_tensor(x) or plan.buf is None:          # (the kernels' bindings check as much, but for what the plan was made for)
         _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
         y = fn.linear(x, w, bias, residual)
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
+    _of_plan("adapter_linear", a, plan)
     if fn._is_decode_shape(x, w) and fn._plain_decode(x, w):
         return _C().adapter_linear(_rows(x), w, a, b, scales, plan.buf, plan.tile_rows, plan.max_tiles, widths, bias, None if residual is None else _rows(residual))
     if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
@@ -148,6 +155,7 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
         _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
         gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
         return ref.swiglu(gu).to(x.dtype)
+    _of_plan("adapter_linear_swiglu", a, plan)
     if x.shape[0] > 256 and not isinstance(wgu, fn.Fp8Weight) and not fn._cublas() and wgu.dtype == x.dtype and _together(a, b):
         return _C().adapter_gemm(_rows(x), fn._g2_operand(wgu), a, b, scales, plan.ids, (n // 2, n // 2), True, None, None)
     d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True), _rows(x)

@@ -294,3 +294,14 @@ def test_adapters_refused_by_the_kernel_entry():
         ops.adapter_linear(c["x"], c["w"], c["a"], c["b"].transpose(1, 2).contiguous().transpose(1, 2), c["scales"], plan)
     with pytest.raises(ValueError, match="plan is of"):
         ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"].cpu(), 2))
+
+
+@pytest.mark.parametrize("t", [1, 4, 300])
+def test_adapters_refuse_the_plan_of_other_stacks(t):
+    c = adapters_case(t, 64, (128, 128), 16, 2, 0, torch.bfloat16, "cuda")
+    for num in (1, 3, 24):
+        plan = ops.adapter_plan(c["ids"], num)
+        with pytest.raises(ValueError, match="a plan for"):
+            ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], plan, (128, 128))
+        with pytest.raises(ValueError, match="a plan for"):
+            ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], plan)

@@ -13,7 +13,7 @@ int prl_gemm2_bf16(const void*, const void*, void*, const void*, int, int, int, 
 int64_t prl_gemm2_ws_floats(int, int, int);
 int64_t prl_gemm2_tail_ws_floats(int, int, int, int);
 int prl_gemm2_tail_bf16(const void*, const void*, const void*, const void*, void*, const void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int, float*, cudaStream_t);
-int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
+int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
 int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, int, int, cudaStream_t);
 int prl_lora_pack(const prl::LoraPackParams*, cudaStream_t);
 int prl_adapter_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, int, const int32_t*, const float*, int, cudaStream_t);
@@ -31,7 +31,7 @@ int prl_rmsnorm_bwd(const void*, const void*, const void*, const float*, const v
 int prl_rmsnorm_bwd_parts(int, int);
 int prl_rope(void*, const int64_t*, const float*, const float*, int, int, int, int, int64_t, float, void*, void*, const int64_t*, int, cudaStream_t);
 int prl_gather_pages(const void*, const void*, const int64_t*, const int64_t*, void*, void*, int, int64_t, int, int, int, cudaStream_t);
-int prl_swiglu_bwd(const void*, const void*, void*, int64_t, int, cudaStream_t);
+int prl_swiglu_bwd(const void*, const void*, const void*, void*, int64_t, int, cudaStream_t);
 int prl_quant_fp8_rowwise(const void*, void*, float*, int, int, cudaStream_t);
 int prl_grad_accum(float*, const void*, int, float, int64_t, float*, cudaStream_t);
 int prl_sumsq(const float*, int64_t, float*, cudaStream_t);
@@ -364,14 +364,16 @@ std::vector<at::Tensor> gather_pages(const at::Tensor& k_cache, const at::Tensor
   return {k, v};
 }
 
-at::Tensor swiglu_bwd(const at::Tensor& gu, const at::Tensor& dh) {
+// low: the eight bits behind gu's sixteen, where the projection was saved in 24
+at::Tensor swiglu_bwd(const at::Tensor& gu, const at::Tensor& dh, const c10::optional<at::Tensor>& low) {
   CHECK_BF16(gu); CHECK_BF16(dh);
   TORCH_CHECK(gu.is_contiguous() && dh.is_contiguous());
+  TORCH_CHECK(!low.has_value() || (low->device() == gu.device() && low->scalar_type() == at::kByte && low->is_contiguous() && low->numel() == gu.numel()), "swiglu_bwd: low");
   const int F = dh.size(-1);
   const int64_t T = dh.numel() / F;
   c10::cuda::CUDAGuard g(gu.device());
   at::Tensor dgu = at::empty_like(gu);
-  check(prl_swiglu_bwd(gu.data_ptr(), dh.data_ptr(), dgu.data_ptr(), T, F, cur_stream()), "swiglu_bwd");
+  check(prl_swiglu_bwd(gu.data_ptr(), low.has_value() ? low->data_ptr() : nullptr, dh.data_ptr(), dgu.data_ptr(), T, F, cur_stream()), "swiglu_bwd");
   return dgu;
 }
 
@@ -602,7 +604,7 @@ at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
   return d;
 }
 
-// {silu(gate) * up, the projection itself if save} of x w^T + t b^T
+// {silu(gate) * up, if save the projection itself: its upper 16 bits as bf16, the next 8 as bytes} of x w^T + t b^T
 std::vector<at::Tensor> lora_gemm_swiglu(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const at::Tensor& b, bool save) {
   const void *px = lora_operand(x, x, "lora_gemm_swiglu: x"), *pw = lora_operand(w, x, "lora_gemm_swiglu: w"), *pt = lora_operand(t, x, "lora_gemm_swiglu: t"),
              *pb = lora_operand(b, x, "lora_gemm_swiglu: b");
@@ -610,17 +612,22 @@ std::vector<at::Tensor> lora_gemm_swiglu(const at::Tensor& x, const at::Tensor& 
   TORCH_CHECK(w.size(1) == K && t.size(0) == M && b.size(1) == R && b.size(0) == N && N % 256 == 0 && K > 0 && R > 0 && M <= 0x7fffffff && K <= 0x7fffff00,
               "lora_gemm_swiglu: sizes");
   c10::cuda::CUDAGuard g(x.device());
-  at::Tensor h = at::empty({M, N / 2}, x.options()), gu = save ? at::empty({M, N}, x.options()) : at::Tensor();
+  at::Tensor h = at::empty({M, N / 2}, x.options()), gu, low;
+  if (save) {
+    gu = at::empty({M, N}, x.options());
+    low = at::empty({M, N}, x.options().dtype(at::kByte));
+  }
   if (M > 0) {
     const at::Tensor ws = split_scratch(prl_gemm2_tail_ws_floats(M, N, K, R), x);
-    check(prl_gemm_swiglu_tail_bf16(px, pw, pt, pb, h.data_ptr(), save ? gu.data_ptr() : nullptr, M, N, K, R, x.stride(0), w.stride(0), t.stride(0), b.stride(0), N / 2,
+    check(prl_gemm_swiglu_tail_bf16(px, pw, pt, pb, h.data_ptr(), save ? gu.data_ptr() : nullptr, save ? low.data_ptr() : nullptr, M, N, K, R, x.stride(0), w.stride(0),
+                                    t.stride(0), b.stride(0), N / 2,
                                     N, split_ptr(ws), cur_stream()), "lora_gemm_swiglu");
   }
-  if (save) return {h, gu};
+  if (save) return {h, gu, low};
   return {h};
 }
 
-// Forward of lora_linear and lora_linear_swiglu in one call: {y, A and B as the products take them, t, the projection (swiglu and save)}
+// Forward of lora_linear and lora_linear_swiglu in one call: {y, A and B as the products take them, t, the projection in two parts (swiglu and save)}
 std::vector<at::Tensor> lora_fwd(const at::Tensor& x, const at::Tensor& w, const std::vector<OptT>& a, const std::vector<OptT>& b, const std::vector<int64_t>& widths,
                                  double scale, bool swiglu, const OptT& bias, const OptT& residual, bool save) {
   TORCH_CHECK(a.size() == widths.size() && b.size() == widths.size() && !a.empty(), "lora_fwd: parts");
@@ -637,7 +644,7 @@ std::vector<at::Tensor> lora_fwd(const at::Tensor& x, const at::Tensor& w, const
   const at::Tensor t = lora_thin(x, pa, 0, scale, 0, pb.size(1) - pa.size(0), save, 0, 0), t1 = t.narrow(1, 0, pb.size(1));
   if (!swiglu) return {lora_gemm(x, w, t1, pb, false, residual), pa, pb, t};
   std::vector<at::Tensor> y = lora_gemm_swiglu(x, w, t1, pb, save);
-  if (save) return {y[0], pa, pb, t, y[1]};
+  if (save) return {y[0], pa, pb, t, y[1], y[2]};
   return {y[0], pa, pb, t};
 }
 
@@ -911,7 +918,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q_norm"), py::arg("k_norm"), py::arg("eps"), py::arg("out") = py::none(), py::arg("k_cache") = py::none(), py::arg("v_cache") = py::none(),
         py::arg("slot_mapping") = py::none(), py::arg("block_size") = 16);
   m.def("qk_norm_rope_bwd_", &qk_norm_rope_bwd_);
-  m.def("swiglu_bwd", &swiglu_bwd);
+  m.def("swiglu_bwd", &swiglu_bwd, py::arg("gu"), py::arg("dh"), py::arg("low") = py::none());
   m.def("quant_fp8_rowwise", &quant_fp8_rowwise);
   m.def("grad_accum_", &grad_accum_);
   m.def("sumsq_", &sumsq_);

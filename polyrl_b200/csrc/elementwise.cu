@@ -338,7 +338,9 @@ gather_pages_kernel(const __nv_bfloat16* __restrict__ kc, const __nv_bfloat16* _
 
 // SwiGLU backward on the block-interleaved layout ([128 gate | 128 up] per 256 columns):
 // dG = dH * u * sig(g) * (1 + g*(1-sig(g))),  dU = dH * silu(g)
-__global__ void swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const __nv_bfloat16* __restrict__ dh,
+// LOW: gu are the upper sixteen bits of fp32 values, low the eight behind them.
+template <bool LOW>
+__global__ void swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const uint8_t* __restrict__ low, const __nv_bfloat16* __restrict__ dh,
                                   __nv_bfloat16* __restrict__ dgu, int64_t T, int F) {
   const int64_t nvec = T * (F >> 3);
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < nvec;
@@ -352,12 +354,22 @@ __global__ void swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const __
     const uint32_t* gu32 = reinterpret_cast<const uint32_t*>(&gq);
     const uint32_t* uu32 = reinterpret_cast<const uint32_t*>(&uq);
     const uint32_t* du32 = reinterpret_cast<const uint32_t*>(&dq);
+    uint2 gl, ul;
+    if constexpr (LOW) {
+      gl = __ldg(reinterpret_cast<const uint2*>(low + t * 2 * F + gcol));
+      ul = __ldg(reinterpret_cast<const uint2*>(low + t * 2 * F + gcol + 128));
+    }
+    auto pair = [](uint32_t hi, const uint2& lo, int j) {
+      if constexpr (!LOW) return unpack_bf16(hi);
+      const uint32_t l = (j & 2 ? lo.y : lo.x) >> (16 * (j & 1));
+      return make_float2(__uint_as_float(__byte_perm(hi, l, 0x1040) & ~0xffu), __uint_as_float(__byte_perm(hi, l, 0x3250) & ~0xffu));
+    };
     int4 og, ou;
     uint32_t* ogu = reinterpret_cast<uint32_t*>(&og);
     uint32_t* ouu = reinterpret_cast<uint32_t*>(&ou);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 g = unpack_bf16(gu32[j]), u = unpack_bf16(uu32[j]), d = unpack_bf16(du32[j]);
+      const float2 g = pair(gu32[j], gl, j), u = pair(uu32[j], ul, j), d = unpack_bf16(du32[j]);
       const float s0 = 1.f / (1.f + __expf(-g.x)), s1 = 1.f / (1.f + __expf(-g.y));
       ogu[j] = pack_bf16(d.x * u.x * s0 * (1.f + g.x * (1.f - s0)), d.y * u.y * s1 * (1.f + g.y * (1.f - s1)));
       ouu[j] = pack_bf16(d.x * g.x * s0, d.y * g.y * s1);
@@ -500,14 +512,15 @@ extern "C" int prl_gather_pages(const void* kc, const void* vc, const int64_t* b
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
 }
-extern "C" int prl_swiglu_bwd(const void* gu, const void* dh, void* dgu, int64_t T, int F, cudaStream_t s) {
+extern "C" int prl_swiglu_bwd(const void* gu, const void* low, const void* dh, void* dgu, int64_t T, int F, cudaStream_t s) {
   if (F % 128 != 0) return -21;
   if (T <= 0) return 0;
   const int64_t nvec = T * (F / 8);
   int grid = static_cast<int>((nvec + 255) / 256);
   if (grid > 148 * 16) grid = 148 * 16;
-  swiglu_bwd_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(gu), static_cast<const __nv_bfloat16*>(dh),
-                                         static_cast<__nv_bfloat16*>(dgu), T, F);
+  auto kern = low ? swiglu_bwd_kernel<true> : swiglu_bwd_kernel<false>;
+  kern<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(gu), static_cast<const uint8_t*>(low), static_cast<const __nv_bfloat16*>(dh),
+                            static_cast<__nv_bfloat16*>(dgu), T, F);
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
 }

@@ -212,7 +212,7 @@ class _LoraFn(torch.autograd.Function):
         if not (need[0] or need[1] or any(need[7:])):
             return (None, None, dbias, dres, *[None] * (3 + 2 * len(ranks)))
         x, w, pa, pb, t, *gu = ctx.saved_tensors
-        dy = C.swiglu_bwd(gu[0], fn._aligned(dy)) if swiglu else _rows(dy)
+        dy = C.swiglu_bwd(gu[0], fn._aligned(dy), gu[1]) if swiglu else _rows(dy)
         dx, *grads = C.lora_bwd(dy, x, w, pa, pb, t, scale, ranks, widths, swiglu, (need[0], *need[7:]))
         dw = fn.mm_tn(dy, x, out=fn._sink_for(w)) if need[1] else None
         return (dx, dw, dbias, dres, None, None, None, *grads)

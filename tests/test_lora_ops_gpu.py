@@ -60,6 +60,30 @@ def test_lora_linear_swiglu(t, k, f, ranks):
     check_lora(lora_case(t, k, (f, f), ranks, t, BF, "cuda", swiglu=True))
 
 
+@pytest.mark.parametrize("t,k,f,r", [(1, 64, 128, 8), (300, 264, 256, 24), (700, 2048, 384, 16)])
+def test_saved_projection_has_sixteen_bits_of_mantissa(t, k, f, r):
+    """Gate and up as the backward gets them: truncated to 24 bits (2^-16); values that are not finite stay what they are."""
+    g = torch.Generator().manual_seed(t)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    x, w, low, b = rnd(t, k), rnd(2 * f, k), rnd(t, r), rnd(2 * f, r)
+    x[0, 0], w[5, 0], w[6, 0] = float("inf"), 1.0, 0.0
+    h, gu, lo = ops.ext().lora_gemm_swiglu(x, w, low, b, True)
+    got = ((gu.view(torch.int16).int() << 16) | (lo.int() << 8)).view(torch.float32).double()
+    ref = x.double() @ w.double().t() + low.double() @ b.double().t()
+    mag = x.double().abs() @ w.double().abs().t() + low.double().abs() @ b.double().abs().t()
+    fine = torch.isfinite(ref)
+    assert ((got - ref).abs() <= 2.0 ** -16 * ref.abs() + (k + r + 2) * 2.0 ** -24 * mag)[fine].all()
+    assert got[0, 5] == float("inf") and got[0, 6].isnan() and fine[1:].all()
+    dh = rnd(t, f)
+    near = ops.ext().swiglu_bwd(gu, dh, lo)
+    v = got.float()
+    gate, up = (v.view(t, -1, 2, 128)[:, :, i].reshape(t, f).double() for i in (0, 1))
+    sig = torch.sigmoid(gate)
+    want = torch.stack([dh.double() * up * sig * (1 + gate * (1 - sig)), dh.double() * gate * sig], 1).view(t, 2, -1, 128).transpose(1, 2).reshape(t, 2 * f)
+    size = torch.stack([dh.double().abs() * up.abs() * (1 + gate.abs()), dh.double().abs() * gate.abs()], 1).view(t, 2, -1, 128).transpose(1, 2).reshape(t, 2 * f)
+    assert ((near.double() - want).abs() <= half_step(BF) * want.abs() + 2.0 ** -19 * size + 2.0 ** -133)[1:].all()      # exp, quotients and four products of fp32
+
+
 def test_adapters_part_is_not_lost_beside_a_frozen_bias():
     """Every output that a subset of the leaves asks for, and the gradient of a trained weight."""
     c = lora_case(200, 128, (128, 64), (8, 16), 0, BF, "cuda", bias=True, residual=True)

@@ -186,38 +186,6 @@ def _lora_reference(x, w, parts, widths, scale, bias, residual, interleaved):
     return fn.linear(x, w, bias, residual) + d * scale
 
 
-class _LoraFn(torch.autograd.Function):
-    """x [T, K] through w [N, K] and the adapters a0, b0, a1, b1, ... (None, None: a part without).  swiglu: gate and up interleaved."""
-
-    @staticmethod
-    def forward(ctx, x, w, bias, residual, scale, widths, swiglu, *ab):
-        x, w = _rows(x), fn._g2_operand(w)
-        a, b = ([None if t is None else fn._aligned(t) for t in ab[i::2]] for i in (0, 1))
-        ranks = [0 if t is None else t.shape[0] for t in a]
-        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or any(ctx.needs_input_grad[7:])
-        y, pa, pb, t, *gu = _C().lora_fwd(x, w, a, b, widths, scale, swiglu, bias if bias is None else fn._aligned(bias),
-                                          residual if residual is None else fn._aligned(residual), need)
-        if need:
-            ctx.save_for_backward(x, w, pa, pb, t, *gu)
-        ctx.meta = (scale, widths, swiglu, ranks)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        C = _C()
-        scale, widths, swiglu, ranks = ctx.meta
-        need = ctx.needs_input_grad
-        dres = dy if need[3] else None
-        dbias = dy.sum(0) if need[2] else None
-        if not (need[0] or need[1] or any(need[7:])):
-            return (None, None, dbias, dres, *[None] * (3 + 2 * len(ranks)))
-        x, w, pa, pb, t, *gu = ctx.saved_tensors
-        dy = C.swiglu_bwd(gu[0], fn._aligned(dy), gu[1]) if swiglu else _rows(dy)
-        dx, *grads = C.lora_bwd(dy, x, w, pa, pb, t, scale, ranks, widths, swiglu, (need[0], *need[7:]))
-        dw = fn.mm_tn(dy, x, out=fn._sink_for(w)) if need[1] else None
-        return (dx, dw, dbias, dres, None, None, None, *grads)
-
-
 def _check_lora(name, x, w, parts, bias=None, residual=None) -> tuple:
     if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"{name}: rows {tuple(x.shape)} do not fit a projection {tuple(w.shape)}")
@@ -248,8 +216,8 @@ def _lora(x, w, parts, widths, scale, bias, residual, swiglu):
         return ref.swiglu(y) if swiglu else y
     ab = [t if t is None or t.dtype == x.dtype else t.to(x.dtype) for p in adapters for t in p or (None, None)]
     if x.dim() == 2:
-        return _LoraFn.apply(x, w, bias, residual, float(scale), widths, swiglu, *ab)
-    y = _LoraFn.apply(x.reshape(-1, x.shape[-1]), w, bias, None if residual is None else residual.reshape(-1, w.shape[0]), float(scale), widths, swiglu, *ab)
+        return _C().lora_linear(x, w, ab, widths, float(scale), bias, residual, swiglu)
+    y = _C().lora_linear(x.reshape(-1, x.shape[-1]), w, ab, widths, float(scale), bias, None if residual is None else residual.reshape(-1, w.shape[0]), swiglu)
     return y.reshape(*x.shape[:-1], y.shape[1])
 
 

@@ -94,11 +94,11 @@ def _delta(x, a, b, scales, plan, widths, interleaved, bias=None, residual=None,
 def _together(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Many rows: whether the adapters' part goes through the large product as further k-blocks, the low-rank values of all adapters side by
     side with a row's own kept (lora.cu).  That is LR (K + N) products a row for LR = adapters * parts * rank, whichever adapters the rows have;
-    a pass of its own is bound by the array of N values a row that it leaves.  The line is where both took as long, at about 1300 LR values' worth
-    of products for one of the array's.  Apart and together, rows, K, N, LR, us: 5003, 2048, 2048, 320: 85 and 66; 2900, 3584, 37888, 640: 892 and
-    732, with 1024 897 and 800; 3000, 896, 9728, 512: 178 and 106; 8000, 4096, 6144, 384: 396 and 381, with 1536 468 and 555; 4000, 14336, 4096, 512:
-    424 and 485."""
-    return a.shape[0] * a.shape[1] * (a.shape[2] + b.shape[1]) <= 1300 * b.shape[1]
+    a pass of its own is bound by the array of N values a row that it leaves.  The line is where both took as long, at about 2000 LR values' worth
+    of products for one of the array's.  Apart and together, rows, K, N, LR, us: 5003, 2048, 2048, 320: 81 and 59, with 768 111 and 82; 2900, 3584,
+    37888, 1024: 924 and 724; 3000, 896, 9728, 512: 204 and 135; 700, 4096, 6144, 384: 64 and 54, 8000 rows 339 and 339, with 1536 437 to 517 and 463
+    to 480; 4000, 14336, 4096, 512: 471 and 406."""
+    return a.shape[0] * a.shape[1] * (a.shape[2] + b.shape[1]) <= 2000 * b.shape[1]
 
 
 def _delta_reference(x, a, b, scales, ids, widths, interleaved):

@@ -153,7 +153,7 @@ def test_adapters(t, k, widths, rank, num):
 
 
 @pytest.mark.parametrize("t,k,widths,rank,num,together", [
-    (257, 64, (64,), 16, 2, True), (300, 896, (896, 128, 128), 16, 8, True), (515, 2048, (1024,), 64, 9, False), (1300, 256, (512, 64, 64), 32, 20, False),
+    (257, 64, (64,), 16, 2, True), (300, 896, (896, 128, 128), 16, 8, True), (515, 2048, (1024,), 64, 11, False), (1300, 256, (512, 64, 64), 32, 20, False),
     (2049, 512, (1536,), 128, 3, True)])
 def test_adapters_many_rows_both_ways(t, k, widths, rank, num, together, monkeypatch):
     """Through the large product, or in a pass of its own: the rule's choice and the other one, each within its bound."""

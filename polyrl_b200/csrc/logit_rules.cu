@@ -10,7 +10,7 @@
 //
 // Split: a block takes a part of one row's vocabulary and has a word in shared memory for each of its tokens.  Half of its warps clear the words, read the
 // row's whole history (out of L2 for all but the row's first block) and count the tokens of the part with shared-memory atomics, while the other half
-// copy the part under the row's mask, 16 bytes a thread.  Then all of them look through the words for touched tokens, pack them 32 to a warp, compute
+// copy the part under the row's mask, 16 bytes a thread (and count with the rest afterwards, where histories are long).  Then all of them look through the words for touched tokens, pack them 32 to a warp, compute
 // those logits from the input and write them over the copy.  In place only masked and touched tokens are written.  Nothing is hashed, sorted or kept
 // between calls; counters are integers, so results do not depend on the order of the threads.
 // Histories are sparse, so what bounds it is instructions before it is bytes.  A hashed table asked again for every token of the history ran its few hits
@@ -119,9 +119,13 @@ __device__ __forceinline__ void copy_part(const T* z, T* out, int size, const ui
 }
 
 template <class T, bool INPLACE, int BITS>
-__global__ void __launch_bounds__(kRuleThreads, 3) rules_kernel(RuleParams p, int parts, int part) {
-  constexpr int kAhead = 6;                            // tokens a thread has in flight
+__global__ void __launch_bounds__(kRuleThreads, BITS == 32 ? 2 : 3) rules_kernel(RuleParams p, int parts, int part) {
+  constexpr int kAhead = 6, kVecsAhead = 4;            // tokens that a thread has in flight; 16-byte loads of long histories
   constexpr int kCounting = kRuleThreads / 2;
+  // Histories so long that counting takes most of the time: the copying warps join once they are done, 16 bytes of tokens a load, with the registers of two
+  // blocks an SM instead of three.  24 rows of 151936 with 30011 tokens 23 -> 20 us, 8 rows with 32000 15 (4-byte loads) -> 13, one row 12 -> 10.
+  constexpr bool kLong = BITS == 32;
+  constexpr int kStride = kLong ? kRuleThreads : kCounting;
   using Word = RuleWord<BITS>;
   constexpr int kEach = 128 / BITS, kStep = 32 * kEach;          // tokens a lane and a warp look at together
   extern __shared__ __align__(16) uint32_t words[];    // [part] words of BITS bits, the row's bias list
@@ -140,7 +144,7 @@ __global__ void __launch_bounds__(kRuleThreads, 3) rules_kernel(RuleParams p, in
   const int32_t* tok = p.tokens + row * p.ld_tokens;
   int32_t token[kAhead];
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) token[u] = tid < kCounting && tid + u * kCounting < p.max_tokens ? __ldg(tok + tid + u * kCounting) : -1;
+  for (int u = 0; u < kAhead; ++u) token[u] = !kLong && tid < kCounting && tid + u * kStride < p.max_tokens ? __ldg(tok + tid + u * kStride) : -1;
   const int len = p.lens ? p.lens[row] : p.max_tokens, prompt = p.prompt_lens ? p.prompt_lens[row] : 0, least = p.num_stop > 0 ? p.min_lens[row] : 0;
   const float rep = p.rep ? p.rep[row] : 1.f, pres = p.pres ? p.pres[row] : 0.f, freq = p.freq ? p.freq[row] : 0.f;
   const uint32_t* mask = mask_of(p, row);
@@ -151,36 +155,63 @@ __global__ void __launch_bounds__(kRuleThreads, 3) rules_kernel(RuleParams p, in
     copy_part<T, INPLACE>(z, out, size, mask, tid, kRuleThreads);
     return;
   }
+  auto note = [&](int i, int32_t tkn) {               // the history's token i
+    const uint32_t at = static_cast<uint32_t>(tkn) - static_cast<uint32_t>(base);
+    if (at < static_cast<uint32_t>(size)) {
+      if (i < prompt) Word::mark(words, at, Word::kPrompt);
+      else Word::add(words, at, 1u);
+    }
+  };
+  // this thread's share of the history; the first of its tokens are there already (long histories: 16 bytes at a time, nothing is there)
+  auto count_tokens = [&]() {
+    if constexpr (kLong) {
+      const int head = min(static_cast<int>(-(reinterpret_cast<uintptr_t>(tok) >> 2) & 3), n), vecs = (n - head) / 4, tail = head + 4 * vecs;
+      if (tid < head) note(tid, __ldg(tok + tid));
+      if (tid < n - tail) note(tail + tid, __ldg(tok + tail + tid));
+      for (int v0 = tid; v0 < vecs; v0 += kVecsAhead * kStride) {
+        int4 q[kVecsAhead];
+#pragma unroll
+        for (int u = 0; u < kVecsAhead; ++u) q[u] = v0 + u * kStride < vecs ? __ldg(reinterpret_cast<const int4*>(tok + head) + v0 + u * kStride) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+        for (int u = 0; u < kVecsAhead; ++u) {
+          if (v0 + u * kStride >= vecs) continue;
+          const int i = head + 4 * (v0 + u * kStride);
+          note(i, q[u].x); note(i + 1, q[u].y); note(i + 2, q[u].z); note(i + 3, q[u].w);
+        }
+      }
+    } else {
+      for (int i0 = tid; i0 < n; i0 += kAhead * kStride) {
+        if (i0 != tid) {
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) token[u] = i0 + u * kStride < n ? __ldg(tok + i0 + u * kStride) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (i0 + u * kStride < n) note(i0 + u * kStride, token[u]);
+      }
+    }
+  };
   if (tid < kCounting) {                               // half of the warps count while the other half copies: both are latencies more than work
     for (int j = tid; j < p.num_bias; j += kCounting) bias_ids[j] = p.bias_ids[row * p.ld_bias + j];
     for (int i = tid; i < part * BITS / 128; i += kCounting) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
     asm volatile("bar.sync 1, %0;" ::"n"(kCounting) : "memory");
-    for (int i0 = tid; i0 < n; i0 += kAhead * kCounting) {
-      if (i0 != tid) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) token[u] = i0 + u * kCounting < n ? __ldg(tok + i0 + u * kCounting) : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const uint32_t at = static_cast<uint32_t>(token[u] - base);
-        const int i = i0 + u * kCounting;
-        if (i < n && at < static_cast<uint32_t>(size)) {
-          if (i < prompt) Word::mark(words, at, Word::kPrompt);
-          else Word::add(words, at, 1u);
-        }
-      }
-    }
+    if (kLong) asm volatile("bar.arrive 2, %0;" ::"n"(kRuleThreads) : "memory");
+    count_tokens();
     for (int j = tid; j < p.num_bias; j += kCounting) {
-      const uint32_t at = static_cast<uint32_t>(bias_ids[j] - base);
+      const uint32_t at = static_cast<uint32_t>(bias_ids[j]) - static_cast<uint32_t>(base);
       if (at < static_cast<uint32_t>(size)) Word::mark(words, at, Word::kBias);
     }
     if (early)
       for (int j = tid; j < p.num_stop; j += kCounting) {
-        const uint32_t at = static_cast<uint32_t>(p.stop_ids[row * p.ld_stop + j] - base);
+        const uint32_t at = static_cast<uint32_t>(p.stop_ids[row * p.ld_stop + j]) - static_cast<uint32_t>(base);
         if (at < static_cast<uint32_t>(size)) Word::mark(words, at, Word::kBanned);
       }
   } else {
     copy_part<T, INPLACE>(z, out, size, mask, tid - kCounting, kRuleThreads - kCounting);
+    if (kLong) {
+      asm volatile("bar.sync 2, %0;" ::"n"(kRuleThreads) : "memory");        // the words are clear
+      count_tokens();
+    }
   }
   __syncthreads();                                     // the words are complete, the copy is written
 
@@ -230,9 +261,9 @@ __global__ void __launch_bounds__(kRuleThreads, 3) rules_kernel(RuleParams p, in
 
 template <class T, int BITS>
 static int run_rules(const RuleParams& p, cudaStream_t stream) {
-  // parts as wide as leave some blocks for every SM: each of them reads the row's history
+  // parts as wide as leave some blocks for every SM: each of them reads the row's history (a long one is worth a block less)
   int part = kRulePart;
-  while (part > 2048 && static_cast<int64_t>(p.rows) * ((p.V + part - 1) / part) < 2 * 148) part /= 2;
+  while (part > 2048 && static_cast<int64_t>(p.rows) * ((p.V + part - 1) / part) < (BITS == 32 ? 222 : 296)) part /= 2;
   const int parts = (p.V + part - 1) / part;
   const int64_t blocks = static_cast<int64_t>(p.rows) * parts;
   if (blocks > 0x7fffffff) return -3;

@@ -44,6 +44,23 @@ def test_rules_counts_long_histories():
     check_rules(ops.adjust_logits(z, LogitRules(**case)), z, **case)
 
 
+@pytest.mark.parametrize("start", [0, 1, 2, 3])
+@pytest.mark.parametrize("n", [8192, 8193, 8195])
+def test_rules_long_histories_start_and_end_anywhere(n, start):
+    z, case = rules_case(12, 3000, n + 8, n + start, torch.bfloat16, "cuda")
+    wide = case["tokens"]
+    case["tokens"] = wide[:, start:start + n]
+    case["lens"] = torch.tensor([0, 1, 2, 3, 4, 5, 8, 4099, 6151, 8190, n - 1, n], dtype=torch.int32, device="cuda")
+    case["prompt_lens"] = case["lens"] // 3
+    assert case["tokens"].data_ptr() % 16 == 4 * start % 16
+    check_rules(ops.adjust_logits(z, LogitRules(**case)), z, **case)
+    y = z.clone()
+    ops.adjust_logits(y, LogitRules(**case), out=y)
+    check_rules(y, z, **case)
+    odd = wide.reshape(-1)[start:start + 12 * (n + 3)].view(12, n + 3)         # every row starts somewhere else
+    check_rules(ops.adjust_logits(z, LogitRules(**{**case, "tokens": odd})), z, **{**case, "tokens": odd})
+
+
 def test_rules_masked_places_may_hold_anything():
     z, case = rules_case(4, 300, 20, 1, torch.bfloat16, "cuda")
     z[:, ::3], z[:, 1::7], z[:, 5::11] = float("nan"), float("inf"), torch.finfo(torch.bfloat16).min

@@ -678,14 +678,6 @@ std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::
   return out;
 }
 
-// rows as the products read them: unit inner stride, pitch and base on 16 bytes (packed: and no gap between rows)
-at::Tensor lora_rows(const at::Tensor& t, bool packed = false) {
-  const bool aligned = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-  if (t.dim() != 2 || (aligned && t.stride(1) == 1 && (packed ? t.stride(0) == t.size(1) : t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)))) return t;
-  const at::Tensor c = t.contiguous(), d = (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
-  return d.size(0) == 1 ? d.as_strided(d.sizes(), {d.size(1), 1}) : d;      // a single row counts as contiguous whatever its pitch is
-}
-
 // lora_linear and lora_linear_swiglu with their gradients, all of it on this side: a call of few rows is bound by the host.  387 rows of a 896 -> 1152
 // projection in three parts, forward and backward: 166 us, 201 with the node in Python.
 struct LoraFn : public torch::autograd::Function<LoraFn> {
@@ -696,17 +688,17 @@ struct LoraFn : public torch::autograd::Function<LoraFn> {
   static at::Tensor forward(Ctx* ctx, const at::Tensor& x_in, const at::Tensor& w_in, const OptT& bias, const OptT& residual, const OptT& a0, const OptT& b0, const OptT& a1,
                             const OptT& b1, const OptT& a2, const OptT& b2, const std::vector<int64_t>& widths, double scale, bool swiglu, bool save) {
     const OptT in[kArgs] = {x_in, w_in, bias, residual, a0, b0, a1, b1, a2, b2};
-    const at::Tensor x = lora_rows(x_in), w = lora_rows(w_in);
+    const at::Tensor x = aligned_rows(x_in), w = aligned_rows(w_in);
     std::vector<OptT> a, b;
     std::vector<int64_t> meta{swiglu, static_cast<int64_t>(widths.size())};
     for (size_t i = 0; i < widths.size(); ++i) {
-      a.push_back(in[4 + 2 * i].has_value() ? OptT(lora_rows(*in[4 + 2 * i], true)) : c10::nullopt);
-      b.push_back(in[5 + 2 * i].has_value() ? OptT(lora_rows(*in[5 + 2 * i], true)) : c10::nullopt);
+      a.push_back(in[4 + 2 * i].has_value() ? OptT(aligned_rows(*in[4 + 2 * i], true)) : c10::nullopt);
+      b.push_back(in[5 + 2 * i].has_value() ? OptT(aligned_rows(*in[5 + 2 * i], true)) : c10::nullopt);
       meta.push_back(widths[i]);
       meta.push_back(a.back().has_value() ? a.back()->size(0) : 0);
     }
     std::vector<at::Tensor> r = lora_fwd(x, w, a, b, widths, scale, swiglu, bias.has_value() ? OptT(bias->contiguous()) : c10::nullopt,
-                                         residual.has_value() ? OptT(lora_rows(*residual, true)) : c10::nullopt, save);
+                                         residual.has_value() ? OptT(aligned_rows(*residual, true)) : c10::nullopt, save);
     if (ctx) {
       int64_t edge = 0;                              // place among the arguments that are there
       for (const OptT& t : in) meta.push_back(t.has_value() ? edge++ : -1);
@@ -743,7 +735,7 @@ struct LoraFn : public torch::autograd::Function<LoraFn> {
     if (!deep) return out;
     const Grads saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1];
-    const at::Tensor dy = swiglu ? swiglu_bwd(saved[5], lora_rows(grads[0], true), saved[6]) : lora_rows(grads[0]);
+    const at::Tensor dy = swiglu ? swiglu_bwd(saved[5], aligned_rows(grads[0], true), saved[6]) : aligned_rows(grads[0]);
     std::vector<bool> ask{want[0]};
     ask.insert(ask.end(), want + 4, want + 4 + 2 * parts);
     const std::vector<OptT> got = lora_bwd(dy, x, w, saved[2], saved[3], saved[4], ctx->saved_data["scale"].toDouble(), ranks, widths, swiglu, ask);

@@ -25,4 +25,12 @@ inline at::Tensor split_scratch(int64_t floats, const at::Tensor& like) {
 }
 inline float* split_ptr(const at::Tensor& ws) { return ws.defined() ? ws.data_ptr<float>() : nullptr; }
 
+// rows as the kernels read them: unit inner stride, pitch and base on 16 bytes (packed: and no gap between rows)
+inline at::Tensor aligned_rows(const at::Tensor& t, bool packed = false) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  if (t.dim() != 2 || (aligned && t.stride(1) == 1 && (packed ? t.stride(0) == t.size(1) : t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)))) return t;
+  const at::Tensor c = t.contiguous(), d = (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+  return d.size(0) == 1 ? d.as_strided(d.sizes(), {d.size(1), 1}) : d;      // a single row counts as contiguous whatever its pitch is
+}
+
 }  // namespace

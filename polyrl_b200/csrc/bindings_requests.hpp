@@ -152,11 +152,15 @@ at::Tensor adapter_delta(const at::Tensor& x, const at::Tensor& a, const at::Ten
 }
 
 // x w^T (+ bias) by the library, as a decode step's plain products, and what the adapters add to it
-at::Tensor adapter_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scales, const at::Tensor& plan,
-                          int64_t tile_rows, int64_t max_tiles, const std::vector<int64_t>& widths, const OptTensor& bias, const OptTensor& residual) {
-  TORCH_CHECK_VALUE(w.dim() == 2 && x.dim() == 2 && w.size(1) == x.size(1) && b.dim() == 3 && w.size(0) == b.size(1), "adapter_linear: the projection does not fit");
-  c10::cuda::CUDAGuard g(x.device());
-  return adapter_delta(x, a, b, scales, plan, tile_rows, max_tiles, widths, false, c10::nullopt, residual, at::linear(x, w, bias), 0, 0);
+at::Tensor adapter_linear(const at::Tensor& x_in, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scales, const at::Tensor& plan,
+                          int64_t adapters, int64_t tile_rows, int64_t max_tiles, const std::vector<int64_t>& widths, const OptTensor& bias, const OptTensor& residual) {
+  TORCH_CHECK_VALUE(w.dim() == 2 && x_in.dim() == 2 && w.size(1) == x_in.size(1) && a.dim() == 3 && b.dim() == 3 && w.size(0) == b.size(1), "adapter_linear: the projection does not fit");
+  TORCH_CHECK_VALUE(a.size(0) == adapters, "adapter_linear: a plan for ", adapters, " adapters, the stacks hold ", a.size(0));
+  c10::cuda::CUDAGuard g(x_in.device());
+  const at::AutoGradMode inference(false);
+  const at::Tensor x = aligned_rows(x_in);
+  return adapter_delta(x, a, b, scales, plan, tile_rows, max_tiles, widths, false, c10::nullopt, residual.has_value() ? OptTensor(aligned_rows(*residual)) : c10::nullopt,
+                       at::linear(x, w, bias), 0, 0);
 }
 
 }  // namespace

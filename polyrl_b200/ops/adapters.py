@@ -105,6 +105,7 @@ def _delta_reference(x, a, b, scales, ids, widths, interleaved):
     out = torch.zeros(x.shape[0], b.shape[1], dtype=torch.float32, device=x.device)
     n, r = b.shape[1], b.shape[2]
     part = (torch.arange(n) // 128) % 2 if interleaved else torch.repeat_interleave(torch.arange(len(widths)), torch.tensor(widths))
+    part = part.to(x.device)
     for l in range(a.shape[0]):
         rows = torch.nonzero(ids == l).flatten()
         if rows.numel():
@@ -115,7 +116,6 @@ def _delta_reference(x, a, b, scales, ids, widths, interleaved):
     return out
 
 
-@torch.no_grad()
 def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan, widths=None,
                    bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
     """Rows of ``x`` [T, K] through the shared projection ``w`` [N, K] (or an ``Fp8Weight``) and each through its own adapter l:
@@ -127,14 +127,19 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     padded with zeros).  Up to 256 rows the adapters add to what ``linear`` gives, so that a row without one is ``linear``'s bit for bit (without
     a residual).  With more rows ``b`` must be finite: rows of other adapters may be multiplied by it and zero.  Inference only."""
     widths = (w.shape[0],) if widths is None else tuple(widths)
+    if plan.buf is not None and x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._plain_decode(x, w):          # one call: a step of few rows is bound by the host
+        return _C().adapter_linear(x, w, a, b, scales, plan.buf, plan.num_adapters, plan.tile_rows, plan.max_tiles, widths, bias, residual)
+    return _adapter_linear(x, w, a, b, scales, plan, widths, bias, residual)
+
+
+@torch.no_grad()
+def _adapter_linear(x, w, a, b, scales, plan, widths, bias, residual):
     if not fn._is_kernel_tensor(x) or plan.buf is None:          # (the kernels' bindings check as much, but for what the plan was made for)
         _check_adapters("adapter_linear", x, w, a, b, scales, plan, widths, bias, residual)
         y = fn.linear(x, w, bias, residual)
         return (y.float() + _delta_reference(x, a, b, scales, plan.ids, widths, False)).to(x.dtype)
     _of_plan("adapter_linear", a, plan)
-    if fn._is_decode_shape(x, w) and fn._plain_decode(x, w):
-        return _C().adapter_linear(_rows(x), w, a, b, scales, plan.buf, plan.tile_rows, plan.max_tiles, widths, bias, None if residual is None else _rows(residual))
-    if fn._is_decode_shape(x, w) or isinstance(w, fn.Fp8Weight) or fn._cublas():
+    if x.shape[0] <= fn._SKINNY_MAX_ROWS or isinstance(w, fn.Fp8Weight) or fn._cublas():
         return _delta(x, a, b, scales, plan, widths, False, None, residual, fn.linear(x, w, bias).contiguous())
     w = fn._g2_operand(w.to(x.dtype))
     if _together(a, b):

@@ -322,3 +322,17 @@ def test_adapters_refuse_the_plan_of_other_stacks(t):
             ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], plan, (128, 128))
         with pytest.raises(ValueError, match="a plan for"):
             ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], plan)
+
+
+@pytest.mark.parametrize("t", [5, 300])
+def test_adapters_plain_form_of_fp32_rows(t):
+    c = adapters_case(t, 64, (64, 32), 16, 3, t, torch.float32, "cuda")
+    check_near(run_adapters(c, (64, 32), 3), *adapters64(**c, widths=(64, 32)))
+
+
+def test_adapter_linear_leaves_no_graph():
+    c = adapters_case(6, 64, (64,), 16, 2, 0, torch.bfloat16, "cuda")
+    w, x = c["w"].clone().requires_grad_(), c["x"].clone().requires_grad_()
+    y = ops.adapter_linear(x, w, c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], 2))
+    assert not y.requires_grad and torch.is_grad_enabled()
+    assert torch.equal(y, ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], 2)))

@@ -16,8 +16,11 @@
 //        both operands of a product use the same permutation, and sums do not mind.
 //        Ranks are a few dozen, so the products are bound by their operands' bytes and mma.sync keeps up; tcgen05 would want 128 rows of
 //        one adapter and a round trip through tensor memory, longer than the whole kernel at decode.  What bounds it is latency: loads, two
-//        cluster barriers and loads again, in 5.2 us for one row (K 896, N 1152), 9.8 for 128 rows of 24 adapters (4096, 6144, rank 16; 17 MB),
-//        18.5 for 45 rows of 9 (3584, 37888, rank 32; 30 MB), 50 for 5003 rows of 5 (2048, 2048, rank 64; 64 MB).
+//        cluster barriers and loads again, in 5.1 us for one row (K 896, N 1152), 8.9 for 128 rows of 24 adapters (4096, 6144, rank 16; 17 MB; 10.0
+//        added to the shared product), 13.4 for 45 rows of 9 (3584, 37888, rank 32; 30 MB), 50 for 5003 rows of 5 (2048, 2048, rank 64; 64 MB).
+//        With cold caches the first product takes half of the time and the second one a quarter.  Rows of a and x copied into shared memory in bulk,
+//        512 bytes a request, took 11.8 us for the 128 rows; the loads of the second product a step ahead of its products, tiles of 64 rows and
+//        three CTAs an SM were slower, too.  Bringing the next product's first weights into L2 from here did not shorten that product.
 #include "adapters.hpp"
 #include "common.cuh"
 

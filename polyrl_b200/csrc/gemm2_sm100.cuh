@@ -41,6 +41,7 @@ constexpr int kSmemMax = 232448;   // 227 KB opt-in limit per CTA
 // (K of about a thousand) leave it no time: the figures are beside its users.
 // TAIL: the sum goes on over a second pair of operands, D = A B^T + A2 B2^T with A2 [M, R] K-major and B2 laid out as B: further k-blocks of the
 // same tiles, out of other tensor maps.  A low-rank adapter beside a weight costs ceil(R / 64) k-blocks this way and no pass over D.
+// Without and with it: 4099 x 6144 x 2048, R 64: 75.2 and 76.1 us; 8191 x 4096 x 6144, R 48: 281 and 297; 6001 x 4096 x 28672 with SwiGLU, R 64: 1162 and 1188.
 struct alignas(64) Gemm2Tail {
   CUtensorMap A, B;
   int main_kb;             // k-blocks of the first pair; K counts those of both, 64 each

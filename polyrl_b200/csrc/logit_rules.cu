@@ -16,6 +16,8 @@
 // Histories are sparse, so what bounds it is instructions before it is bytes.  A hashed table asked again for every token of the history ran its few hits
 // a warp one lane at a time (256 rows of 128256 bf16 logits with histories of up to 1100: 52 us); a list that the counting threads append to saves the
 // search but waits for every atomic's answer (24 rows with histories of 30011: 42 us).
+// Now 39 us for the former (34 in place; a plain copy of these logits takes 22), 20 for the latter, 9 for 37 rows of 50257 fp32 logits, 4.5 for one row of
+// 151936.
 #include "common.cuh"
 #include "logit_rules.hpp"
 

@@ -14,7 +14,9 @@
 //        where the sum runs over tokens: dA is computed as x^T dt and stored transposed).  A cluster of S CTAs shares a tile's reduction,
 //        because R is narrow and 128-row tiles alone are too few to draw HBM bandwidth: 32 tiles for dA of a 4096-wide layer.  The CTAs
 //        leave their fp32 sums in shared memory and each adds up its share of the tile over distributed shared memory, in the order of the
-//        ranks: results do not depend on timing.
+//        ranks: results do not depend on timing.  Bound by the stream of its large operand where its rows are contiguous (8191 rows, 48 columns: t from
+//        4096 columns 11 us, 5.9 TB/s; dt from 6144 19 us, 5.3 TB/s), by pieces of 128 bytes a row out of it where the sum runs over its rows (dA 20 us, 3.4
+//        TB/s; dB 25 us, 4.0 TB/s).
 // pack   A parts one below the other, B parts block-diagonal in the order of the projection's columns, ranks padded to 8 with zeros; a bias
 //        becomes one more column of B against a column of ones in t, which the forward product then adds for nothing.
 #include "gemm_sm100.cuh"

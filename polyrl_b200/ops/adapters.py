@@ -149,31 +149,40 @@ def _adapter_linear(x, w, a, b, scales, plan, widths, bias, residual):
     return _C().gemm_bf16(_rows(x), w, d)
 
 
-@torch.no_grad()
 def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
     """``linear_swiglu`` with an adapter for every row: ``a`` [adapters, 2 * rank, K] (gate, up), ``b`` [adapters, 2 F, rank] with its rows in the
     order of ``wgu``'s (blocks of 128 gate and 128 up rows); the adapters act before the activation.  Inference only."""
     n = wgu.shape[0]
     if n % 256:
         raise ValueError("adapter_linear_swiglu: gate and up in blocks of 128 rows each")
+    widths = (n // 2, n // 2)
+    if not fn._is_kernel_tensor(x) or plan.buf is None or isinstance(wgu, fn.Fp8Weight) or fn._cublas():
+        return _adapter_linear_swiglu(x, wgu, a, b, scales, plan, widths)
+    _of_plan("adapter_linear_swiglu", a, plan)
+    if x.shape[0] > fn._SKINNY_MAX_ROWS and wgu.dtype == x.dtype and _together(a, b):
+        return _C().adapter_gemm(_rows(x), fn._g2_operand(wgu), a, b, scales, plan.ids, widths, True, None, None)
+    x = _rows(x)
+    d = _delta(x, a, b, scales, plan, widths, True)
+    if fn._stream_swiglu(x, wgu):
+        return _C().stream_gemm(x, wgu, d, None, None, None, 2, 0, None, -1)
+    return _C().gemm_swiglu_add(x, wgu, d)
+
+
+@torch.no_grad()
+def _adapter_linear_swiglu(x, wgu, a, b, scales, plan, widths):
     if not fn._is_kernel_tensor(x) or plan.buf is None:
-        _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, (n // 2, n // 2))
-        gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, (n // 2, n // 2), True)
+        _check_adapters("adapter_linear_swiglu", x, wgu, a, b, scales, plan, widths)
+        gu = fn.linear(x, wgu).float() + _delta_reference(x, a, b, scales, plan.ids, widths, True)
         return ref.swiglu(gu).to(x.dtype)
     _of_plan("adapter_linear_swiglu", a, plan)
-    if x.shape[0] > 256 and not isinstance(wgu, fn.Fp8Weight) and not fn._cublas() and wgu.dtype == x.dtype and _together(a, b):
-        return _C().adapter_gemm(_rows(x), fn._g2_operand(wgu), a, b, scales, plan.ids, (n // 2, n // 2), True, None, None)
-    d, x = _delta(x, a, b, scales, plan, (n // 2, n // 2), True), _rows(x)
+    x = _rows(x)
+    d = _delta(x, a, b, scales, plan, widths, True)
     if isinstance(wgu, fn.Fp8Weight):
         xq, xs = fn.quantize_fp8_rowwise(x)
         if 0 < x.shape[0] <= fn._SKINNY_MAX_ROWS and fn._stream_impl():
             return _C().stream_gemm(xq, wgu.q, d, None, xs, wgu.scale, 2, 0, None, 0)
         return ref.swiglu(_C().gemm_fp8(xq, wgu.q, xs, wgu.scale, 0) + d)
-    if fn._cublas():
-        return ref.swiglu(d.addmm_(x, wgu.t()))
-    if fn._stream_swiglu(x, wgu):
-        return _C().stream_gemm(x, wgu, d, None, None, None, 2, 0, None, -1)
-    return _C().gemm_swiglu_add(x, wgu, d)
+    return ref.swiglu(d.addmm_(x, wgu.t()))
 
 
 # --------------------------------------------------------------------------------------------

@@ -77,7 +77,6 @@ def _check(logits: torch.Tensor, r: LogitRules, out: torch.Tensor | None) -> Non
         raise ValueError("adjust_logits: out must be like the logits")
 
 
-@torch.no_grad()
 def adjust_logits(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
     """``logits`` [B, V] (bf16 or fp32) under ``rules``, in a new tensor, in ``out``, or in place (``out=logits``), which leaves alone what
     no rule touches.  With c the times that a token is among the row's output tokens:
@@ -95,8 +94,9 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | N
         return ext().adjust_logits(logits, out, r.tokens, r.lens, r.prompt_lens, r.repetition, r.presence, r.frequency, r.bias_ids, r.bias_values, r.stop_ids,
                                    r.min_lens, r.masks, r.mask_rows)
     _check(logits, rules, out)
-    z = _adjust_reference(logits, rules)
-    return z if out is None else out.copy_(z)
+    with torch.no_grad():
+        z = _adjust_reference(logits, rules)
+        return z if out is None else out.copy_(z)
 
 
 def _adjust_reference(logits: torch.Tensor, r: LogitRules) -> torch.Tensor:

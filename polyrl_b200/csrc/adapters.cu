@@ -27,31 +27,58 @@
 namespace prl {
 
 // ------------------------------------------------------------------------------------------------------------ plan
-// Rows in passes of 1024: a warp ranks its rows among those of the same adapter by match, a scan over the 32 warps' counts does the rest.
+// Every warp has a run of rows: it counts them by adapter, sums over the warps and groups give each count its first place, and the warp goes through its
+// rows again, 32 at a time ranked by match, to put them there.  Nothing waits for the block between 32 rows: 128 rows 2.7 us, 5003 of five adapters 4.4 (8.3
+// where the block ranks 1024 rows at a time).
 constexpr int kPlanThreads = 1024;
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int tile_rows, int max_tiles,
                                                             int32_t* __restrict__ order, AdapterTile* __restrict__ tiles, int32_t* __restrict__ num_tiles) {
   extern __shared__ int32_t sm[];
+  constexpr int kAhead = 4;                          // ids a lane has in flight
   const int G = L + 1;                               // the last group: no adapter
-  int32_t* at = sm;                                  // [G] where the group's next row goes
+  int32_t* rows_of = sm;                             // [G] rows of the group, then where its first one goes
   int32_t* tile_at = sm + G;                         // [G] its first tile
-  int32_t* per_warp = sm + 2 * G;                    // [32][G]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* mine = sm + (2 + warp) * G;               // [warps][G] a warp's rows of each group, then how many are before its next one
   grid_behind();
-  for (int g = tid; g < G; g += kPlanThreads) at[g] = 0;
-  for (int i = tid; i < 32 * G; i += kPlanThreads) per_warp[i] = 0;
+  const int each = (T + kPlanThreads - 1) / kPlanThreads * 32, warps = (T + each - 1) / each, row0 = min(warp * each, T), row1 = min(row0 + each, T);
+  for (int i = tid; i < warps * G; i += kPlanThreads) sm[2 * G + i] = 0;
   __syncthreads();
-  auto group_of = [&](int row) {
-    const int id = ids[row];
-    return id >= 0 && id < L ? id : L;
+  // f(row, its group or -1), 32 rows of the warp at a time
+  auto rows = [&](auto f) {
+    for (int r0 = row0; r0 < row1; r0 += 32 * kAhead) {
+      int g[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int row = r0 + 32 * u + lane, id = row < row1 ? __ldg(ids + row) : 0;
+        g[u] = row >= row1 ? -1 : id >= 0 && id < L ? id : L;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (r0 + 32 * u >= row1) break;
+        f(r0 + 32 * u + lane, g[u]);
+      }
+    }
   };
-  for (int i = tid; i < T; i += kPlanThreads) atomicAdd(&at[group_of(i)], 1);
+  rows([&](int, int g) {
+    if (g >= 0) atomicAdd(mine + g, 1);
+  });
+  __syncthreads();
+  for (int g = tid; g < G; g += kPlanThreads) {      // counts -> how many of the group's rows are before the warp's
+    int n = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int c = sm[(2 + w) * G + g];
+      sm[(2 + w) * G + g] = n;
+      n += c;
+    }
+    rows_of[g] = n;
+  }
   __syncthreads();
   if (warp == 0) {                                   // exclusive sums of rows and of tiles over the groups
     int rows0 = 0, tiles0 = 0;
     for (int g0 = 0; g0 < G; g0 += 32) {
-      const int g = g0 + lane, n = g < G ? at[g] : 0, nt = (n + tile_rows - 1) / tile_rows;
+      const int g = g0 + lane, n = g < G ? rows_of[g] : 0, nt = (n + tile_rows - 1) / tile_rows;
       int rs = n, ts = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -59,11 +86,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
         if (lane >= o) { rs += r; ts += t; }
       }
       if (g < G) {
-        const int first = rows0 + rs - n, t0 = tiles0 + ts - nt;
-        at[g] = first;
-        tile_at[g] = t0;
-        for (int k = 0; k < nt && t0 + k < max_tiles; ++k)
-          tiles[t0 + k] = AdapterTile{g < L ? g : -1, first + k * tile_rows, min(tile_rows, n - k * tile_rows), 0};
+        rows_of[g] = rows0 + rs - n;
+        tile_at[g] = tiles0 + ts - nt;
       }
       rows0 += __shfl_sync(0xffffffffu, rs, 31);
       tiles0 += __shfl_sync(0xffffffffu, ts, 31);
@@ -71,28 +95,20 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
     if (lane == 0) *num_tiles = min(tiles0, max_tiles);
   }
   __syncthreads();
-  for (int i0 = 0; i0 < T; i0 += kPlanThreads) {
-    const int row = i0 + tid;
-    const int g = row < T ? group_of(row) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, g);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    if (g >= 0 && rank == 0) per_warp[warp * G + g] = __popc(same);
-    __syncthreads();
-    for (int k = tid; k < G; k += kPlanThreads) {    // counts -> places, and the group moves on
-      int p = at[k];
-      for (int w = 0; w < 32; ++w) {
-        const int c = per_warp[w * G + k];
-        per_warp[w * G + k] = p;
-        p += c;
-      }
-      at[k] = p;
-    }
-    __syncthreads();
-    if (g >= 0) order[per_warp[warp * G + g] + rank] = row;
-    __syncthreads();
-    for (int k = tid; k < 32 * G; k += kPlanThreads) per_warp[k] = 0;
-    __syncthreads();
+  for (int g = warp; g < G; g += 32) {
+    const int first = rows_of[g], n = (g + 1 < G ? rows_of[g + 1] : T) - first, t0 = tile_at[g];
+    for (int k = lane; k * tile_rows < n && t0 + k < max_tiles; k += 32) tiles[t0 + k] = AdapterTile{g < L ? g : -1, first + k * tile_rows, min(tile_rows, n - k * tile_rows), 0};
   }
+  rows([&](int row, int g) {
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    const int before = g >= 0 ? mine[g] : 0;
+    __syncwarp();
+    if (g >= 0) {
+      order[rows_of[g] + before + __popc(same & ((1u << lane) - 1))] = row;
+      if (lane == __ffs(same) - 1) mine[g] = before + __popc(same);
+    }
+    __syncwarp();
+  });
 }
 
 // ------------------------------------------------------------------------------------------------------------ delta

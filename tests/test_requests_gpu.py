@@ -139,7 +139,8 @@ def run_adapters(c, widths, num):
     return ops.adapter_linear(c["x"], c["w"], c["a"], c["b"], c["scales"], plan, widths, c["bias"], c["residual"])
 
 
-@pytest.mark.parametrize("t,num,kind", [(1, 1, "all"), (5, 3, "mixed"), (33, 2, "one"), (256, 40, "mixed"), (257, 1, "none"), (700, 5, "runs"), (3000, 1000, "mixed")])
+@pytest.mark.parametrize("t,num,kind", [(1, 1, "all"), (5, 3, "mixed"), (33, 2, "one"), (256, 40, "mixed"), (257, 1, "none"), (700, 5, "runs"), (3000, 1000, "mixed"),
+                                        (1025, 3, "mixed"), (4098, 6, "runs"), (20011, 1024, "mixed"), (9999, 8, "mixed")])
 def test_plan_sorts_rows(t, num, kind):
     ids = {"all": torch.zeros(t), "one": torch.ones(t), "none": torch.full((t,), -7.0), "mixed": torch.randint(-1, num + 1, (t,)).float(),
            "runs": torch.arange(num).repeat_interleave(t // num).float()}[kind].int().cuda()

@@ -16,6 +16,7 @@ int64_t prl_gemm2_tail_ws_floats(int, int, int, int);
 int prl_gemm2_tail_bf16(const void*, const void*, const void*, const void*, void*, const void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int, float*, cudaStream_t);
 int prl_gemm_swiglu_tail_bf16(const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*, cudaStream_t);
 int prl_lora_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, float, int, int, int, int, int, cudaStream_t);
+int prl_lora_grads(const void*, const void*, void*, const void*, const void*, void*, int, int, int, int, int64_t, int64_t, int64_t, int64_t, int, int, int, cudaStream_t);
 int prl_lora_pack(const prl::LoraPackParams*, cudaStream_t);
 int prl_adapter_thin(const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, int, const int32_t*, const float*, int, cudaStream_t);
 int prl_adapter_pack(const void*, const void*, void*, const prl::LoraPackParams*, int, int, cudaStream_t);
@@ -584,6 +585,21 @@ at::Tensor lora_thin(const at::Tensor& a, const at::Tensor& b, int64_t layout, d
   return out;
 }
 
+// {dA [R, K], dB [N, R]} of an adapter: dt^T x and dy^T t in one launch, dt [T, 2 R] and t [T, lo + R] in two halves
+std::vector<at::Tensor> lora_grads(const at::Tensor& x, const at::Tensor& dt, const at::Tensor& dy, const at::Tensor& t, int64_t R, int64_t lo, int64_t split) {
+  const void *px = lora_operand(x, x, "lora_grads: x"), *pdt = lora_operand(dt, x, "lora_grads: dt"), *pdy = lora_operand(dy, x, "lora_grads: dy"),
+             *pt = lora_operand(t, x, "lora_grads: t");
+  const int64_t T = x.size(0), K = x.size(1), N = dy.size(1);
+  TORCH_CHECK(dt.size(0) == T && dy.size(0) == T && t.size(0) == T && R > 0 && R % 8 == 0 && lo >= R && lo % 8 == 0 && dt.size(1) == 2 * R && t.size(1) == lo + R &&
+              T <= 0x7fffffff && K <= 0x7fffffff && N <= 0x7fffffff, "lora_grads: sizes");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor da = at::empty({R, K}, x.options()), db = at::empty({N, R}, x.options());
+  if (T == 0) return {da.zero_(), db.zero_()};
+  check(prl_lora_grads(px, pdt, da.data_ptr(), pdy, pt, db.data_ptr(), K, N, R, T, x.stride(0), dt.stride(0), dy.stride(0), t.stride(0), R, lo, static_cast<int>(split),
+                       cur_stream()), "lora_grads");
+  return {da, db};
+}
+
 // x w^T + t b^T (b_mn: x w + t b, w [K, N], b [R, N]) (+ residual)
 at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const at::Tensor& b, bool b_mn, const OptT& residual) {
   const void *px = lora_operand(x, x, "lora_gemm: x"), *pw = lora_operand(w, x, "lora_gemm: w"), *pt = lora_operand(t, x, "lora_gemm: t"),
@@ -662,9 +678,16 @@ std::vector<OptT> lora_bwd(const at::Tensor& dy, const at::Tensor& x, const at::
   std::vector<OptT> out(want.size());
   at::Tensor dt, da, db;
   if (want[0] || need_a) dt = lora_thin(dy, pb, 1, scale, r, 0, need_a, 0, 0);
-  if (need_b) db = lora_thin(dy, t, 2, 1.0, r, 0, false, pb.size(1), 0);              // right behind the other product that reads dy
+  if (need_a && need_b) {                             // right behind the other product that reads dy
+    const std::vector<at::Tensor> both = lora_grads(x, dt, dy, t, r, pb.size(1), 0);
+    da = both[0];
+    db = both[1];
+  } else if (need_b) {
+    db = lora_thin(dy, t, 2, 1.0, r, 0, false, pb.size(1), 0);
+  } else if (need_a) {
+    da = lora_thin(x, dt, 3, 1.0, r, 0, false, r, 0);
+  }
   if (want[0]) out[0] = lora_gemm(dy, w, dt.narrow(1, 0, r), pa, true, c10::nullopt);
-  if (need_a) da = lora_thin(x, dt, 3, 1.0, r, 0, false, r, 0);
   int64_t col = 0, row = 0;
   for (size_t i = 0; i < ranks.size(); ++i) {
     if (ranks[i] > 0 && want[1 + 2 * i]) out[1 + 2 * i] = da.narrow(0, col, ranks[i]);
@@ -984,6 +1007,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adapter_gemm", &adapter_gemm);
   m.def("lora_thin", &lora_thin, py::arg("a"), py::arg("b"), py::arg("layout"), py::arg("scale") = 1.0, py::arg("rank") = 0, py::arg("pad") = 0,
         py::arg("halves") = false, py::arg("lo") = 0, py::arg("split") = 0);
+  m.def("lora_grads", &lora_grads, py::arg("x"), py::arg("dt"), py::arg("dy"), py::arg("t"), py::arg("R"), py::arg("lo"), py::arg("split") = 0);
   m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("b"), py::arg("b_mn") = false, py::arg("residual") = py::none());
   m.def("lora_gemm_swiglu", &lora_gemm_swiglu);
   m.def("stream_gemm", &stream_gemm, py::arg("x"), py::arg("w"), py::arg("residual") = py::none(), py::arg("bias") = py::none(),

@@ -16,7 +16,8 @@
 //        leave their fp32 sums in shared memory and each adds up its share of the tile over distributed shared memory, in the order of the
 //        ranks: results do not depend on timing.  Bound by the stream of its large operand where its rows are contiguous (8191 rows, 48 columns: t from
 //        4096 columns 11 us, 5.9 TB/s; dt from 6144 19 us, 5.3 TB/s), by pieces of 128 bytes a row out of it where the sum runs over its rows (dA 20 us, 3.4
-//        TB/s; dB 25 us, 4.0 TB/s).
+//        TB/s; dB 25 us, 4.0 TB/s).  So dA and dB are one launch, whose CTAs fill the chip together: one after the other and together 52 and 39 us there,
+//        34 and 22 for 4099 x 6144 / 2048, 64 columns, 11.2 and 6.5 for 387 x 896 / 1152.
 // pack   A parts one below the other, B parts block-diagonal in the order of the projection's columns, ranks padded to 8 with zeros; a bias
 //        becomes one more column of B against a column of ones in t, which the forward product then adds for nothing.
 #include "gemm_sm100.cuh"
@@ -46,11 +47,21 @@ struct ThinParams {
   const int32_t* ids;
   const float* scales;
   int each;
+  int trans;                                         // out is [R, M]
+  int tiles;                                         // of 128 rows
 };
 
-// grid (S, blocks of NR columns, tiles), so that the blocks that read the same rows of A run together; A_MN / B_MN: the reduction runs over the operand's rows in memory; TRANS: out is [R, M]
-template <bool A_MN, bool B_MN, bool TRANS>
-__global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const ThinParams p) {
+struct alignas(64) ThinMaps {
+  CUtensorMap A, B;
+};
+
+// grid (S, blocks of NR columns, tiles), so that the blocks that read the same rows of A run together; A_MN / B_MN: the reduction runs over the operand's rows
+// in memory.  Tiles from the first product's last one on are a second product's, with the same reduction length and columns.
+template <bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constant__ ThinMaps maps1, const __grid_constant__ ThinMaps maps2, const ThinParams p1, const ThinParams p2) {
+  const bool second = static_cast<int>(blockIdx.z) >= p1.tiles;
+  const CUtensorMap *tmA = second ? &maps2.A : &maps1.A, *tmB = second ? &maps2.B : &maps1.B;
+  const ThinParams p = second ? p2 : p1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[8], empty_bar[8], done_bar;
@@ -61,13 +72,13 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
   uint32_t S;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
   const uint32_t rank = cluster_ctarank();
-  const int m0 = blockIdx.z * kBlockM, r0 = blockIdx.y * p.NR;
+  const int m0 = (static_cast<int>(blockIdx.z) - (second ? p1.tiles : 0)) * kBlockM, r0 = blockIdx.y * p.NR;
   const int num_kb = (p.K + 63) / 64, kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
   const uint32_t tmem_cols = cols_acc <= 32 ? 32 : cols_acc <= 64 ? 64 : cols_acc <= 128 ? 128 : 256;
 
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(tmA);
+    tma_prefetch_desc(tmB);
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&full_bar[i], 1);
       mbar_init(&empty_bar[i], 1);
@@ -95,18 +106,18 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
         uint8_t* sa = smem + stage * stage_bytes;
         uint8_t* sb = sa + kThinStageA;
         if constexpr (A_MN) {
-          tma_load_2d(&tmA, &full_bar[stage], sa, m0, kb * 64);
-          tma_load_2d(&tmA, &full_bar[stage], sa + 8192, m0 + 64, kb * 64);
+          tma_load_2d(tmA, &full_bar[stage], sa, m0, kb * 64);
+          tma_load_2d(tmA, &full_bar[stage], sa + 8192, m0 + 64, kb * 64);
         } else {
-          tma_load_2d(&tmA, &full_bar[stage], sa, kb * 64, m0);
+          tma_load_2d(tmA, &full_bar[stage], sa, kb * 64, m0);
         }
         if constexpr (B_MN) {
           for (int c = 0; c < p.NR; c += 64) {
-            tma_load_2d(&tmB, &full_bar[stage], sb + c / 64 * 8192, r0 + c, kb * 64);
-            if (p.lo_in > 0) tma_load_2d(&tmB, &full_bar[stage], sb + (thin_lo(p.NR) + c) / 64 * 8192, p.lo_in + r0 + c, kb * 64);
+            tma_load_2d(tmB, &full_bar[stage], sb + c / 64 * 8192, r0 + c, kb * 64);
+            if (p.lo_in > 0) tma_load_2d(tmB, &full_bar[stage], sb + (thin_lo(p.NR) + c) / 64 * 8192, p.lo_in + r0 + c, kb * 64);
           }
         } else {
-          tma_load_2d(&tmB, &full_bar[stage], sb, kb * 64, r0);
+          tma_load_2d(tmB, &full_bar[stage], sb, kb * 64, r0);
         }
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
     return make_float4(v.x * p.scale, v.y * p.scale, v.z * p.scale, v.w * p.scale);
   };
   const int cols = min(p.NR, p.R - r0);
-  if constexpr (!TRANS) {                            // a share of the rows, four columns a thread
+  if (!p.trans) {                                    // a share of the rows, four columns a thread
     const int rows0 = kBlockM * rank / S, rows1 = kBlockM * (rank + 1) / S;
     const int last = blockIdx.y + 1 == gridDim.y ? p.pad : 0, quads = (cols + last) / 4;
     for (int e = threadIdx.x; e < (rows1 - rows0) * quads; e += kThinThreads) {
@@ -221,22 +232,40 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const __grid_constan
   cluster_sync_all();                                // a peer may still read this CTA's sums
 }
 
-template <bool A_MN, bool B_MN, bool TRANS>
-static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int64_t ldb, int split, cudaStream_t stream) {
-  const bool halves = B_MN && p.lo_in > 0;
+// a product's operands, A and B with their pitches, and what is done with it
+struct ThinProduct {
+  const void *A, *B;
+  int64_t lda, ldb;
+  ThinParams p;
+};
+
+template <bool A_MN, bool B_MN>
+static int run_thin(ThinProduct* q, int count, int split, cudaStream_t stream) {
+  const ThinParams& f = q[0].p;
+  const bool halves = B_MN && f.lo_in > 0;
   // blocks of up to 128 columns, as even as 16 allows: their CTAs share an SM with another's, whose loads run while these sum up.  Up to 256 columns a
   // block, K-major: 5003 x 2048, 320 columns 29 -> 15 us; 2900 x 3584, 768 columns 41 -> 22; 8191 x 4096, 192 columns 27 -> 21.
-  const int even = (p.R + 127) / 128;
-  p.NR = ((p.R + even - 1) / even + 15) / 16 * 16;
-  const int cols = halves ? thin_lo(p.NR) + p.NR : p.NR;
-  const int stage = kThinStageA + thin_b_bytes<B_MN>(p.NR, halves), sums = kBlockM * (cols + 4) * 4;
+  const int even = (f.R + 127) / 128, NR = ((f.R + even - 1) / even + 15) / 16 * 16;
+  const int cols = halves ? thin_lo(NR) + NR : NR;
+  const int stage = kThinStageA + thin_b_bytes<B_MN>(NR, halves), sums = kBlockM * (cols + 4) * 4;
   const int budget = cols <= 128 ? 100 * 1024 : 200 * 1024;           // two CTAs an SM where two fit
-  p.stages = budget / stage > 8 ? 8 : budget / stage;
-  const int smem = (p.stages * stage > sums ? p.stages * stage : sums) + 1024;
-  CUtensorMap tmA, tmB;
-  if (A_MN ? make_tmap_kmajor(&tmA, A, p.K, p.M, lda * 2, 64, 2) : make_tmap_kmajor(&tmA, A, p.M, p.K, lda * 2, kBlockM, 2)) return -2;
-  if (B_MN ? make_tmap_kmajor(&tmB, B, p.K, halves ? p.lo_in + p.R : p.R, ldb * 2, 64, 2) : make_tmap_kmajor(&tmB, B, p.R, p.K, ldb * 2, p.NR, 2)) return -3;
-  const int tiles = (p.M + kBlockM - 1) / kBlockM, blocks = (p.R + p.NR - 1) / p.NR, num_kb = (p.K + 63) / 64;
+  const int stages = budget / stage > 8 ? 8 : budget / stage;
+  const int smem = (stages * stage > sums ? stages * stage : sums) + 1024;
+  ThinMaps maps[2];
+  int tiles = 0;
+  for (int i = 0; i < count; ++i) {
+    ThinParams& p = q[i].p;
+    if (p.R != f.R || p.K != f.K || (p.lo_in > 0) != (f.lo_in > 0)) return -6;
+    p.NR = NR;
+    p.stages = stages;
+    p.tiles = (p.M + kBlockM - 1) / kBlockM;
+    tiles += p.tiles;
+    if (A_MN ? make_tmap_kmajor(&maps[i].A, q[i].A, p.K, p.M, q[i].lda * 2, 64, 2) : make_tmap_kmajor(&maps[i].A, q[i].A, p.M, p.K, q[i].lda * 2, kBlockM, 2)) return -2;
+    if (B_MN ? make_tmap_kmajor(&maps[i].B, q[i].B, p.K, halves ? p.lo_in + p.R : p.R, q[i].ldb * 2, 64, 2) : make_tmap_kmajor(&maps[i].B, q[i].B, p.R, p.K, q[i].ldb * 2, NR, 2))
+      return -3;
+  }
+  if (count == 1) maps[1] = maps[0];
+  const int blocks = (f.R + NR - 1) / NR, num_kb = (f.K + 63) / 64;
   int S = split;
   if (S <= 0) {
     // CTAs for every SM; clusters of eight only where four leave half of the chip idle (they are harder to place, and sum over more CTAs).
@@ -248,7 +277,7 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
     if (S == 4 && whole * S < 74 && num_kb >= 32) S = 8;
   }
   if (S > 8 || S > num_kb || (S & (S - 1)) || tiles > 65535 || blocks > 65535) return -4;
-  auto kern = thin_kernel<A_MN, B_MN, TRANS>;
+  auto kern = thin_kernel<A_MN, B_MN>;
   PRL_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kThinSmemMax));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(S, blocks, tiles);
@@ -263,7 +292,7 @@ static int run_thin(const void* A, const void* B, ThinParams p, int64_t lda, int
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  PRL_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, static_cast<const ThinParams>(p)));
+  PRL_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], q[0].p, q[count - 1].p));
   PRL_CUDA_CHECK(cudaGetLastError());
   return 0;
 }
@@ -315,14 +344,24 @@ extern "C" int prl_lora_thin(const void* A, const void* B, void* out, int M, int
                              int lo_out, int lo_in, int split, cudaStream_t stream) {
   if (M <= 0 || R <= 0 || K <= 0) return 0;
   if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || lo_out % 8 || lo_in % 8 || (layout != 3 && ldo % 4) || (layout == 3 && lo_out) || (layout == 0 && lo_in)) return -1;
-  const ThinParams p{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad, lo_out, lo_in, nullptr, nullptr, 1};
+  ThinProduct q{A, B, lda, ldb, ThinParams{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, scale, pad, lo_out, lo_in, nullptr, nullptr, 1, layout == 3, 0}};
   switch (layout) {
-    case 0: return run_thin<false, false, false>(A, B, p, lda, ldb, split, stream);
-    case 1: return run_thin<false, true, false>(A, B, p, lda, ldb, split, stream);
-    case 2: return run_thin<true, true, false>(A, B, p, lda, ldb, split, stream);
-    case 3: return run_thin<true, true, true>(A, B, p, lda, ldb, split, stream);
+    case 0: return run_thin<false, false>(&q, 1, split, stream);
+    case 1: return run_thin<false, true>(&q, 1, split, stream);
+    case 2:
+    case 3: return run_thin<true, true>(&q, 1, split, stream);
   }
   return -5;
+}
+
+// Both gradients of an adapter in one launch, over the same K rows: da [R, M1] = dt^T x, x [K, M1], dt [K, ..] with its halves R and R + lo_dt on; db [M2, R] = dy^T t
+extern "C" int prl_lora_grads(const void* x, const void* dt, void* da, const void* dy, const void* t, void* db, int M1, int M2, int R, int K, int64_t ldx, int64_t lddt,
+                              int64_t lddy, int64_t ldt, int lo_dt, int lo_t, int split, cudaStream_t stream) {
+  if (M1 <= 0 || M2 <= 0 || R <= 0 || K <= 0) return -1;
+  if (R % 8 || ldx % 8 || lddt % 8 || lddy % 8 || ldt % 8 || lo_dt % 8 || lo_t % 8 || lo_dt <= 0 || lo_t <= 0) return -1;
+  ThinProduct q[2] = {{dy, t, lddy, ldt, ThinParams{static_cast<__nv_bfloat16*>(db), R, M2, R, K, 0, 0, 1.f, 0, 0, lo_t, nullptr, nullptr, 1, 0, 0}},
+                      {x, dt, ldx, lddt, ThinParams{static_cast<__nv_bfloat16*>(da), M1, M1, R, K, 0, 0, 1.f, 0, 0, lo_dt, nullptr, nullptr, 1, 1, 0}}};
+  return run_thin<true, true>(q, 2, split, stream);
 }
 
 // layout 0 for rows whose adapters differ: B [adapters * each, K], out [M, adapters * each (+ pad)], see ThinParams
@@ -330,7 +369,8 @@ extern "C" int prl_adapter_thin(const void* A, const void* B, void* out, int M, 
                                 const float* scales, int each, cudaStream_t stream) {
   if (M <= 0 || R <= 0 || K <= 0) return 0;
   if (R % 8 || lda % 8 || ldb % 8 || pad % 8 || ldo % 4 || each < 4 || each % 4 || R % each) return -1;
-  return run_thin<false, false, false>(A, B, ThinParams{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, 1.f, pad, 0, 0, ids, scales, each}, lda, ldb, 0, stream);
+  ThinProduct q{A, B, lda, ldb, ThinParams{static_cast<__nv_bfloat16*>(out), ldo, M, R, K, 0, 0, 1.f, pad, 0, 0, ids, scales, each, 0, 0}};
+  return run_thin<false, false>(&q, 1, 0, stream);
 }
 
 namespace prl {

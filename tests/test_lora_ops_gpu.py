@@ -60,6 +60,24 @@ def test_lora_linear_swiglu(t, k, f, ranks):
     check_lora(lora_case(t, k, (f, f), ranks, t, BF, "cuda", swiglu=True))
 
 
+@pytest.mark.parametrize("t,k,n,r,pad", [(1, 8, 8, 8, 0), (70, 72, 520, 8, 8), (130, 1032, 136, 48, 0), (515, 256, 384, 136, 8), (300, 136, 2048, 264, 0)])
+def test_both_gradients_in_one_launch(t, k, n, r, pad):
+    """The same values as each product by itself, split the same way."""
+    g = torch.Generator().manual_seed(t + k)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    x, dy, dt, low = rnd(t, k), rnd(t, n), rnd(t, 2 * r), rnd(t, 2 * r + pad)
+    C = ops.ext()
+    for split in (1, 2):
+        if split > (t + 63) // 64:
+            continue
+        da, db = C.lora_grads(x, dt, dy, low, r, r + pad, split)
+        assert torch.equal(da, C.lora_thin(x, dt, 3, 1.0, r, 0, False, r, split)) and torch.equal(db, C.lora_thin(dy, low, 2, 1.0, r, 0, False, r + pad, split))
+    da, db = C.lora_grads(x, dt, dy, low, r, r + pad)
+    both = lambda v, lo: v[:, :r].double() + v[:, lo:lo + r].double()  # noqa: E731
+    for got, a, b in ((da, both(dt, r), x.double()), (db, dy.double(), both(low, r + pad))):
+        check_near(got, a.t() @ b, (2 * t + 4) * 2.0 ** -24 * (a.abs().t() @ b.abs()) * (1 + 2.0 ** -7))
+
+
 @pytest.mark.parametrize("t,k,f,r", [(1, 64, 128, 8), (300, 264, 256, 24), (700, 2048, 384, 16)])
 def test_saved_projection_has_sixteen_bits_of_mantissa(t, k, f, r):
     """Gate and up as the backward gets them: truncated to 24 bits (2^-16); values that are not finite stay what they are."""

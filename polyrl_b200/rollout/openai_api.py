@@ -105,7 +105,7 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
         n = max(1, int(body.get("n") or 1))
         adapter = srv.adapter_of(body.get("model"))
         srv.check_request(sp, adapter)
-    except (ValueError, TypeError, KeyError, AttributeError) as e:
+    except (ValueError, TypeError, KeyError, AttributeError, OverflowError) as e:
         h._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})
         return
     room = srv.engine.max_model_len - 1

@@ -221,7 +221,7 @@ class EngineServer:
         try:
             sp = SamplingParams.from_dict(body.get("sampling_params") or {})
             self.check_request(sp, adapter)
-        except (ValueError, TypeError, AttributeError) as e:
+        except (ValueError, TypeError, AttributeError, OverflowError) as e:
             h._json(400, {"error": str(e)})
             return
         stream = bool(body.get("stream", False))

@@ -307,3 +307,17 @@ def test_server_routes(tmp_path):
         assert post("/unload_lora_adapter", {"lora_name": "mine"})[0] == 200 and post("/unload_lora_adapter", {"lora_name": "mine"})[0] == 400
     finally:
         srv.stop()
+
+
+def test_server_refuses_what_is_no_number():
+    from polyrl_b200.rollout.server import EngineServer
+
+    srv = EngineServer(make_engine()[2]).start()
+    try:
+        for sp in ({"min_new_tokens": float("inf")}, {"allowed_token_ids": [float("inf")]}, {"logit_bias": {"x": 1}}, {"logit_bias": [3]}, {"presence_penalty": "high"}):
+            req = urllib.request.Request(f"http://{srv.endpoint}/generate", json.dumps({"input_ids": [5, 6], "sampling_params": sp}).encode(), {"Content-Type": "application/json"})
+            with pytest.raises(urllib.error.HTTPError) as e:
+                urllib.request.urlopen(req, timeout=60)
+            assert e.value.code == 400
+    finally:
+        srv.stop()

@@ -56,12 +56,12 @@ class RequestRules:
         self.version = 0                 # of the tensors: graphs captured over others are stale
 
     # ------------------------------------------------------------------ slots
-    def _wide(self, t, need: int, fill):
-        """Rows of at least ``need`` columns, what is there kept; None as long as nothing is needed."""
+    def _wide(self, t, need: int, fill, most: int = 1 << 30):
+        """Rows of at least ``need`` columns, of ``most`` at most, what is there kept; None as long as nothing is needed."""
         have = 0 if t is None else t.shape[1]
         if need <= have:
             return t
-        new = torch.full((self.slots, max(8, 1 << (need - 1).bit_length())), fill, dtype=torch.float32 if fill == 0.0 and isinstance(fill, float) else torch.int32,
+        new = torch.full((self.slots, min(most, max(8, 1 << (need - 1).bit_length()))), fill, dtype=torch.float32 if fill == 0.0 and isinstance(fill, float) else torch.int32,
                          device=self.device)
         if have:
             new[:, :have] = t
@@ -76,9 +76,10 @@ class RequestRules:
         self.lens[slot], self.prompt_lens[slot] = n, prompt_len
         self.repetition[slot], self.presence[slot], self.frequency[slot] = p.repetition_penalty, p.presence_penalty, p.frequency_penalty
         if p.logit_bias:
-            self.bias_ids, self.bias_values = self._wide(self.bias_ids, len(p.logit_bias), -1), self._wide(self.bias_values, len(p.logit_bias), 0.0)
-            self.bias_ids[slot, :len(p.logit_bias)] = torch.tensor([int(t) for t in p.logit_bias], dtype=torch.int32).to(self.device)
-            self.bias_values[slot, :len(p.logit_bias)] = torch.tensor([float(v) for v in p.logit_bias.values()], dtype=torch.float32).to(self.device)
+            m = len(p.logit_bias)
+            self.bias_ids, self.bias_values = self._wide(self.bias_ids, m, -1, MAX_BIAS), self._wide(self.bias_values, m, 0.0, MAX_BIAS)
+            self.bias_ids[slot, :m] = torch.tensor([int(t) for t in p.logit_bias], dtype=torch.int32).to(self.device)
+            self.bias_values[slot, :m] = torch.tensor([float(v) for v in p.logit_bias.values()], dtype=torch.float32).to(self.device)
         stops = sorted(set(stop_ids))
         if p.min_new_tokens > 0 and stops:
             self.stop_ids = self._wide(self.stop_ids, len(stops), -1)

@@ -80,7 +80,7 @@ class RequestRules:
             self.bias_ids, self.bias_values = self._wide(self.bias_ids, m, -1, MAX_BIAS), self._wide(self.bias_values, m, 0.0, MAX_BIAS)
             self.bias_ids[slot, :m] = torch.tensor([int(t) for t in p.logit_bias], dtype=torch.int32).to(self.device)
             self.bias_values[slot, :m] = torch.tensor([float(v) for v in p.logit_bias.values()], dtype=torch.float32).to(self.device)
-        stops = sorted(set(stop_ids))
+        stops = sorted({int(t) for t in stop_ids if 0 <= t < self.vocab and t == int(t)})        # no other can be sampled
         if p.min_new_tokens > 0 and stops:
             self.stop_ids = self._wide(self.stop_ids, len(stops), -1)
             self.stop_ids[slot, :len(stops)] = torch.tensor(stops, dtype=torch.int32).to(self.device)

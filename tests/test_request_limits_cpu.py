@@ -49,3 +49,24 @@ def check_long_bias_lists(eng):
 
 def test_bias_lists_up_to_the_limit():
     check_long_bias_lists(make_engine()[2])
+
+
+def test_stop_tokens_outside_the_vocabulary():
+    """They cannot be sampled, so there is nothing to hold back; the ones inside still wait for the least length."""
+    from polyrl_b200.rollout.server import EngineServer
+
+    eng = make_engine()[2]
+    odd = (2 ** 31, 2 ** 63, VOCAB, -1, float("inf"), 7.5, 9)
+    r = eng.add_request([5, 6], SamplingParams(max_new_tokens=6, temperature=0.0, min_new_tokens=4, stop_token_ids=odd, logit_bias={9: 1e4, 7: 9e3, 8: 8e3}))
+    run(eng)
+    assert r.output_ids == [7, 7, 7, 7, 9] and r.finish_reason == "stop"
+    srv = EngineServer(eng).start()
+    try:
+        for stops in ([2 ** 31], [2 ** 40, 9]):
+            code, got = post(f"http://{srv.endpoint}/generate", {"input_ids": [5, 6], "sampling_params": {
+                "max_new_tokens": 3, "temperature": 0.0, "min_new_tokens": 1, "stop_token_ids": stops, "logit_bias": {"7": 1e4}}})
+            assert code == 200 and got["output_ids"] == [7, 7, 7]
+        code, got = post(f"http://{srv.endpoint}/generate", {"input_ids": [5, 6], "sampling_params": {"max_new_tokens": 3, "temperature": 0.0, "ignore_eos": True}})
+        assert code == 200 and len(got["output_ids"]) == 3
+    finally:
+        srv.stop()

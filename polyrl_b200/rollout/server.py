@@ -17,6 +17,7 @@ import os
 import queue
 import threading
 import time
+import traceback
 import urllib.request
 from http.server import BaseHTTPRequestHandler, ThreadingHTTPServer
 
@@ -27,6 +28,7 @@ class _Tracked:
     def __init__(self, req: Request, index: int):
         self.req, self.index = req, index
         self.sent = 0
+        self.error: str | None = None               # why the engine refused it in the middle
 
 
 class EngineServer:
@@ -50,6 +52,7 @@ class EngineServer:
         self._inbox: list = []                          # (kind, payload) commands for the engine thread
         self._streams: dict[str, tuple[queue.Queue, list[_Tracked]]] = {}
         self._stop = threading.Event()
+        self._broken: str | None = None                 # the engine can take no further step
         self._paused = threading.Event()
         self.weight_version = 0
         srv = self
@@ -71,7 +74,7 @@ class EngineServer:
             def do_GET(self):
                 path = self.path.split("?")[0]
                 if path in ("/health", "/health_generate"):
-                    self._json(200, {"status": "ok"})
+                    self._json(*(200, {"status": "ok"}) if srv._broken is None else (503, {"status": srv._broken}))
                 elif path == "/get_server_info":
                     info = srv.engine.server_info()
                     self._json(200, {"internal_states": [info], "weight_version": srv.weight_version})
@@ -206,9 +209,18 @@ class EngineServer:
         """Queue token-id prompts for the engine thread; events (index, payload, finished) arrive on the returned queue."""
         q: queue.Queue = queue.Queue()
         key = f"g{id(q)}"
+        if self._broken is not None:
+            self._decline(q, len(prompts), {"type": "abort", "message": self._broken})
+            return key, q
         with self._lock:
             self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter), None))
         return key, q
+
+    @staticmethod
+    def _decline(q, n: int, reason: dict, **more) -> None:
+        """The last events of n prompts that the engine has not taken."""
+        for i in range(n):
+            q.put((i, {**more, "text": "", "index": i, "output_ids": [], "meta_info": {"finish_reason": reason, "completion_tokens": 0, "output_token_logprobs": []}}, True))
 
     def _handle_generate(self, h, body: dict):
         ids = body.get("input_ids")
@@ -273,7 +285,7 @@ class EngineServer:
             fr = {"type": r.finish_reason}
             if r.finish_reason == "length":
                 fr["length"] = len(r.output_ids)
-        return {"text": "", "index": t.index, "output_ids": list(r.output_ids),
+        return {**({} if t.error is None else {"error": t.error}), "text": "", "index": t.index, "output_ids": list(r.output_ids),
                 "meta_info": {"id": r.rid, "finish_reason": fr, "prompt_tokens": len(r.prompt_ids),
                               "completion_tokens": len(r.output_ids),
                               "output_token_logprobs": [[lp, tok, None] for lp, tok in zip(r.logprobs, r.output_ids)]}}
@@ -320,6 +332,8 @@ class EngineServer:
                         if self.tp_cmd_group is not None:
                             _tp_broadcast(self.tp_cmd_group, wire + [("update_weights", body)], 0)
                             wire = []
+                        if self._broken is not None:
+                            raise RuntimeError(self._broken)
                         while eng.has_work() and not body.get("bootstrap"):
                             if self.tp_cmd_group is not None:
                                 _tp_broadcast(self.tp_cmd_group, [], 1)
@@ -341,21 +355,46 @@ class EngineServer:
                     if kind == "update_weights":
                         payload[1]["ok"], payload[1]["msg"] = False, repr(e)
                     elif kind == "generate" and payload[0] not in self._streams:      # refused: the caller must not wait for it
-                        for i in range(len(payload[1])):
-                            payload[3].put((i, {"index": i, "error": str(e), "output_ids": [], "meta_info": {"finish_reason": {"type": "abort"}}}, True))
+                        self._decline(payload[3], len(payload[1]), {"type": "abort"}, error=str(e))
                 finally:
                     if done is not None:
                         done.set()
-            do_step = eng.layer_w is not None and eng.has_work()
+            do_step = self._broken is None and eng.layer_w is not None and eng.has_work()
             if self.tp_cmd_group is not None and (wire or do_step):
                 _tp_broadcast(self.tp_cmd_group, wire, int(do_step))
             if do_step:
-                eng.step()
+                try:
+                    eng.step()
+                except Exception as e:
+                    self._step_failed(e)
+                    if self.tp_cmd_group is not None:      # the other ranks have failed as well, or are a step ahead: no lock-step to go on with
+                        self._broken = self._broken or f"engine failed: {e!r}"
+                        self._flush_streams()
+                        raise
                 self._flush_streams()
             else:
                 time.sleep(0.002)
         if self.tp_cmd_group is not None:
             _tp_broadcast(self.tp_cmd_group, [("shutdown", None)], 0)
+
+    def _step_failed(self, e: Exception) -> None:
+        """A step that raised ends the requests in flight, not the thread: each gets its last event with the tokens that it has.  A step that
+        refuses its arguments (ValueError) refuses what requests brought: those that brought something get an error, which nobody retries;
+        all others are aborted, so that they can be continued elsewhere."""
+        traceback.print_exc()
+        eng = self.engine
+        flying = [t for _, tracked in self._streams.values() for t in tracked if not t.req.finished]
+        try:
+            eng.abort(abort_all=True)
+        except Exception:                                  # noqa: BLE001  the device is gone: nothing can be given back, and nothing will run
+            traceback.print_exc()
+            self._broken = f"engine failed: {e!r}"
+            for t in flying:
+                t.req.finish_reason = t.req.finish_reason or "abort"
+        for t in flying:
+            brought = getattr(t.req.params, "has_rules", False) or t.req.adapter >= 0
+            if isinstance(e, ValueError) and brought and t.req.finish_reason == "abort":
+                t.error = str(e)
 
     def _flush_streams(self) -> None:
         for key in list(self._streams):

@@ -70,3 +70,74 @@ def test_stop_tokens_outside_the_vocabulary():
         assert code == 200 and len(got["output_ids"]) == 3
     finally:
         srv.stop()
+
+
+def stream(srv, body, timeout=60):
+    """The last payload of every index of a streamed /generate."""
+    req = urllib.request.Request(f"http://{srv.endpoint}/generate", json.dumps({**body, "stream": True}).encode(), {"Content-Type": "application/json"})
+    last = {}
+    with urllib.request.urlopen(req, timeout=timeout) as r:
+        for line in r:
+            if line.startswith(b"data: {"):
+                p = json.loads(line[6:])
+                last[p["index"]] = p
+    return last
+
+
+@pytest.mark.parametrize("error", [ValueError, RuntimeError])
+def test_a_step_that_fails_ends_its_requests_and_not_the_server(error):
+    import threading
+
+    from polyrl_b200.rollout.server import EngineServer
+
+    eng = make_engine()[2]
+    real, fail = eng.step, threading.Event()
+
+    def step():
+        if fail.is_set() and any(r.params.has_rules and len(r.output_ids) > 3 for r in eng.running.values()):
+            fail.clear()
+            raise error("no such step")
+        return real()
+
+    eng.step = step
+    srv = EngineServer(eng, stream_interval=1).start()
+    try:
+        fail.set()
+        sp = {"max_new_tokens": 60, "temperature": 0.0, "ignore_eos": True}
+        out = [None, None]
+        ts = [threading.Thread(target=lambda i=i, more=more: out.__setitem__(i, stream(srv, {"input_ids": [5, 6], "sampling_params": {**sp, **more}})[0]))
+              for i, more in enumerate([{}, {"presence_penalty": 1.0}])]
+        [t.start() for t in ts]
+        [t.join(60) for t in ts]
+        plain, ruled = out
+        assert ruled["meta_info"]["finish_reason"]["type"] == "abort" and len(ruled["output_ids"]) > 3
+        assert ("error" in ruled) == (error is ValueError) and "error" not in plain        # what is in the middle can go on elsewhere
+        assert len(plain["output_ids"]) == plain["meta_info"]["completion_tokens"] == len(plain["meta_info"]["output_token_logprobs"])
+        assert not eng.has_work() or not eng.running
+        code, got = post(f"http://{srv.endpoint}/generate", {"input_ids": [5, 6], "sampling_params": {**sp, "presence_penalty": 1.0}})
+        assert code == 200 and len(got["output_ids"]) == 60
+        assert urllib.request.urlopen(f"http://{srv.endpoint}/health_generate", timeout=30).status == 200
+    finally:
+        srv.stop()
+
+
+def test_an_engine_that_cannot_go_on_says_so():
+    from polyrl_b200.rollout.server import EngineServer
+
+    eng = make_engine()[2]
+
+    def gone(*a, **k):
+        raise RuntimeError("the device is gone")
+
+    eng.step = eng.abort = gone
+    srv = EngineServer(eng).start()
+    try:
+        for _ in range(2):
+            code, got = post(f"http://{srv.endpoint}/generate", {"input_ids": [5, 6], "sampling_params": {"max_new_tokens": 4}})
+            assert code == 200 and got["meta_info"]["finish_reason"]["type"] == "abort" and got["output_ids"] == []
+        with pytest.raises(urllib.error.HTTPError) as e:
+            urllib.request.urlopen(f"http://{srv.endpoint}/health_generate", timeout=30)
+        assert e.value.code == 503
+        assert post(f"http://{srv.endpoint}/update_weights_from_agent", {"weight_version": 3})[0] == 500
+    finally:
+        srv.stop()

@@ -3,7 +3,8 @@
 // same scheduling semantics:
 //   * per-stats-tick admission quota + round-robin among engines whose queue is empty, otherwise park
 //   * token-level fault-tolerant continuation: on stream failure / abort keep the partial generation, evict
-//     the (remote) engine, append the generated tokens to the prompt, shrink max_new_tokens, re-dispatch (<=5x)
+//     the (remote) engine, append the generated tokens to the prompt, shrink max_new_tokens, re-dispatch (<=5x);
+//     a request that an engine refuses (HTTP 4xx) is its caller's fault: answered, not retried, no engine is evicted
 //   * time-boxed generation on colocated ("local") engines, then abort-all and continue remotely
 //   * weight-version protocol (update_weight_version / get_receive_instances CAS / update_weights activate)
 //   * load-balance controller fed by /update_metrics
@@ -238,8 +239,12 @@ static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json b
   std::vector<Json> latest(n_sub);
   std::vector<bool> got(n_sub, false);
   bool done = false, aborted = false, decode_err = false;
+  std::string plain;                 // what an answer without events says
   auto on_line = [&](const std::string& line) -> bool {
-    if (line.rfind("data:", 0) != 0) return true;
+    if (line.rfind("data:", 0) != 0) {
+      if (plain.size() < 4096) plain += line;
+      return true;
+    }
     std::string payload = line.substr(5);
     payload.erase(0, payload.find_first_not_of(' '));
     if (payload == "[DONE]") { done = true; return false; }
@@ -267,6 +272,14 @@ static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json b
     }
     return build_final_response(cur, accumulated);
   };
+  if (r.status >= 400 && r.status < 500 && r.status != 404 && r.status != 408 && r.status != 429) {
+    // The request is at fault, not the engine: any other would answer the same.
+    Json answer;
+    err.status = r.status; err.error_type = "refused";
+    err.error = Json::try_parse(plain, answer) && answer["error"].is_string() ? answer["error"].as_string() : "engine returned HTTP " + std::to_string(r.status);
+    err.partial = partial_json();
+    return false;
+  }
   if (r.status != 0 && r.status != 200) {
     err.status = 502; err.error_type = "request_error";
     err.error = "engine returned HTTP " + std::to_string(r.status);

@@ -240,6 +240,7 @@ static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json b
   std::vector<bool> got(n_sub, false);
   bool done = false, aborted = false, decode_err = false;
   std::string plain;                 // what an answer without events says
+  std::string refusal;               // an event with an error: the engine took the request and then refused it
   auto on_line = [&](const std::string& line) -> bool {
     if (line.rfind("data:", 0) != 0) {
       if (plain.size() < 4096) plain += line;
@@ -253,6 +254,7 @@ static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json b
     size_t idx = is_batch ? static_cast<size_t>(chunk["index"].as_int(0)) : 0;
     if (idx >= n_sub) return true;
     if (chunk.at_path({"meta_info", "finish_reason", "type"}).as_string() == "abort") aborted = true;
+    if (const Json* e = chunk.find("error"); e && e->is_string()) refusal = e->as_string().empty() ? "refused by the engine" : e->as_string();
     latest[idx] = std::move(chunk);
     got[idx] = true;
     return true;
@@ -285,6 +287,7 @@ static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json b
     err.error = "engine returned HTTP " + std::to_string(r.status);
     return false;
   }
+  if (!refusal.empty()) { err.status = 400; err.error_type = "refused"; err.error = refusal; err.partial = partial_json(); return false; }
   if (decode_err) { err.error_type = "decode_error"; err.error = "bad SSE chunk"; err.partial = partial_json(); return false; }
   if (!done) {
     err.error_type = r.error_type.empty() ? "connection_error" : r.error_type;

@@ -149,7 +149,17 @@ def handle_openai(srv, h, body: dict, chat: bool) -> None:
                         ch = {"index": ci, "delta": {"content": delta}, "finish_reason": None} if chat else {"index": ci, "text": delta, "finish_reason": None}
                         write({**base, "object": obj + ".chunk" if chat else obj, "choices": [ch]})
                 if "error" in payload:                              # refused by the engine after it was queued
-                    raise ConnectionAbortedError(payload["error"])
+                    for key, _ in keys_qs:
+                        srv._command("abort_key", key)
+                    err = {"error": {"message": payload["error"], "type": "invalid_request_error"}}
+                    if not stream:
+                        h._json(400, err)
+                        return
+                    write(err)
+                    write("[DONE]")
+                    h.wfile.write(b"0\r\n\r\n")
+                    h.wfile.flush()
+                    return
                 if fin and final[ci] is None:
                     final[ci] = payload
                     pending[pi] -= 1

@@ -272,7 +272,8 @@ class EngineServer:
                 h.wfile.write(b"0\r\n\r\n")
                 h.wfile.flush()
             else:
-                h._json(200, latest if batch else latest[0])
+                refused = next((p["error"] for p in latest if "error" in p), None)          # by the engine, after it was queued
+                h._json(*(200, latest if batch else latest[0]) if refused is None else (400, {"error": refused}))
         except (BrokenPipeError, ConnectionResetError, OSError, queue.Empty):
             self._command("abort_key", key)
 
@@ -355,7 +356,7 @@ class EngineServer:
                     if kind == "update_weights":
                         payload[1]["ok"], payload[1]["msg"] = False, repr(e)
                     elif kind == "generate" and payload[0] not in self._streams:      # refused: the caller must not wait for it
-                        self._decline(payload[3], len(payload[1]), {"type": "abort"}, error=str(e))
+                        self._decline(payload[3], len(payload[1]), {"type": "abort"}, error=str(e) or repr(e))
                 finally:
                     if done is not None:
                         done.set()
@@ -394,7 +395,7 @@ class EngineServer:
         for t in flying:
             brought = getattr(t.req.params, "has_rules", False) or t.req.adapter >= 0
             if isinstance(e, ValueError) and brought and t.req.finish_reason == "abort":
-                t.error = str(e)
+                t.error = str(e) or repr(e)
 
     def _flush_streams(self) -> None:
         for key in list(self._streams):

@@ -77,3 +77,38 @@ def test_an_engine_that_fails_is_still_left_for_another(manager):
         assert ready(m) == 1 and bad.shutdown_called.wait(5)
     finally:
         bad.stop(); fine.stop()
+
+
+def test_a_request_refused_after_it_was_queued(manager):
+    """An adapter may be unloaded between a request's check and its turn: the same answer, over every route."""
+    import urllib.request
+
+    from polyrl_b200.data.rl_dataset import ByteTokenizer
+
+    m = manager
+    servers = [EngineServer(make_engine(max_adapters=1)[2], stream_interval=2, tokenizer=ByteTokenizer(), model_name="tiny").start() for _ in range(2)]
+    try:
+        join_remote(m, [s.port for s in servers])
+        for s in servers:
+            s.check_request = lambda sp, adapter: None            # it was there when the request came in
+            s.adapter_of = lambda name: name if name == "gone" else None
+        req = {"input_ids": [5, 6], "lora_path": "gone", "sampling_params": {"max_new_tokens": 4, "ignore_eos": True}}
+        for body in (req, {**req, "input_ids": [[5, 6]] * 2}):
+            code, got = _http("POST", m.url + "/generate", body)
+            assert code == 400 and json.loads(got)["error_type"] == "refused" and "gone" in json.loads(got)["error"]
+            code, got = _http("POST", f"http://{servers[0].endpoint}/generate", body)
+            assert code == 400 and "gone" in json.loads(got)["error"]
+        for n in (1, 3):
+            code, got = _http("POST", f"http://{servers[0].endpoint}/v1/completions", {"model": "gone", "prompt": "abc", "max_tokens": 4, "n": n})
+            assert code == 400 and "gone" in json.loads(got)["error"]["message"]
+            r = urllib.request.Request(f"http://{servers[0].endpoint}/v1/completions", json.dumps({"model": "gone", "prompt": "abc", "n": n, "stream": True}).encode(),
+                                       {"Content-Type": "application/json"})
+            with urllib.request.urlopen(r, timeout=60) as f:
+                events = [line[6:].strip() for line in f if line.startswith(b"data: ")]
+            assert "gone" in json.loads(events[0])["error"]["message"] and events[-1] == b"[DONE]"
+        good = {"input_ids": [5, 6], "sampling_params": {"max_new_tokens": 4, "temperature": 0.0, "ignore_eos": True}}
+        assert len(_tokens(json.loads(_http("POST", m.url + "/generate", good)[1]))) == 4
+        assert ready(m) == 2 and not any(s._stop.is_set() for s in servers)
+    finally:
+        for s in servers:
+            s.stop()

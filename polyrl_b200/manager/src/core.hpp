@@ -86,14 +86,17 @@ inline void trim_response_to_used_tokens(Json& resp, size_t used) {
   if (resp.is_array()) for (auto& r : resp.arr()) trim_one(r); else trim_one(resp);
 }
 
-// Shrink max_new_tokens by what was already generated.  For a grouped request (n samples in one body) all
+// Shrink max_new_tokens and min_new_tokens by what was already generated.  For a grouped request (n samples in one body) all
 // samples are truncated to the SHORTEST partial so the group stays aligned.
 inline void adjust_sampling_params_for_used_tokens(Json& sampling_params, Json& prev_response) {
-  if (!sampling_params["max_new_tokens"].is_number()) return;
-  int64_t max_new = sampling_params["max_new_tokens"].as_int();
-  size_t used = count_output_tokens(prev_response, /*sum=*/false);
+  Json *most = sampling_params.find("max_new_tokens"), *least = sampling_params.find("min_new_tokens");
+  if (most && !most->is_number()) most = nullptr;
+  if (least && !least->is_number()) least = nullptr;
+  if (!most && !least) return;
+  const size_t used = count_output_tokens(prev_response, /*sum=*/false);
   trim_response_to_used_tokens(prev_response, used);
-  sampling_params["max_new_tokens"] = std::max<int64_t>(0, max_new - static_cast<int64_t>(used));
+  for (Json* n : {most, least})
+    if (n) *n = std::max<int64_t>(0, n->as_int() - static_cast<int64_t>(used));
 }
 
 // Append the token ids already generated (2nd element of each logprob triple) to the prompt(s).
@@ -111,6 +114,17 @@ inline void extend_input_ids_with_response_tokens(Json& input_ids, const Json& p
   } else {
     append(input_ids, prev_response);
   }
+}
+
+// How many of each prompt's last tokens are such output (one number, or one a prompt of a batch): rules on a request's output
+// (penalties) go on over them.
+inline Json count_continued_tokens(const Json& input_ids, const Json& prev_response) {
+  const bool batch = input_ids.size() > 0 && input_ids[static_cast<size_t>(0)].is_array();
+  if (!batch) return Json(static_cast<int64_t>(count_single_response_tokens(prev_response)));
+  Json out = Json::array();
+  for (size_t i = 0; i < input_ids.size(); ++i)
+    out.push_back(Json(static_cast<int64_t>(prev_response.is_array() && i < prev_response.size() ? count_single_response_tokens(prev_response[i]) : 0)));
+  return out;
 }
 
 // ------------------------------------------------------------------------------------------ CIDR

@@ -3,7 +3,7 @@
 // same scheduling semantics:
 //   * per-stats-tick admission quota + round-robin among engines whose queue is empty, otherwise park
 //   * token-level fault-tolerant continuation: on stream failure / abort keep the partial generation, evict
-//     the (remote) engine, append the generated tokens to the prompt, shrink max_new_tokens, re-dispatch (<=5x);
+//     the (remote) engine, append the generated tokens to the prompt, shrink max_new_tokens and min_new_tokens, re-dispatch (<=5x);
 //     a request that an engine refuses (HTTP 4xx) is its caller's fault: answered, not retried, no engine is evicted
 //   * time-boxed generation on colocated ("local") engines, then abort-all and continue remotely
 //   * weight-version protocol (update_weight_version / get_receive_instances CAS / update_weights activate)
@@ -232,7 +232,10 @@ struct GenError {
 static bool collect_streaming_response(AppState& st, const InstPtr& inst, Json body, const Json* accumulated, Json& out,
                                        GenError& err) {
   body["stream"] = true;
-  if (accumulated && !accumulated->is_null()) extend_input_ids_with_response_tokens(body["input_ids"], *accumulated);
+  if (accumulated && !accumulated->is_null()) {
+    extend_input_ids_with_response_tokens(body["input_ids"], *accumulated);
+    body["continued_tokens"] = count_continued_tokens(body["input_ids"], *accumulated);
+  }
   const Json& ids = body["input_ids"];
   const bool is_batch = ids.is_array() && ids.size() > 0 && ids[static_cast<size_t>(0)].is_array();
   const size_t n_sub = is_batch ? ids.size() : 1;
@@ -317,7 +320,8 @@ static bool process_single_generate_request(AppState& st, const Json& original, 
     Json body = original;
     if (!accumulated.is_null()) {
       adjust_sampling_params_for_used_tokens(body["sampling_params"], accumulated);
-      if (body["sampling_params"]["max_new_tokens"].is_number() && body["sampling_params"]["max_new_tokens"].as_int() <= 0) {
+      const Json& left = static_cast<const Json&>(body).at_path({"sampling_params", "max_new_tokens"});
+      if (left.is_number() && left.as_int() <= 0) {
         inst->pending.fetch_sub(1);
         out = accumulated;      // budget exhausted by the partial: it is the final answer
         return true;

@@ -97,6 +97,7 @@ class Request:
     state_slot: int = 0                    # recurrent-state slot (mixer stacks), 0 = none
     fed: bool = False                      # tokens are supplied step by step (RolloutEngine.extend), nothing is sampled
     adapter: int = -1                      # place in the engine's adapter bank (models/lora.py), -1 = the plain model
+    continued: int = 0                     # the prompt's last tokens that an earlier part of this request has sampled
 
     @property
     def decoding(self) -> bool:
@@ -600,10 +601,14 @@ class RolloutEngine:
         self.adapters.unload(name)
 
     def add_request(self, prompt_ids: list[int], params: SamplingParams | dict | None = None, rid: str | None = None,
-                    group=None, mm: dict | None = None, adapter: str | None = None) -> Request:
+                    group=None, mm: dict | None = None, adapter: str | None = None, continued: int = 0) -> Request:
+        """``continued``: so many of the prompt's last tokens are output of the same request, from a part of it that was cut short: rules on
+        its output go on over them (``params`` hold what is left of its lengths)."""
         if not isinstance(params, SamplingParams):
             params = SamplingParams.from_dict(params)
         self.check_request(params, adapter)
+        if not 0 <= continued <= len(prompt_ids):
+            raise ValueError(f"{continued} continued tokens in a prompt of {len(prompt_ids)}")
         mrope_pos, mrope_delta = None, 0
         if mm is not None:
             from ..models import vision as V
@@ -623,7 +628,8 @@ class RolloutEngine:
         if params.max_new_tokens > budget:
             params = SamplingParams(**{**params.__dict__, "max_new_tokens": budget})
         r = Request(rid or f"r{next(self._rid)}", list(prompt_ids), params, t_arrival=time.time(), group=group, mm=mm,
-                    mrope_pos=mrope_pos, mrope_delta=mrope_delta, adapter=-1 if adapter is None else self.adapters.place(adapter))
+                    mrope_pos=mrope_pos, mrope_delta=mrope_delta, adapter=-1 if adapter is None else self.adapters.place(adapter),
+                    continued=min(continued, len(prompt_ids)))
         self.waiting.append(r)
         return r
 
@@ -894,7 +900,7 @@ class RolloutEngine:
             self.rules = RequestRules(self.max_num_seqs, self.max_model_len, vocab, self.device)
         version = self.rules.version
         for r in ruled:
-            self.rules.set(r.slot, r.params, r.prompt_ids + r.output_ids, len(r.prompt_ids), self._stop_ids(r.params))
+            self.rules.set(r.slot, r.params, r.prompt_ids + r.output_ids, len(r.prompt_ids), self._stop_ids(r.params), r.continued)
         if self.rules.version != version:                    # steps captured over tensors that have been replaced
             self._graphs = {k: g for k, g in self._graphs.items() if "rules" not in k}
         return torch.tensor([i for i, r in enumerate(reqs) if r.params.has_rules], dtype=torch.long, device=self.device)

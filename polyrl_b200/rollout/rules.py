@@ -68,12 +68,13 @@ class RequestRules:
         self.version += 1
         return new
 
-    def set(self, slot: int, p, history: list[int], prompt_len: int, stop_ids) -> None:
-        """Rules of the request that now has ``slot``; ``history``: its tokens so far, the first ``prompt_len`` of them its prompt."""
+    def set(self, slot: int, p, history: list[int], prompt_len: int, stop_ids, continued: int = 0) -> None:
+        """Rules of the request that now has ``slot``; ``history``: its tokens so far, the first ``prompt_len`` of them its prompt, whose last
+        ``continued`` ones count as output."""
         self.clear(slot)
         n = len(history)
         self.tokens[slot, :n] = torch.tensor(history, dtype=torch.int32).to(self.device)
-        self.lens[slot], self.prompt_lens[slot] = n, prompt_len
+        self.lens[slot], self.prompt_lens[slot] = n, prompt_len - continued
         self.repetition[slot], self.presence[slot], self.frequency[slot] = p.repetition_penalty, p.presence_penalty, p.frequency_penalty
         if p.logit_bias:
             m = len(p.logit_bias)

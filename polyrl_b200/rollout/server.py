@@ -205,15 +205,16 @@ class EngineServer:
         done.wait(timeout=600)
         return result.get("ok", False), result.get("msg", "timeout")
 
-    def submit(self, prompts: list[list[int]], sp: SamplingParams, mm=None, adapter: str | None = None) -> tuple[str, "queue.Queue"]:
-        """Queue token-id prompts for the engine thread; events (index, payload, finished) arrive on the returned queue."""
+    def submit(self, prompts: list[list[int]], sp: SamplingParams, mm=None, adapter: str | None = None, continued=None) -> tuple[str, "queue.Queue"]:
+        """Queue token-id prompts for the engine thread; events (index, payload, finished) arrive on the returned queue.  ``continued``: see
+        ``RolloutEngine.add_request``, one number a prompt."""
         q: queue.Queue = queue.Queue()
         key = f"g{id(q)}"
         if self._broken is not None:
             self._decline(q, len(prompts), {"type": "abort", "message": self._broken})
             return key, q
         with self._lock:
-            self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter), None))
+            self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter, continued), None))
         return key, q
 
     @staticmethod
@@ -233,6 +234,11 @@ class EngineServer:
         try:
             sp = SamplingParams.from_dict(body.get("sampling_params") or {})
             self.check_request(sp, adapter)
+            continued = body.get("continued_tokens")    # of a request that the manager continues: how much of each prompt is its output
+            if continued is not None:
+                continued = [int(n) for n in (continued if batch else [continued])]
+                if len(continued) != len(prompts) or any(not 0 <= n <= len(p) for n, p in zip(continued, prompts)):
+                    raise ValueError("continued_tokens: one number a prompt, up to its length")
         except (ValueError, TypeError, AttributeError, OverflowError) as e:
             h._json(400, {"error": str(e)})
             return
@@ -243,7 +249,7 @@ class EngineServer:
 
             img = body["image_data"]
             mm = [decode_mm_wire(d) if d is not None else None for d in img] if isinstance(img, list) else [decode_mm_wire(img)] * len(prompts)
-        key, q = self.submit(prompts, sp, mm, adapter)
+        key, q = self.submit(prompts, sp, mm, adapter, continued)
         n = len(prompts)
         latest = [None] * n
         if stream:
@@ -305,13 +311,13 @@ class EngineServer:
             for kind, payload, done in cmds:
                 try:
                     if kind == "generate":
-                        key, prompts, sp, q, mm, adapter = payload
+                        key, prompts, sp, q, mm, adapter, continued = payload
                         rids = []
                         for _ in prompts:
                             self._rid += 1
                             rids.append(f"s{self._rid}")
-                        wire.append(("generate", {"prompts": prompts, "sp": sp.__dict__, "rids": rids, "mm": mm}))
-                        tracked = [_Tracked(r, i) for i, r in enumerate(_add_group(eng, prompts, sp, rids, mm, adapter))]
+                        wire.append(("generate", {"prompts": prompts, "sp": sp.__dict__, "rids": rids, "mm": mm, "continued": continued}))
+                        tracked = [_Tracked(r, i) for i, r in enumerate(_add_group(eng, prompts, sp, rids, mm, adapter, continued))]
                         self._streams[key] = (q, tracked)
                     elif kind == "adapter":
                         what, body, result = payload
@@ -416,20 +422,22 @@ class EngineServer:
 
 
 # ---------------------------------------------------------------------------------------------- TP lock-step helpers
-def _add_group(eng: RolloutEngine, prompts, sp: SamplingParams, rids, mm=None, adapter: str | None = None) -> list[Request]:
+def _add_group(eng: RolloutEngine, prompts, sp: SamplingParams, rids, mm=None, adapter: str | None = None, continued=None) -> list[Request]:
     """Requests of one HTTP call; identical prompts (with the same image inputs) share their prompt KV as an n-sample group."""
     same_mm = mm is None or all(m is mm[0] for m in mm)
     tag = object() if len(prompts) > 1 and same_mm and all(p == prompts[0] for p in prompts) else None
-    kw = {} if adapter is None else {"adapter": adapter}
+    kws = [{} if adapter is None else {"adapter": adapter} for _ in prompts]
+    if sp.has_rules and continued is not None:            # nothing else goes by it
+        kws = [{**kw, "continued": n} for kw, n in zip(kws, continued)]
     return [eng.add_request(list(map(int, p)), sp, rid=rid, group=tag, mm=mm[i] if mm is not None else None, **kw)
-            for i, (p, rid) in enumerate(zip(prompts, rids))]
+            for i, (p, rid, kw) in enumerate(zip(prompts, rids, kws))]
 
 
 def _apply_wire(eng: RolloutEngine, kind: str, payload, weight_update_fn) -> bool:
     """Apply one broadcast command on an engine replica.  Returns False on shutdown."""
     if kind == "generate":
         _add_group(eng, payload["prompts"], SamplingParams(**{**payload["sp"], "stop_token_ids": tuple(payload["sp"].get("stop_token_ids", ()))}),
-                   payload["rids"], payload.get("mm"))
+                   payload["rids"], payload.get("mm"), continued=payload.get("continued"))
     elif kind == "abort_rids":
         for rid in payload:
             eng.abort(rid)

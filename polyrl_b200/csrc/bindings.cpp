@@ -4,6 +4,8 @@
 #include "bindings_common.hpp"
 #include "lora.hpp"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <algorithm>
 #include <cstdint>
 #include <string>
@@ -737,7 +739,6 @@ struct LoraFn : public torch::autograd::Function<LoraFn> {
   }
 
   static Grads backward(Ctx* ctx, Grads grads) {
-    const at::AutoGradMode once(false);              // no gradients of gradients
     const std::vector<int64_t> meta = ctx->saved_data["meta"].toIntVector();
     const bool swiglu = meta[0];
     const int64_t parts = meta[1];
@@ -756,6 +757,27 @@ struct LoraFn : public torch::autograd::Function<LoraFn> {
     if (want[2]) out[2] = grads[0].sum(0);
     if (want[3]) out[3] = grads[0];
     if (!deep) return out;
+    const bool graph = at::GradMode::is_enabled();   // create_graph: what follows has no gradients of its own, and says so when it is asked for them
+    {
+      const at::AutoGradMode once(false);
+      products(ctx, grads, swiglu, widths, ranks, want, out);
+    }
+    if (graph) {
+      Grads given;
+      for (int i = 0; i < kArgs; ++i)
+        if (i != 2 && i != 3 && out[i].defined()) given.push_back(out[i].detach().requires_grad_(true));
+      const auto node = std::make_shared<torch::autograd::DelayedError>("lora_linear and lora_linear_swiglu can be differentiated once only", given.size());
+      const Grads marked = (*node)(std::move(given));
+      size_t next = 0;
+      for (int i = 0; i < kArgs; ++i)
+        if (i != 2 && i != 3 && out[i].defined()) out[i] = marked[next++];
+    }
+    return out;
+  }
+
+  // the gradients that take products: of x, w and the adapters
+  static void products(Ctx* ctx, const Grads& grads, bool swiglu, const std::vector<int64_t>& widths, const std::vector<int64_t>& ranks, const bool (&want)[kArgs], Grads& out) {
+    const int64_t parts = widths.size();
     const Grads saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1];
     const at::Tensor dy = swiglu ? swiglu_bwd(saved[5], aligned_rows(grads[0], true), saved[6]) : aligned_rows(grads[0]);
@@ -766,7 +788,6 @@ struct LoraFn : public torch::autograd::Function<LoraFn> {
     if (want[1]) out[1] = gemm2_bf16(dy, x, true, true, c10::nullopt, c10::nullopt, 0);
     for (int64_t i = 0; i < 2 * parts; ++i)
       if (got[1 + i].has_value()) out[4 + i] = *got[1 + i];
-    return out;
   }
 };
 

@@ -85,27 +85,43 @@ struct SwigluParams {
   int64_t ldr = 0;
   uint8_t* L = nullptr;                  // LOW: [M, ldgu], the eight bits of the fp32 values behind GU's sixteen
 };
-// ADD: R is there.  LOW: GU and L are there, and GU holds the upper sixteen bits of fp32, so that the two are gate and up to 2^-16 (a NaN stays one).
+// ADD: R is there.  LOW: GU and L are there, and GU holds the upper sixteen bits of fp32 rounded to 24, so that the two are gate and up to 2^-16.
 template <bool ADD, bool LOW = false>
 struct EpiSwigluOf {
   using Params = SwigluParams;
-  // the middle bytes of four fp32 values
-  __device__ __forceinline__ static uint32_t low4(float a, float b, float c, float d) {
-    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0051), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0051), 0x5410);
+  // the middle bytes of four fp32 values, the upper halves of two
+  __device__ __forceinline__ static uint32_t low4(const uint32_t* u) { return __byte_perm(__byte_perm(u[0], u[1], 0x0051), __byte_perm(u[2], u[3], 0x0051), 0x5410); }
+  __device__ __forceinline__ static uint32_t high2(const uint32_t* u) { return __byte_perm(u[0], u[1], 0x7632); }
+  // N values rounded to their upper 24 bits (ties away from zero).  Where one of them is not finite, each is looked at: a NaN must not run over
+  // into the sign.
+  template <int N>
+  __device__ __forceinline__ static void round24(const float (&v)[N], uint32_t (&u)[N]) {
+    float zero = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      zero = fmaf(v[i], 0.f, zero);
+      u[i] = __float_as_uint(v[i]) + 0x80u;
+    }
+    if (zero != 0.f) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!isfinite(v[i])) u[i] = __float_as_uint(v[i]);
+    }
   }
-  __device__ __forceinline__ static uint32_t high2(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
   __device__ __forceinline__ static void save4(__nv_bfloat16* gu, uint8_t* low, const float4& v) {
-    *reinterpret_cast<uint2*>(gu) = make_uint2(high2(v.x, v.y), high2(v.z, v.w));
-    *reinterpret_cast<uint32_t*>(low) = low4(v.x, v.y, v.z, v.w);
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    uint32_t u[4];
+    round24(f, u);
+    *reinterpret_cast<uint2*>(gu) = make_uint2(high2(u), high2(u + 2));
+    *reinterpret_cast<uint32_t*>(low) = low4(u);
   }
   __device__ __forceinline__ static void save32(__nv_bfloat16* gu, uint8_t* low, const float (&v)[32]) {
+    uint32_t u[32];
+    round24(v, u);
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      st_v4(gu + i, make_int4(high2(v[i], v[i + 1]), high2(v[i + 2], v[i + 3]), high2(v[i + 4], v[i + 5]), high2(v[i + 6], v[i + 7])));
+    for (int i = 0; i < 32; i += 8) st_v4(gu + i, make_int4(high2(u + i), high2(u + i + 2), high2(u + i + 4), high2(u + i + 6)));
 #pragma unroll
-    for (int i = 0; i < 32; i += 16)
-      st_v4(low + i, make_int4(low4(v[i], v[i + 1], v[i + 2], v[i + 3]), low4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]), low4(v[i + 8], v[i + 9], v[i + 10], v[i + 11]),
-                               low4(v[i + 12], v[i + 13], v[i + 14], v[i + 15])));
+    for (int i = 0; i < 32; i += 16) st_v4(low + i, make_int4(low4(u + i), low4(u + i + 4), low4(u + i + 8), low4(u + i + 12)));
   }
   // v += 32 consecutive bf16 values
   __device__ __forceinline__ static void add32(float (&v)[32], const __nv_bfloat16* r) {

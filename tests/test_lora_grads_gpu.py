@@ -36,3 +36,17 @@ def test_a_second_gradient_is_refused(swiglu):
         (gr,) = torch.autograd.grad(ops.lora_linear(x.detach(), w.detach(), [(a.detach(), b.detach())], 0.5, residual=res).float().square().sum(), res, create_graph=True)
         (second,) = torch.autograd.grad(gr.float().sum(), res)
         assert torch.equal(second, torch.full_like(second, 2.0))
+
+
+@pytest.mark.parametrize("t,k,f", [(130, 64, 128), (300, 128, 512), (5, 256, 128)])
+def test_saved_projection_is_rounded(t, k, f):
+    """Sums of whole numbers that fp32 holds exactly (below 2^24): what is kept of them is the nearest 24-bit value, half of its last place off at most."""
+    g = torch.Generator().manual_seed(t)
+    whole = lambda *s: torch.randint(-200, 201, s, generator=g).to(BF).cuda()  # noqa: E731
+    x, w, low, b = whole(t, k), whole(2 * f, k), whole(t, 8), whole(2 * f, 8)
+    exact = x.double() @ w.double().t() + low.double() @ b.double().t()
+    assert (x.double().abs() @ w.double().abs().t() + low.double().abs() @ b.double().abs().t()).max() < 2 ** 24
+    _, gu, lo = ops.ext().lora_gemm_swiglu(x, w, low, b, True)
+    got = ((gu.view(torch.int16).int() << 16) | (lo.int() << 8)).view(torch.float32).double()
+    step = torch.exp2(torch.floor(torch.log2(exact.abs().clamp(min=1))) - 15)               # of 16 bits of mantissa, the leading one among them
+    assert ((got - exact).abs() <= step / 2).all() and ((got - exact).abs() > step / 4).any()

@@ -815,8 +815,12 @@ at::Tensor adapter_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tens
   prl::LoraPackParams p{};
   p.parts = widths.size();
   int64_t end = 0;
-  for (int i = 0; i < p.parts; ++i) p.ends[i] = end += widths[i];
-  TORCH_CHECK_VALUE(end == N && each == p.parts * rank && rank % 8 == 0 && rank > 0 && K % 8 == 0 && R <= 0x7ffffff && N <= 0x7fffffff &&
+  for (int i = 0; i < p.parts; ++i) {
+    TORCH_CHECK_VALUE(widths[i] > 0 && widths[i] % 32 == 0, "adapter_gemm: parts of a multiple of 32 columns");
+    p.ends[i] = end += widths[i];
+  }
+  // (what adapter_delta takes, no more: a call's shapes are good for any number of rows, or for none)
+  TORCH_CHECK_VALUE(end == N && each == p.parts * rank && rank >= 16 && rank % 16 == 0 && each <= 384 && K > 0 && K % 32 == 0 && R <= 0x7ffffff && N <= 0x7fffffff &&
                     (!swiglu || (p.parts == 2 && widths[0] == widths[1] && N % 256 == 0)) && w.size(0) == N && w.size(1) == K && x.dim() == 2 && x.size(1) == K,
                     "adapter_gemm: stacked adapters do not fit");
   TORCH_CHECK_VALUE(scales.device() == x.device() && scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 1 && scales.size(0) == L,

@@ -156,10 +156,12 @@ def adapter_linear_swiglu(x: torch.Tensor, wgu: torch.Tensor, a: torch.Tensor, b
     if n % 256:
         raise ValueError("adapter_linear_swiglu: gate and up in blocks of 128 rows each")
     widths = (n // 2, n // 2)
+    if not isinstance(wgu, fn.Fp8Weight) and wgu.dtype != x.dtype:
+        wgu = wgu.to(x.dtype)
     if not fn._is_kernel_tensor(x) or plan.buf is None or isinstance(wgu, fn.Fp8Weight) or fn._cublas():
         return _adapter_linear_swiglu(x, wgu, a, b, scales, plan, widths)
     _of_plan("adapter_linear_swiglu", a, plan)
-    if x.shape[0] > fn._SKINNY_MAX_ROWS and wgu.dtype == x.dtype and _together(a, b):
+    if x.shape[0] > fn._SKINNY_MAX_ROWS and _together(a, b):
         return _C().adapter_gemm(_rows(x), fn._g2_operand(wgu), a, b, scales, plan.ids, widths, True, None, None)
     x = _rows(x)
     d = _delta(x, a, b, scales, plan, widths, True)

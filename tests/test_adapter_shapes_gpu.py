@@ -4,7 +4,7 @@ import torch
 
 from polyrl_b200 import ops
 
-from .requests_oracle import check_near
+from .requests_oracle import adapters64, check_near, swiglu64
 from .test_requests_cpu import adapters_case
 from .test_requests_gpu import near64, run_adapters
 
@@ -27,3 +27,14 @@ def test_shapes_are_refused_for_any_number_of_rows(t, way, monkeypatch):
             ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], ops.adapter_plan(c["ids"], 2))
     c = adapters_case(t, 64, (64, 64, 64), 128, 2, 1, BF, "cuda")                    # the most that is taken
     check_near(run_adapters(c, (64, 64, 64), 2), *near64(c, (64, 64, 64)))
+
+
+@pytest.mark.parametrize("t", [3, *ROWS])
+def test_a_weight_of_another_type_is_converted(t):
+    c = adapters_case(t, 128, (256,), 16, 3, t, BF, "cuda")
+    assert torch.equal(run_adapters(dict(c, w=c["w"].float()), (256,), 3), run_adapters(c, (256,), 3))
+    c = adapters_case(t, 128, (256, 256), 16, 3, t, BF, "cuda", extra=False)
+    plan = ops.adapter_plan(c["ids"], 3)
+    y = ops.adapter_linear_swiglu(c["x"], c["w"].float(), c["a"], c["b"], c["scales"], plan)
+    assert torch.equal(y, ops.adapter_linear_swiglu(c["x"], c["w"], c["a"], c["b"], c["scales"], plan))
+    check_near(y, *swiglu64(*adapters64(**c, widths=(256, 256), interleaved=True)))

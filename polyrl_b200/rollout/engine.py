@@ -371,6 +371,7 @@ class RolloutEngine:
         self._step_count = 0
         self._top_k, self._top_p = -1, 1.0
         self._with_rules = self._with_adapters = False
+        self._bringing: dict[int, Request] = {}      # requests with rules or an adapter that have not ended: what a step looks at for them
         self.vision_w = None                         # VLM tower weights (set_vision_weights)
         self.stats = {"prefill_tokens": 0, "decode_tokens": 0, "steps": 0, "last_gen_throughput": 0.0}
         self._alloc_static()
@@ -630,6 +631,8 @@ class RolloutEngine:
         r = Request(rid or f"r{next(self._rid)}", list(prompt_ids), params, t_arrival=time.time(), group=group, mm=mm,
                     mrope_pos=mrope_pos, mrope_delta=mrope_delta, adapter=-1 if adapter is None else self.adapters.place(adapter),
                     continued=min(continued, len(prompt_ids)))
+        if params.has_rules or r.adapter >= 0:
+            self._bringing[id(r)] = r
         self.waiting.append(r)
         return r
 
@@ -1145,8 +1148,13 @@ class RolloutEngine:
     def _run_decode(self, bs: int, sample: bool = True) -> torch.Tensor:
         """One decode step, through its CUDA graph where there is one; returns the step's logits (overwritten by the next step)."""
         # what some request of the batch brings is part of the step, and of the graph; a batch without is the step without
-        self._with_rules = sample and any(r.params.has_rules and r.decoding for r in self.running.values())
-        self._with_adapters = sample and any(r.adapter >= 0 and r.decoding for r in self.running.values())
+        self._with_rules = self._with_adapters = False
+        for key, r in list(self._bringing.items()) if sample else ():
+            if r.finished:
+                del self._bringing[key]
+            elif r.decoding:
+                self._with_rules |= r.params.has_rules
+                self._with_adapters |= r.adapter >= 0
         if not self.use_cuda_graph or (sample and (self._top_k > 0 or self._top_p < 1.0)):
             # top-k / top-p go through the sort-based library sampler (host-seeded RNG): not captured into a graph
             return self._decode_body(bs, sample)

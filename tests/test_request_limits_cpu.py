@@ -141,3 +141,25 @@ def test_an_engine_that_cannot_go_on_says_so():
         assert post(f"http://{srv.endpoint}/update_weights_from_agent", {"weight_version": 3})[0] == 500
     finally:
         srv.stop()
+
+
+def test_steps_of_requests_without_rules_do_not_look_for_any(monkeypatch):
+    asked = [0]
+    has = SamplingParams.has_rules.fget
+
+    def counted(self):
+        asked[0] += 1
+        return has(self)
+
+    monkeypatch.setattr(SamplingParams, "has_rules", property(counted))
+    counts = []
+    for length in (4, 60):
+        eng = make_engine()[2]
+        asked[0] = 0
+        eng.generate([[5 + i, 6] for i in range(8)], SamplingParams(max_new_tokens=length, ignore_eos=True))
+        counts.append(asked[0])
+    assert counts[0] == counts[1]
+    r = eng.add_request([5, 6], SamplingParams(max_new_tokens=9, temperature=0.0, allowed_token_ids=(7,)))
+    eng.add_request([5, 6], SamplingParams(max_new_tokens=30, ignore_eos=True))
+    run(eng)
+    assert r.output_ids == [7] * 9 and not eng._bringing

@@ -258,6 +258,7 @@ class AdapterBank:
             raise NotImplementedError("adapters of requests for checkpoints whose rotary layout is permuted at load time")
         if not 1 <= capacity <= 1024 or not 1 <= max_rank <= 128:
             raise ValueError("1 to 1024 adapters of rank 1 to 128")
+        self.dtype = dtype
         self.cfg, self.capacity, self.rank = cfg, capacity, -(-max_rank // 16) * 16
         self.dims = _proj_dims(cfg)
         self.widths = {n: tuple(self.dims[p][0] for p in parts) for n, parts in self.PARTS.items()}
@@ -294,7 +295,7 @@ class AdapterBank:
         if len(sd) != len(source):
             raise ValueError(f"adapter {name!r}: {len(source) - len(sd)} of its {len(source)} tensors belong to no module that is adapted here")
         ranks = {t.shape[0] for n, t in sd.items() if n.endswith("_A")}
-        if len(ranks) != 1:
+        if len(ranks) != 1 or 0 in ranks:
             raise ValueError(f"adapter {name!r}: one rank for all of its modules expected, not {sorted(ranks)}")
         (rank,) = ranks
         if rank > self.rank:
@@ -307,11 +308,14 @@ class AdapterBank:
             want = (rank, self.dims[p][1]) if m == "A" else (self.dims[p][0], rank)
             if tuple(t.shape) != want or n[:-1] + "AB"[m == "A"] not in sd:
                 raise ValueError(f"adapter {name!r}: {n} is {tuple(t.shape)}, {want} and its partner expected")
-            if not torch.isfinite(t).all():
-                raise ValueError(f"adapter {name!r}: {n} is not finite")
+            if not torch.isfinite(t.to(self.dtype)).all():      # (as the stacks hold it: zeros of other requests' rows are multiplied by it)
+                raise ValueError(f"adapter {name!r}: {n} is not finite in {self.dtype}")
+        scale = (rank if alpha is None else float(alpha)) / (rank ** 0.5 if root else rank)
+        if not abs(scale) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"adapter {name!r}: a scale of {scale}")
         at = free[0]
         self._write(at, sd, rank)
-        self.scales[at] = (rank if alpha is None else float(alpha)) / (rank ** 0.5 if root else rank)
+        self.scales[at] = scale
         self.names[name] = at
         return at
 

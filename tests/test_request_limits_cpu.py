@@ -163,3 +163,28 @@ def test_steps_of_requests_without_rules_do_not_look_for_any(monkeypatch):
     eng.add_request([5, 6], SamplingParams(max_new_tokens=30, ignore_eos=True))
     run(eng)
     assert r.output_ids == [7] * 9 and not eng._bringing
+
+
+def test_adapters_that_the_bank_cannot_hold_are_refused():
+    """Finite as they come is not enough: what the bank's type makes infinite would reach other requests, as zero times infinity."""
+    from polyrl_b200.models.lora import AdapterBank
+
+    from .test_engine_requests_cpu import make_adapter
+
+    cfg = make_engine()[0]
+    sd = make_adapter(cfg, 8, 5)
+    key = "layers.1.lora.lora_o_proj_B"
+    for dtype, huge in ((torch.bfloat16, torch.float32), (torch.float32, torch.float64)):
+        bank = AdapterBank(cfg, 2, 16, "cpu", dtype)
+        for value in (torch.finfo(huge).max, -torch.finfo(huge).max, float("nan")):
+            bad = {**sd, key: torch.full_like(sd[key], value, dtype=huge)}
+            with pytest.raises(ValueError, match="not finite"):
+                bank.load("a", bad)
+        for alpha in (float("inf"), float("nan"), 1e300):
+            with pytest.raises(ValueError, match="scale"):
+                bank.load("a", sd, alpha)
+        with pytest.raises(ValueError, match="one rank"):
+            bank.load("a", {k: v[:0] if k.endswith("_A") else v[:, :0] for k, v in sd.items()})
+        assert not bank.names and not bank.scales.any() and not any(t.any() for layer in bank.layers for pair in layer.values() for t in pair)
+        bank.load("a", sd, 4.0)
+        assert bank.scales.tolist() == [0.5, 0.0]

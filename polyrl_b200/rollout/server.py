@@ -38,6 +38,8 @@ class EngineServer:
         # OpenAI-compatible text front-end (/v1/completions, /v1/chat/completions, /v1/models): needs a tokenizer; the token-id
         # /generate route the manager and the trainers use does not
         self.tokenizer, self.model_name, self.tool_parser = tokenizer, model_name or engine.full_cfg.name, tool_parser
+        if self.model_name in self.adapter_names():        # its requests would get the adapter
+            raise ValueError(f"an adapter has the served model's name {self.model_name!r}")
         # tensor-parallel serving: this object lives on TP rank 0; every scheduler iteration its command list is
         # broadcast over ``tp_cmd_group`` (a gloo group of the TP ranks) so that followers (``run_tp_follower``) apply the
         # same requests / aborts / weight updates and then take the same engine step (reference: SGLang broadcasts
@@ -199,6 +201,8 @@ class EngineServer:
             return False, "lora_name" + (" and lora_path" if what == "load" else "") + " required"
         if self.tp_cmd_group is not None:
             return False, "adapters with tensor parallelism are not implemented"
+        if what == "load" and body["lora_name"] == self.model_name:
+            return False, f"{self.model_name!r} is the served model's name"
         done, result = threading.Event(), {}
         with self._lock:
             self._inbox.append(("adapter", (what, body, result), done))

@@ -188,3 +188,26 @@ def test_adapters_that_the_bank_cannot_hold_are_refused():
         assert not bank.names and not bank.scales.any() and not any(t.any() for layer in bank.layers for pair in layer.values() for t in pair)
         bank.load("a", sd, 4.0)
         assert bank.scales.tolist() == [0.5, 0.0]
+
+
+def test_no_adapter_takes_the_served_models_name(tmp_path):
+    from polyrl_b200.models.lora import export_peft_state_dict
+    from polyrl_b200.rollout.server import EngineServer
+
+    from .test_engine_requests_cpu import make_adapter
+
+    cfg, _, eng = make_engine(max_adapters=2)
+    sd = make_adapter(cfg, 8, 1)
+    torch.save(export_peft_state_dict(sd), tmp_path / "adapter_model.bin")
+    srv = EngineServer(eng, model_name="policy").start()
+    try:
+        code, got = post(f"http://{srv.endpoint}/load_lora_adapter", {"lora_name": "policy", "lora_path": str(tmp_path)})
+        assert code == 400 and "served model" in got["message"] and not eng.adapters.names
+        assert post(f"http://{srv.endpoint}/load_lora_adapter", {"lora_name": "other", "lora_path": str(tmp_path)})[0] == 200
+        with urllib.request.urlopen(f"http://{srv.endpoint}/v1/models", timeout=30) as r:
+            assert [d["id"] for d in json.loads(r.read())["data"]] == ["policy", "other"]
+        assert srv.adapter_of("policy") is None and srv.adapter_of("other") == "other"
+    finally:
+        srv.stop()
+    with pytest.raises(ValueError, match="served model"):
+        EngineServer(eng, model_name="other")

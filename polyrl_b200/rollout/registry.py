@@ -72,13 +72,31 @@ class NaiveRollout:
         h = tf.final_norm(self.cfg, self.head_w, last)
         return tf.logits_forward(self.cfg, self.head_w, self.embed_w, h).float()
 
+    def _rules(self, p: SamplingParams, reqs: list[Request]):
+        """The rules of ``p`` for every request, each with a slot of its own."""
+        from .rules import RequestRules, check_params
+
+        vocab = tf.lm_head_weight(self.cfg, self.head_w, self.embed_w).shape[0]
+        stops = set() if p.ignore_eos else {t for t in (self.cfg.eos_token_id, *p.stop_token_ids) if t is not None and t >= 0}
+        longest = max(self.max_model_len, max(len(r.prompt_ids) for r in reqs) + 1)
+        check_params(p, self.cfg.vocab_size, stops, longest)
+        rules = RequestRules(len(reqs), longest, vocab, self.device)
+        for slot, r in enumerate(reqs):
+            r.slot = slot
+            rules.set(slot, p, r.prompt_ids, len(r.prompt_ids), stops)
+        return rules
+
     @torch.no_grad()
     def generate(self, prompts: list[list[int]], params: SamplingParams | dict | None = None, on_finish=None):
         p = params if isinstance(params, SamplingParams) else SamplingParams.from_dict(params)
         groups = [[Request(f"n{i}_{j}", list(pr), p) for j in range(p.n)] for i, pr in enumerate(prompts)]
         live = [r for g in groups for r in g]
+        rules = self._rules(p, live) if p.has_rules and live else None
         while live:
             logits = self._next_logits([r.prompt_ids + r.output_ids for r in live])
+            if rules is not None:
+                slots = torch.tensor([r.slot for r in live], device=self.device)
+                rules.apply_to(logits, slots)
             if p.temperature > 0:
                 lp = torch.log_softmax(logits / p.temperature, -1)
                 tok = torch.multinomial(lp.exp().cpu(), 1, generator=self.gen).squeeze(1).to(lp.device)
@@ -86,6 +104,8 @@ class NaiveRollout:
                 lp = torch.log_softmax(logits, -1)
                 tok = lp.argmax(-1)
             sel = lp.gather(1, tok[:, None]).squeeze(1)
+            if rules is not None:
+                rules.append(slots, tok)
             nxt = []
             for r, t, l in zip(live, tok.tolist(), sel.tolist()):
                 r.output_ids.append(t)

@@ -111,3 +111,20 @@ def test_counts_that_cannot_be_are_refused():
             assert code == 400 and json.loads(got)["error"], (ids, n)
     finally:
         srv.stop()
+
+
+@pytest.mark.parametrize("name", ["naive", "hf"])
+def test_the_rollout_without_a_cache_has_the_same_rules(name):
+    """It is what the engine is compared with: greedy tokens and log-probs of all rules agree."""
+    from polyrl_b200.rollout.registry import get_rollout_cls
+
+    cfg, w, eng = make_engine()
+    plain = get_rollout_cls(name)(cfg, "cpu", max_model_len=128)
+    plain.set_weights(w.embed, w.layers, w.head)
+    prompts = [PROMPT, [4] * 20, [7, 300]]
+    for kw in RULES:
+        p = SamplingParams.from_dict({"max_new_tokens": LENGTH, "temperature": 0.0, **kw})
+        for a, b in zip(eng.generate(prompts, p), plain.generate(prompts, p)):
+            assert a[0].output_ids == b[0].output_ids and max(abs(x - y) for x, y in zip(a[0].logprobs, b[0].logprobs)) < 1e-4, kw
+    with pytest.raises(ValueError, match="repetition_penalty"):
+        plain.generate(prompts, {"repetition_penalty": 0.0})

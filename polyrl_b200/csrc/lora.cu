@@ -16,8 +16,9 @@
 //        leave their fp32 sums in shared memory and each adds up its share of the tile over distributed shared memory, in the order of the
 //        ranks: results do not depend on timing.  Bound by the stream of its large operand where its rows are contiguous (8191 rows, 48 columns: t from
 //        4096 columns 11 us, 5.9 TB/s; dt from 6144 19 us, 5.3 TB/s), by pieces of 128 bytes a row out of it where the sum runs over its rows (dA 20 us, 3.4
-//        TB/s; dB 25 us, 4.0 TB/s).  So dA and dB are one launch, whose CTAs fill the chip together: one after the other and together 52 and 39 us there,
-//        34 and 22 for 4099 x 6144 / 2048, 64 columns, 11.2 and 6.5 for 387 x 896 / 1152.
+//        TB/s; dB 25 us, 4.0 TB/s).  So dA and dB are one launch, whose CTAs fill the chip together: one after the other and together 53 and 40 us there,
+//        35 and 22 for 4099 x 6144 / 2048, 64 columns, 11.2 and 6.4 for 387 x 896 / 1152.  One cluster size serves both: where one product is alone enough for the
+//        chip and the other is not, that costs what the overlap gives, or more (2500 x 3584 / 37888, 32 columns: 50 and 54).
 // pack   A parts one below the other, B parts block-diagonal in the order of the projection's columns, ranks padded to 8 with zeros; a bias
 //        becomes one more column of B against a column of ones in t, which the forward product then adds for nothing.
 #include "gemm_sm100.cuh"

@@ -95,7 +95,7 @@ def _together(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Many rows: whether the adapters' part goes through the large product as further k-blocks, the low-rank values of all adapters side by
     side with a row's own kept (lora.cu).  That is LR (K + N) products a row for LR = adapters * parts * rank, whichever adapters the rows have;
     a pass of its own is bound by the array of N values a row that it leaves.  The line, 2000 LR values' worth of products for one of the array's, was
-    drawn before the pass of its own got faster; it is right within a tenth but for the last size below.  The call on the device with its plan made
+    drawn before the pass of its own got faster; it is right to about a tenth but for the last size below.  The call on the device with its plan made
     before (packing of ``b`` and the shared product are part of it), apart and together, rows, K, N, LR, us: 5003, 2048, 2048, 320: 68 and 59, with 768
     69 and 76; 2900, 3584, 37888 (gate and up), 1024: 1020 and 938; 3000, 896, 9728 (gate and up), 512: 284 and 225; 700, 4096, 6144, 384: 53 and 41,
     8000 rows 353 and 370; 4000, 14336, 4096, 512, which the line puts apart: 485 and 422."""

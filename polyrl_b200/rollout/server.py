@@ -2,7 +2,8 @@
 manager and the reference trainer use (reference patches:
 rlboost/sglang/patches.py:390-566, rlboost/verl_stream/workers/rollout/sglang_rollout/sglang_http_async_engine.py:155-299):
 
-  POST /generate (stream => SSE ``data: {...}`` cumulative chunks, ``data: [DONE]``), GET /health_generate,
+  POST /generate (stream => SSE ``data: {...}`` cumulative chunks, ``data: [DONE]``; ``continued_tokens``: how many of each prompt's
+  last tokens are output of the same request; 400, or an event with ``error``, for what the engine refuses), GET /health_generate,
   GET /get_server_info (``#running_req`` / ``#queue_req`` / ``last_gen_throughput``), POST /abort_request,
   POST /shutdown, POST /update_weights_from_agent, POST /update_weights_from_tensor,
   POST /release_memory_occupation, /resume_memory_occupation, /flush_cache.

@@ -71,7 +71,7 @@ class VLLMRollout:
                   stop_token_ids=[self.cfg.eos_token_id, *self.cfg.extra_eos_token_ids, *p.stop_token_ids])
         if p.has_rules:
             kw |= dict(repetition_penalty=p.repetition_penalty, presence_penalty=p.presence_penalty, frequency_penalty=p.frequency_penalty,
-                       min_tokens=p.min_new_tokens, logit_bias=p.logit_bias or None,
+                       min_tokens=min(p.min_new_tokens, p.max_new_tokens), logit_bias=p.logit_bias or None,
                        allowed_token_ids=None if p.allowed_token_ids is None else list(p.allowed_token_ids))
         try:
             from vllm import SamplingParams as VSP

@@ -128,3 +128,16 @@ def test_the_rollout_without_a_cache_has_the_same_rules(name):
             assert a[0].output_ids == b[0].output_ids and max(abs(x - y) for x, y in zip(a[0].logprobs, b[0].logprobs)) < 1e-4, kw
     with pytest.raises(ValueError, match="repetition_penalty"):
         plain.generate(prompts, {"repetition_penalty": 0.0})
+
+
+def test_least_lengths_reach_the_library_engine_up_to_the_limit(monkeypatch):
+    """The native engine holds stop tokens back to the last token at most; the library refuses a least length beyond the limit."""
+    import sys
+
+    from polyrl_b200.rollout.vllm_adapter import VLLMRollout
+
+    monkeypatch.setitem(sys.modules, "vllm", None)                    # parameters stay a dict
+    roll = VLLMRollout(make_engine()[0], "cpu", llm=object())
+    for least, most, want in ((5, 9, 5), (9, 9, 9), (10 ** 6, 9, 9)):
+        kw = roll._sampling_params(SamplingParams(max_new_tokens=most, min_new_tokens=least))
+        assert (kw["min_tokens"], kw["max_tokens"]) == (want, most)

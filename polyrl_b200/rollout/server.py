@@ -385,6 +385,8 @@ class EngineServer:
                         raise
                 self._flush_streams()
             else:
+                if cmds:                                   # an abort may have ended the last requests: no step passes their events on
+                    self._flush_streams()
                 time.sleep(0.002)
         if self.tp_cmd_group is not None:
             _tp_broadcast(self.tp_cmd_group, [("shutdown", None)], 0)

@@ -211,3 +211,30 @@ def test_no_adapter_takes_the_served_models_name(tmp_path):
         srv.stop()
     with pytest.raises(ValueError, match="served model"):
         EngineServer(eng, model_name="other")
+
+
+@pytest.mark.parametrize("path,body", [("/abort_request", {"abort_all": True}), ("/release_memory_occupation", {})])
+def test_an_abort_of_everything_answers_everything(path, body):
+    """Nothing is left for the engine to do after it, and no step comes that would pass the last events on."""
+    import threading
+    import time
+
+    from polyrl_b200.rollout.server import EngineServer
+
+    eng = make_engine()[2]
+    real = eng.step
+    eng.step = lambda: (time.sleep(0.02), real())[1]
+    srv = EngineServer(eng).start()
+    try:
+        out = [None] * 3
+        req = {"input_ids": [5, 6], "sampling_params": {"max_new_tokens": 120, "temperature": 0.0, "ignore_eos": True}}
+        ts = [threading.Thread(target=lambda i=i: out.__setitem__(i, post(f"http://{srv.endpoint}/generate", req))) for i in range(3)]
+        [t.start() for t in ts]
+        until = time.time() + 30
+        while sum(len(r.output_ids) > 2 for r in list(eng.running.values())) < 3 and time.time() < until:
+            time.sleep(0.01)
+        assert post(f"http://{srv.endpoint}{path}", body)[0] == 200
+        [t.join(30) for t in ts]
+        assert all(o is not None and o[0] == 200 and o[1]["meta_info"]["finish_reason"]["type"] == "abort" and 2 < len(o[1]["output_ids"]) < 120 for o in out)
+    finally:
+        srv.stop()

@@ -215,11 +215,11 @@ class EngineServer:
         ``RolloutEngine.add_request``, one number a prompt."""
         q: queue.Queue = queue.Queue()
         key = f"g{id(q)}"
-        if self._broken is not None:
-            self._decline(q, len(prompts), {"type": "abort", "message": self._broken})
-            return key, q
         with self._lock:
-            self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter, continued), None))
+            if self._broken is None:
+                self._inbox.append(("generate", (key, prompts, sp, q, mm, adapter, continued), None))
+            else:
+                self._decline(q, len(prompts), {"type": "abort", "message": self._broken})
         return key, q
 
     @staticmethod
@@ -317,6 +317,9 @@ class EngineServer:
                 try:
                     if kind == "generate":
                         key, prompts, sp, q, mm, adapter, continued = payload
+                        if self._broken is not None:                        # since it was queued
+                            self._decline(q, len(prompts), {"type": "abort", "message": self._broken})
+                            continue
                         rids = []
                         for _ in prompts:
                             self._rid += 1
@@ -380,7 +383,14 @@ class EngineServer:
                 except Exception as e:
                     self._step_failed(e)
                     if self.tp_cmd_group is not None:      # the other ranks have failed as well, or are a step ahead: no lock-step to go on with
-                        self._broken = self._broken or f"engine failed: {e!r}"
+                        with self._lock:
+                            self._broken = self._broken or f"engine failed: {e!r}"
+                            cmds, self._inbox = self._inbox, []
+                        for kind, payload, done in cmds:
+                            if kind == "generate":
+                                self._decline(payload[3], len(payload[1]), {"type": "abort", "message": self._broken})
+                            if done is not None:
+                                done.set()
                         self._flush_streams()
                         raise
                 self._flush_streams()

@@ -1,5 +1,6 @@
 """What a request may bring at its limits, and what becomes of an engine and its server when a step refuses something."""
 import json
+import queue
 import urllib.error
 import urllib.request
 
@@ -135,6 +136,10 @@ def test_an_engine_that_cannot_go_on_says_so():
         for _ in range(2):
             code, got = post(f"http://{srv.endpoint}/generate", {"input_ids": [5, 6], "sampling_params": {"max_new_tokens": 4}})
             assert code == 200 and got["meta_info"]["finish_reason"]["type"] == "abort" and got["output_ids"] == []
+        q = queue.Queue()                                       # one that was queued while the step failed
+        with srv._lock:
+            srv._inbox.append(("generate", ("key", [[5], [6]], SamplingParams(), q, None, None, None), None))
+        assert [q.get(timeout=30)[1]["meta_info"]["finish_reason"]["type"] for _ in range(2)] == ["abort"] * 2
         with pytest.raises(urllib.error.HTTPError) as e:
             urllib.request.urlopen(f"http://{srv.endpoint}/health_generate", timeout=30)
         assert e.value.code == 503
